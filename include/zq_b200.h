@@ -284,6 +284,81 @@ void zq_moe_ep_shutdown(zq_ctx *ctx);
 int zq_moe_forward_ep(zq_ctx *ctx, const zq_moe_experts *local_experts, const zq_weight *shared_gate, const zq_weight *shared_up, const zq_weight *shared_down, const void *dev_x, int x_dtype, size_t m, size_t m_cap,
                       const uint32_t *dev_ids, const float *dev_weights, size_t top_k, void *dev_y, int y_dtype, const void *dev_residual, zq_error *err);
 
+/* ---- decoding drafted tokens from a paged cache ----
+ * One step of a decoder that drafts tokens: every sequence of a batch brings `rows` rows, row 0 its newest known token, the others
+ * drafted tokens that hang below it as a tree (parents[row] < row; a chain has parents[row] = row - 1, a single row is plain decode).
+ * Their keys and values are written to the cache at positions context_len + row; attention reads the cache, shows each row its
+ * context and the drafted rows above it; after the choice of the path that is kept, its cache rows are moved together.
+ * `dev_draft_lens` (int32 [batch], or NULL: `rows` each) gives how many rows of a sequence there are; the rest of its rows is
+ * padding, neither read nor written unless said below.  Device-side values out of their range (a page, a length, a parent, a token)
+ * are skipped and reported by the next zq_ctx_sync.  None of these calls uses the context's buffers: they may be captured first, replayed
+ * after any other call and issued on several streams (zq_ctx_set_stream between them); zq_tree_attention takes its scratch in
+ * stream order, in a graph as an allocation node. */
+
+/* A cache of pages: K and V pages hold [page_size, heads, head_dim] values, 16 bits each; position p of sequence s is row
+ * p % page_size of page dev_blocks[s * max_blocks + p / page_size].  page_size is a power of two, head_dim a multiple of 8 up to 256,
+ * dev_k and dev_v 16-byte aligned, the strides (in values, the same for K and V) multiples of 8. */
+typedef struct zq_kv_cache {
+    void *dev_k, *dev_v;
+    int dtype; /* ZQ_F16 or ZQ_BF16 */
+    size_t pages, page_size, heads, head_dim, page_stride;
+    size_t layers, layer_stride; /* of zq_cache_keep_path; the other calls take the layer that dev_k and dev_v point to */
+    const int32_t *dev_blocks;   /* [batch, max_blocks] */
+    size_t batch, max_blocks;
+    const int32_t *dev_context_lens; /* [batch]: positions in front of the rows of this step */
+} zq_kv_cache;
+
+/* Angles per position of the rotary_dim / 2 pairs, on the host: base^(-2 i / rotary_dim), divided by `pair_factors[i]` where given (the
+ * rope_freqs tensor of a GGUF file), scaled for contexts longer than a model was trained on: ZQ_ROPE_SCALE_LINEAR divides by `factor`,
+ * ZQ_ROPE_SCALE_YARN divides pairs that turn less than `beta_slow` times over `original_context` positions by `factor`, keeps those
+ * that turn more than `beta_fast` times, and blends linearly in the turns between; *out_factor is what cos and sin are multiplied by
+ * (0.1 ln(factor) + 1 for YARN with factor > 1, else 1). */
+enum { ZQ_ROPE_SCALE_NONE = 0, ZQ_ROPE_SCALE_LINEAR = 1, ZQ_ROPE_SCALE_YARN = 2 };
+int zq_rope_frequencies(size_t rotary_dim, double base, int scaling, double factor, double original_context, double beta_slow, double beta_fast, const float *pair_factors, float *out_inv_freq, float *out_factor, zq_error *err);
+
+/* zq_rope_qk with a position of its own for every row and angles from frequencies instead of tables: angle = dev_positions[row] *
+ * dev_inv_freq[pair] (int32, f32) without rounding the product, cos and sin multiplied by `factor`; `inverse` turns back (and multiplies
+ * by the factor again: the transposed map).  Rows of q lie q_stride values apart, [q_heads, head_dim] each; q_out is dense
+ * [rows, q_heads * head_dim] and may be dev_q itself where that is dense; the same for k (dev_k may be NULL).  A row of negative position is
+ * copied as it is.  All three dtypes; computed in f32 and rounded once. */
+int zq_rope_rows(zq_ctx *ctx, const void *dev_q, size_t q_heads, size_t q_stride, const void *dev_k, size_t k_heads, size_t k_stride, int dtype, size_t rows, size_t head_dim, size_t rotary_dim, int layout, int placement,
+                 const int32_t *dev_positions, const float *dev_inv_freq, float factor, int inverse, void *dev_q_out, void *dev_k_out, zq_error *err);
+/* The same with the keys, rotated, and the values written to the cache (dtype, heads and head_dim are the cache's) instead of to a
+ * tensor: rows_per_seq rows for each of the cache's sequences, row i of sequence s at position context_len[s] + i.  Rows from draft_len
+ * on and rows of negative position are not written to the cache (their q is copied as zq_rope_rows does it). */
+int zq_rope_append(zq_ctx *ctx, const void *dev_q, size_t q_heads, size_t q_stride, const void *dev_k, size_t k_stride, const void *dev_v, size_t v_stride, size_t rows_per_seq, const zq_kv_cache *cache, const int32_t *dev_draft_lens,
+                   size_t rotary_dim, int layout, int placement, const int32_t *dev_positions, const float *dev_inv_freq, float factor, void *dev_q_out, zq_error *err);
+
+/* Positions and mask of drafted trees.  dev_parents: int32 [batch, rows], or [rows] for all sequences where parents_shared; a root has
+ * parent -1.  positions[s][i] = context_len[s] + number of rows above row i; bit j % 64 of dev_mask[s][i][j / 64] (ceil(rows / 64) words a
+ * row) is set where j is i or above it.  Padding rows, and rows below a parent out of range, get position -1 and an empty mask.
+ * rows <= 1024. */
+int zq_draft_tree(zq_ctx *ctx, const int32_t *dev_parents, int parents_shared, size_t batch, size_t rows, const int32_t *dev_context_lens, const int32_t *dev_draft_lens, int32_t *dev_positions, uint64_t *dev_mask, zq_error *err);
+
+/* softmax(scale q k^T) v over the cache, q_heads / heads query heads for each of the cache's.  q: rows of [q_heads, head_dim] values of
+ * the cache's dtype, q_stride values apart, `rows` (<= 1024) for each of the cache's sequences.  Row i sees the positions below
+ * context_len and the drafted rows that its mask shows (dev_mask as zq_draft_tree writes it; NULL: the rows up to itself).
+ * dev_out: dense, as many rows; rows that see nothing and padding rows become zero.  What a row does not see does not reach
+ * it, infinities and NaN included.  Sums and softmax in f32; the weights are rounded to the cache's type for the second product. */
+int zq_tree_attention(zq_ctx *ctx, const void *dev_q, size_t q_heads, size_t q_stride, size_t rows, const zq_kv_cache *cache, const uint64_t *dev_mask, const int32_t *dev_draft_lens, float scale, void *dev_out, zq_error *err);
+
+/* Which drafted tokens are kept, from given random numbers, and the token behind them.  dev_logits [batch, rows, vocab]: row i holds the
+ * target's logits behind token i (dev_tokens, int32 [batch, rows]; row 0 is known already).  The walk begins at row 0, p =
+ * softmax(logits / temperature[s]), and tries the rows that hang below its row in ascending order: child c of token t is kept if
+ * accept_u[s][c] q(t) < p(t); else p becomes max(p - q, 0) over its sum and the next child is tried.  q is
+ * softmax(draft_logits / temperature) of the same row, from which the children were drawn independently, or, with dev_draft_logits NULL, 1
+ * for the child's token (children that were chosen).  Where no child is kept, the walk ends: dev_token[s] is the first
+ * token at which the running sum of p exceeds sample_u[s], dev_path[s] holds the rows of the walk, padded with -1, dev_accepted[s] their
+ * number (row 0 included).  Random numbers are f32 of [0, 1).  temperature 0 (f32 [batch]): the most likely token, ties to the lowest, and the
+ * children that equal it.  A row with a NaN, or without a finite largest logit, ends the walk with token -1; a sequence without rows gets
+ * 0 and -1.  All three dtypes; sums and comparisons in 64 bits. */
+int zq_verify_draft(zq_ctx *ctx, const void *dev_logits, const void *dev_draft_logits, int dtype, size_t batch, size_t rows, size_t vocab, const int32_t *dev_tokens, const int32_t *dev_parents, int parents_shared, const float *dev_accept_u,
+                    const float *dev_sample_u, const float *dev_temperature, const int32_t *dev_draft_lens, int32_t *dev_path, int32_t *dev_accepted, int32_t *dev_token, zq_error *err);
+
+/* Moves the kept rows together: for k below accepted[s], the K and V rows at context_len[s] + path[s][k] go to context_len[s] + k, in all
+ * cache->layers layers.  dev_path: int32 [batch, rows] as zq_verify_draft writes it (path[s][k] >= k). */
+int zq_cache_keep_path(zq_ctx *ctx, const zq_kv_cache *cache, const int32_t *dev_path, size_t rows, const int32_t *dev_accepted, zq_error *err);
+
 #ifdef __cplusplus
 }
 #endif

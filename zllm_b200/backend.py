@@ -238,6 +238,49 @@ class B200Context:
         self._native.rope(self._h, query, key, num_heads, num_kv_heads, rotary_dim, position, cos, sin, interleaved, suffix)
         return query, key
 
+    # ---- drafted tokens over a paged cache
+    def draft_tree(self, parents: torch.Tensor, context_lens: torch.Tensor, draft_lens: Optional[torch.Tensor] = None):
+        """``(positions [sequences, rows] int32, mask [sequences, rows, ceil(rows / 64)] int64)`` of drafted trees: ``parents``
+        (int32, [sequences, rows] or [rows] for all) holds for each row the row above it, -1 for the root; ``context_lens``
+        (int32) the cache positions in front; ``draft_lens`` (int32 or None: all) how many rows a sequence has."""
+        positions, mask = self._native.draft_tree(self._h, self.device.index, parents, context_lens, draft_lens)
+        return positions, mask
+
+    def rope_rows(self, query: torch.Tensor, key: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, suffix: bool = False, factor: float = 1.0, inverse: bool = False):
+        """``(query, key)`` turned, [..., heads, head_dim] each (rows may lie apart): row r by ``positions[r] * inv_freq`` (int32, f32;
+        ``rope_frequencies``), all of a head or its first (``suffix``: last) ``2 * len(inv_freq)`` values.  Rows of negative position
+        are copied as they are; ``inverse`` turns back."""
+        q, k = self._native.rope_rows(self._h, self.device.index, query, key, positions, inv_freq, interleaved, suffix, factor, inverse)
+        return q, k
+
+    def rope_append(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, positions: torch.Tensor,
+                    inv_freq: torch.Tensor, draft_lens: Optional[torch.Tensor] = None, interleaved: bool = False, suffix: bool = False, factor: float = 1.0) -> torch.Tensor:
+        """The query turned, as ``rope_rows``; the key, turned, and the value written to the cache: row i of sequence s at position
+        ``context_lens[s] + i``, but no row from ``draft_lens[s]`` on and none of negative position.  ``k_pages`` / ``v_pages``: [pages,
+        page_size, heads, head_dim], f16 or bf16; ``block_table``: int32 [sequences, blocks]."""
+        return self._native.rope_append(self._h, self.device.index, query, key, value, k_pages, v_pages, block_table, context_lens, positions, inv_freq, draft_lens, interleaved, suffix, factor)
+
+    def tree_attention(self, query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, mask: Optional[torch.Tensor] = None,
+                       draft_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+        """Attention of ``query`` [sequences, rows, q_heads, head_dim] over the cache, which holds the rows' own keys and values
+        already (``rope_append``): each row sees its context and the drafted rows that ``mask`` (``draft_tree``; None: a chain) shows.
+        Rows from ``draft_lens`` on, and rows that see nothing, come out as zero.  ``scale`` None: 1 / sqrt(head_dim)."""
+        return self._native.tree_attention(self._h, self.device.index, query, k_pages, v_pages, block_table, context_lens, mask, draft_lens, scale)
+
+    def verify_draft(self, logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, accept_u: torch.Tensor, sample_u: torch.Tensor, temperature: torch.Tensor, draft_logits: Optional[torch.Tensor] = None,
+                     draft_lens: Optional[torch.Tensor] = None):
+        """``(path [sequences, rows], accepted [sequences], token [sequences])`` int32: the rows that are kept of a drafted tree (row 0
+        first, -1 behind the last), how many, and the token drawn behind them.  ``logits`` [sequences, rows, vocabulary]: the
+        target's behind each row; ``tokens`` / ``accept_u`` [sequences, rows], ``sample_u`` / ``temperature`` [sequences]; ``draft_logits``: the
+        distributions that each row's children were drawn from, or None where they were chosen."""
+        path, accepted, token = self._native.verify_draft(self._h, self.device.index, logits, tokens, parents, accept_u, sample_u, temperature, draft_logits, draft_lens)
+        return path, accepted, token
+
+    def cache_keep_path(self, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor) -> None:
+        """Moves the cache rows of a kept path together, in place: row ``context_lens[s] + path[s][k]`` to ``context_lens[s] + k`` for k
+        below ``accepted[s]``; pages [layers, pages, page_size, heads, head_dim], or one layer's."""
+        self._native.cache_keep_path(self._h, self.device.index, k_pages, v_pages, block_table, context_lens, path, accepted)
+
     def gated_linear(self, x: torch.Tensor, gate: Weight, up: Weight, out_dtype=None) -> torch.Tensor:
         return self._native.gated(self._h, x, gate, up, None, out_dtype, None)
 
@@ -330,6 +373,19 @@ class GgufFile:
         out = C.c_void_p()
         ffi.call("zq_gguf_load_matrix_slice", ctx.handle, self.handle, name.encode(), int(index), C.byref(out))
         return Weight(ctx, out)
+
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: int = ffi.ROPE_SCALE_NONE, factor: float = 1.0, original_context: float = 0.0, beta_slow: float = 1.0, beta_fast: float = 32.0,
+                     pair_factors: Optional[Sequence[float]] = None, device=None):
+    """``(inv_freq f32 [rotary_dim / 2], factor)`` for ``rope_rows`` / ``rope_append`` (``zq_rope_frequencies``): plain, linear or
+    YaRN scaling, ``pair_factors`` as a GGUF file's rope_freqs tensor holds them."""
+    half = max(rotary_dim // 2, 1)
+    out, by = (C.c_float * half)(), C.c_float()
+    if pair_factors is not None and len(pair_factors) != half:
+        raise ffi.ZqFailure(1, f"rope_frequencies: {len(pair_factors)} pair factors for {half} pairs")
+    given = (C.c_float * half)(*[float(v) for v in pair_factors]) if pair_factors is not None else None
+    ffi.call("zq_rope_frequencies", rotary_dim, float(base), int(scaling), float(factor), float(original_context), float(beta_slow), float(beta_fast), given, out, C.byref(by))
+    return torch.tensor(list(out), dtype=torch.float32, device=device), float(by.value)
 
 
 def lm_head_argmax(ctx: B200Context, head: Weight, x: torch.Tensor) -> torch.Tensor:

@@ -1,0 +1,483 @@
+// Attention of drafted rows over a paged cache.
+//
+//     out_i = sum_j w_ij v_j / sum_j w_ij,   w_ij = exp(scale q_i k_j - top_i)
+//
+// One pass over the keys with a running maximum and sum per row (the sums so far are multiplied down when the maximum rises).  The rows of
+// all query heads that share a head of the cache go through the matrix instructions together (m16n8k16), so that the cache is read once for them: bytes
+// bound while rows * group stays below about 100.
+//
+// Work: an item is a (sequence, cache head, tile of rows); its keys are cut into units.  The units of all items, in one line, are
+// dealt to the CTAs (one per SM) in equal shares, so that one long sequence or many unequal ones keep all SMs at work; an item cut by a border is
+// left in parts (largest score, sum of weights and weighted sums per row, f32) which a second, small kernel joins in ascending order:
+// results do not depend on timing.  The lengths are on the device, so each CTA finds its share from them itself.
+//
+// A CTA has key groups (its warps of one group share keys, each with 16 rows of its own; the groups take the keys in turn), every one with a ring
+// of its own that cp.async fills: no barrier between groups until the item ends.  Shared memory rows are swizzled by 16-byte chunks so that
+// ldmatrix reads without conflicts.
+#include "zq_attn.cuh"
+
+namespace zq {
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool there) {
+    const int n = there ? 16 : 0;  // 0: sixteen zero bytes, nothing is read
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool BF16> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        mma_16816(d, a[0], a[1], a[2], a[3], b0, b1);
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if (BF16) {
+        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t *>(&v);
+    }
+    __half2 v = __floats2half2_rn(lo, hi);
+    return h2_as_u32(v);
+}
+template <bool BF16> __device__ __forceinline__ float unpack16(uint32_t bits) { return BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits)); }
+// Values of a word whose exponent is all ones (infinities, NaN) become zero; true if there was one.
+template <bool BF16> __device__ __forceinline__ bool drop_nonfinite(uint32_t &w) {
+    const uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+    const bool lo = (w & e) == e, hi = (w >> 16 & e) == e;
+    if (lo) w &= 0xffff0000u;
+    if (hi) w &= 0x0000ffffu;
+    return lo || hi;
+}
+
+// Shape of the kernel for a head of up to D values and WM warps of 16 rows.
+template <int D, int WM> struct AttnShape {
+    static constexpr int kGroups = WM == 4 ? 2 : 4;              // key groups of a CTA
+    static constexpr int kWarps = WM * kGroups, kThreads = 32 * kWarps;
+    static constexpr int kKeys = D <= 128 ? 32 : 16;             // keys per group and step
+    static constexpr int kUnit = kKeys * kGroups;                // keys per unit of work
+    static constexpr int kPitch = D <= 64 ? 128 : D <= 128 ? 256 : 512;  // bytes of a key in shared memory: chunks are swizzled in eights
+    static constexpr int kStage = 2 * kKeys * kPitch;
+    static constexpr int kStages = (200 << 10) / (kGroups * kStage) > 6 ? 6 : (200 << 10) / (kGroups * kStage);
+    static constexpr int kRows = 16 * WM;
+    static constexpr int kRing = kGroups * kStages * kStage;
+    static constexpr int kMerge = kGroups * kRows * (D + 2) * 4;  // the groups' sums at the end of an item, in place of the ring
+    static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + 1024;
+    static constexpr int kPartFloats = kRows * (D + 2);
+    static_assert(kStages >= 2 && kSmem <= 227 << 10, "ring");
+};
+
+struct Share {
+    int64_t first, last, total;  // units of this CTA; of all
+    int ctas;                    // with a share
+    int seq;                     // of the first unit
+    int64_t seq_first;           // first unit of that sequence
+};
+
+__device__ __forceinline__ int units_of(const SeqLen &s, int unit) {
+    return s.rows ? (s.context + s.rows + unit - 1) / unit : 1;  // a sequence without rows has its output set to zero by its one unit
+}
+
+// The CTA's share of the units.  Every thread adds up some sequences, the thread whose sequences hold the first unit looks for it.
+template <int kThreads> __device__ Share find_share(const AttnArgs &a, int unit, uint8_t *scratch) {
+    int64_t *s_sum = reinterpret_cast<int64_t *>(scratch);  // [kThreads / 32 + 3]
+    const int tid = threadIdx.x, lane = tid & 31, per = (a.batch + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+    const int64_t items = (int64_t)a.c.heads * a.tiles;
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += units_of(seq_len(a, b), unit) * items;
+    int64_t incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 31) s_sum[tid / 32] = incl;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < tid / 32) before += s_sum[w];
+        total += s_sum[w];
+    }
+    int64_t at = before + incl - mine;
+    Share s;
+    s.total = total;
+    s.ctas = (int)min((int64_t)gridDim.x, total);
+    const int64_t c = blockIdx.x;
+    s.first = c < s.ctas ? c * total / s.ctas : total;
+    s.last = c < s.ctas ? (c + 1) * total / s.ctas : total;
+    int64_t *s_found = s_sum + kThreads / 32;
+    if (s.first >= at && s.first < at + mine) {
+        for (int b = b0; b < b1; ++b) {
+            const int64_t n = units_of(seq_len(a, b), unit) * items;
+            if (s.first < at + n) {
+                s_found[0] = b;
+                s_found[1] = at;
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+    s.seq = s.first < total ? (int)s_found[0] : 0;
+    s.seq_first = s.first < total ? s_found[1] : 0;
+    __syncthreads();
+    return s;
+}
+
+template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<D, WM>::kThreads, 1) tree_attention_kernel(const AttnArgs a) {
+    using S = AttnShape<D, WM>;
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp / WM, wm = warp % WM, gtid = tid - group * WM * 32;
+    const Share share = find_share<S::kThreads>(a, S::kUnit, smem + S::kSmem - 1024);
+    if (tid == 0) a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (share.first >= share.last) return;
+    const int d = a.c.head_dim, chunks = d / 8;
+    uint8_t *ring = smem + group * S::kStages * S::kStage;
+    const uint32_t ring_u32 = smem_u32(ring);
+    int seq = share.seq;
+    int64_t seq_first = share.seq_first;
+    SeqLen len = seq_len(a, seq);
+    int units = units_of(len, S::kUnit);
+
+    for (int64_t u = share.first; u < share.last;) {
+        while (u >= seq_first + (int64_t)units * a.c.heads * a.tiles) {
+            seq_first += (int64_t)units * a.c.heads * a.tiles;
+            len = seq_len(a, ++seq);
+            units = units_of(len, S::kUnit);
+        }
+        const int item = (int)((u - seq_first) / units);
+        const int64_t item_first = seq_first + (int64_t)item * units;
+        const int head = item / a.tiles, tile = item % a.tiles;
+        const int ua = (int)(u - item_first), ub = (int)min((int64_t)units, share.last - item_first);
+        const int steps = ub - ua, keys = len.rows ? len.context + len.rows : 0;
+        const int row0 = tile * S::kRows + wm * 16, n_rows = len.rows * a.group;
+
+        // ---- the ring: step s of this share holds keys [(ua + s) * kUnit + group * kKeys, + kKeys)
+        const int64_t head_off = (int64_t)head * d;
+        auto page_of = [&](int s) -> int64_t {  // first value of this lane's key of step s, -1 where there is none
+            const int key = (ua + s) * S::kUnit + group * S::kKeys + lane % S::kKeys;
+            if (s >= steps || key >= keys) return -1;
+            const int64_t r = cache_row(a.c, seq, key);
+            if (r < 0) atomicMax(a.status, (uint32_t)kStatusBadIndex);
+            return r < 0 ? -1 : r + head_off;
+        };
+        auto fill = [&](int s, int64_t mine) {
+            if (s < steps) {
+                const uint32_t base = ring_u32 + (s % S::kStages) * S::kStage;
+                constexpr int kChunks = D / 8, kCopies = S::kKeys * kChunks;
+#pragma unroll
+                for (int i = 0; i < (kCopies + WM * 32 - 1) / (WM * 32); ++i) {
+                    const int idx = i * WM * 32 + gtid, key = idx / kChunks, chunk = idx % kChunks;
+                    const int64_t at = __shfl_sync(0xffffffffu, mine, key % S::kKeys);
+                    if (kCopies % (WM * 32) && idx >= kCopies) continue;
+                    const bool there = at >= 0 && chunk < chunks;
+                    const int64_t off = there ? 2 * at + 16 * chunk : 0;
+                    const uint32_t dst = base + key * S::kPitch + ((chunk ^ (key & 7)) << 4);
+                    cp_async16(dst, a.c.k + off, there);
+                    cp_async16(dst + S::kKeys * S::kPitch, a.c.v + off, there);
+                }
+            }
+            cp_commit();
+        };
+        int64_t ahead[1];
+#pragma unroll
+        for (int s = 0; s < S::kStages - 1; ++s) fill(s, page_of(s));
+        ahead[0] = page_of(S::kStages - 1);
+
+        // ---- the rows of this warp
+        constexpr int kK = D / 16;
+        uint32_t qf[kK][4];
+        const int r_lo = row0 + lane / 4, r_hi = r_lo + 8;
+        {
+            auto q_at = [&](int r, int col) -> uint32_t {
+                if (r >= n_rows || col >= d) return 0u;
+                const uint8_t *p = a.q + 2 * (((int64_t)seq * a.rows + r / a.group) * a.q_stride + (int64_t)(head * a.group + r % a.group) * d + col);
+                return *reinterpret_cast<const uint32_t *>(p);
+            };
+#pragma unroll
+            for (int k = 0; k < kK; ++k) {
+                const int col = 16 * k + 2 * (lane & 3);
+                qf[k][0] = q_at(r_lo, col);
+                qf[k][1] = q_at(r_hi, col);
+                qf[k][2] = q_at(r_lo, col + 8);
+                qf[k][3] = q_at(r_hi, col + 8);
+            }
+        }
+        const int i_lo = r_lo / a.group, i_hi = r_hi / a.group;
+        float o[D / 8][4];
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+
+        for (int s = 0; s < steps; ++s) {
+            cp_wait<S::kStages - 2>();
+            if (WM == 1) __syncwarp();
+            else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(WM * 32) : "memory");
+            fill(s + S::kStages - 1, ahead[0]);
+            ahead[0] = page_of(s + S::kStages);
+            const uint32_t kb = ring_u32 + (s % S::kStages) * S::kStage, vb = kb + S::kKeys * S::kPitch;
+            const int key0 = (ua + s) * S::kUnit + group * S::kKeys;
+
+            constexpr int kN = S::kKeys / 8;
+            float sc[kN][4];
+#pragma unroll
+            for (int n = 0; n < kN; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+            const int mi = lane >> 3, mr = lane & 7;
+#pragma unroll
+            for (int k = 0; k < kK; ++k) {
+#pragma unroll
+                for (int n = 0; n < kN; n += 2) {
+                    const int key = n * 8 + (mi >> 1) * 8 + mr, chunk = 2 * k + (mi & 1);
+                    uint32_t b[4];
+                    ldmatrix_x4(b, kb + key * S::kPitch + ((chunk ^ (key & 7)) << 4));
+                    mma16<BF16>(sc[n], qf[k], b[0], b[1]);
+                    mma16<BF16>(sc[n + 1], qf[k], b[2], b[3]);
+                }
+            }
+            const bool masked = key0 + S::kKeys > len.context;  // drafted rows among the keys, or the end
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[n][e] *= a.scale;
+            }
+            if (masked) {
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + n * 8 + 2 * (lane & 3) + (e & 1), i = e < 2 ? i_lo : i_hi;
+                        if (key >= len.context && (key >= keys || i >= len.rows || !sees(a, seq, i, key - len.context))) sc[n][e] = -INFINITY;
+                    }
+                }
+            }
+            float base[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float m = top[h];
+#pragma unroll
+                for (int n = 0; n < kN; ++n) m = fmaxf(m, fmaxf(sc[n][2 * h], sc[n][2 * h + 1]));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                base[h] = m == -INFINITY ? 0.f : m;
+                const float down = exp2f(top[h] - base[h]);
+                if (__any_sync(0xffffffffu, top[h] != m)) {
+#pragma unroll
+                    for (int n = 0; n < D / 8; ++n) {
+                        o[n][2 * h] *= down;
+                        o[n][2 * h + 1] *= down;
+                    }
+                    sum[h] *= down;
+                }
+                top[h] = m;
+            }
+            uint32_t pf[S::kKeys / 16][4];
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[e] = exp2f(sc[n][e] - base[e >> 1]);
+                    sum[e >> 1] += p[e];
+                }
+                pf[n / 2][(n & 1) * 2] = pack2<BF16>(p[0], p[1]);
+                pf[n / 2][(n & 1) * 2 + 1] = pack2<BF16>(p[2], p[3]);
+            }
+            if (!masked) {
+#pragma unroll
+                for (int k = 0; k < S::kKeys / 16; ++k) {
+#pragma unroll
+                    for (int n = 0; n < D / 8; n += 2) {
+                        const int key = k * 16 + (mi & 1) * 8 + mr, chunk = n + (mi >> 1);
+                        uint32_t b[4];
+                        ldmatrix_x4_trans(b, vb + key * S::kPitch + ((chunk ^ (key & 7)) << 4));
+                        mma16<BF16>(o[n], pf[k], b[0], b[1]);
+                        mma16<BF16>(o[n + 1], pf[k], b[2], b[3]);
+                    }
+                }
+            } else {
+                // a weight of zero times an infinity of a row that is not seen would be a NaN: such values leave the product, and come
+                // back for the rows that see them
+                bool dropped = false;
+#pragma unroll
+                for (int k = 0; k < S::kKeys / 16; ++k) {
+#pragma unroll
+                    for (int n = 0; n < D / 8; n += 2) {
+                        const int key = k * 16 + (mi & 1) * 8 + mr, chunk = n + (mi >> 1);
+                        uint32_t b[4];
+                        ldmatrix_x4_trans(b, vb + key * S::kPitch + ((chunk ^ (key & 7)) << 4));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dropped |= drop_nonfinite<BF16>(b[e]);
+                        mma16<BF16>(o[n], pf[k], b[0], b[1]);
+                        mma16<BF16>(o[n + 1], pf[k], b[2], b[3]);
+                    }
+                }
+                if (__any_sync(0xffffffffu, dropped)) {
+                    const uint8_t *v = ring + (s % S::kStages) * S::kStage + S::kKeys * S::kPitch;
+                    for (int j = 0; j < S::kKeys; ++j) {
+                        const int key = key0 + j;
+                        if (key >= keys) break;
+                        const bool lo = i_lo < len.rows && (key < len.context || sees(a, seq, i_lo, key - len.context));
+                        const bool hi = i_hi < len.rows && (key < len.context || sees(a, seq, i_hi, key - len.context));
+#pragma unroll
+                        for (int n = 0; n < D / 8; ++n) {
+                            uint32_t w = *reinterpret_cast<const uint32_t *>(v + j * S::kPitch + ((n ^ (j & 7)) << 4) + 4 * (lane & 3));
+                            uint32_t finite = w;
+                            if (!drop_nonfinite<BF16>(finite)) continue;
+                            w &= (finite & 0xffffu) == (w & 0xffffu) ? 0xffff0000u : 0xffffffffu;  // the values that were left out, zero beside them
+                            w &= (finite >> 16) == (w >> 16) ? 0x0000ffffu : 0xffffffffu;
+                            const float x = unpack16<BF16>(w & 0xffffu), y = unpack16<BF16>(w >> 16);
+                            if (lo) o[n][0] += x, o[n][1] += y;
+                            if (hi) o[n][2] += x, o[n][3] += y;
+                        }
+                    }
+                }
+            }
+        }
+        cp_wait<0>();
+        __syncthreads();
+
+        // ---- the groups' sums meet in shared memory
+        float *m_o = reinterpret_cast<float *>(smem), *m_top = m_o + S::kGroups * S::kRows * D, *m_sum = m_top + S::kGroups * S::kRows;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+            sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+            const int r = group * S::kRows + wm * 16 + lane / 4 + 8 * h;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2 *>(m_o + r * D + n * 8 + 2 * (lane & 3)) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+            if ((lane & 3) == 0) {
+                m_top[r] = top[h];
+                m_sum[r] = sum[h];
+            }
+        }
+        __syncthreads();
+        const bool whole = ua == 0 && ub == units;
+        float *part = a.parts + ((size_t)blockIdx.x * 2 + (ua == 0 ? 1 : 0)) * S::kPartFloats;
+        for (int idx = tid; idx < S::kRows * (D / 2); idx += S::kThreads) {
+            const int r = idx / (D / 2), col = 2 * (idx % (D / 2)), row = tile * S::kRows + r, i = row / a.group;
+            float m = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < S::kGroups; ++g) m = fmaxf(m, m_top[g * S::kRows + r]);
+            const float b = m == -INFINITY ? 0.f : m;
+            float x = 0.f, y = 0.f, l = 0.f;
+#pragma unroll
+            for (int g = 0; g < S::kGroups; ++g) {
+                const float w = exp2f(m_top[g * S::kRows + r] - b);
+                const float2 v = *reinterpret_cast<const float2 *>(m_o + (g * S::kRows + r) * D + col);
+                x += w * v.x;
+                y += w * v.y;
+                l += w * m_sum[g * S::kRows + r];
+            }
+            if (whole) {
+                if (i < a.rows && col < d) {
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    const bool none = l == 0.f || i >= len.rows;
+                    *reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col)) = none ? 0u : pack2<BF16>(x * inv, y * inv);
+                }
+            } else {
+                *reinterpret_cast<float2 *>(part + r * D + col) = make_float2(x, y);
+                if (col == 0) {
+                    part[S::kRows * D + r] = m;
+                    part[S::kRows * D + S::kRows + r] = l;
+                }
+            }
+        }
+        if (tid == 0 && ua == 0 && ub < units) {
+            const int64_t end = item_first + units;  // the CTA of the item's last unit
+            const int last = (int)((end * share.ctas - 1) / share.total);
+            a.info[blockIdx.x] = make_int4(seq, item, last - (int)blockIdx.x + 1, len.rows);
+        }
+        __syncthreads();
+        u = item_first + ub;
+    }
+}
+
+// Joins the parts of the item that starts in CTA blockIdx.x's share, in the order of its keys.
+template <bool BF16> __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, int rows, int d_pad) {
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    const int4 info = a.info[blockIdx.x];
+    if (info.z == 0) return;
+    const int seq = info.x, head = info.y / a.tiles, tile = info.y % a.tiles, pieces = info.z, d = a.c.head_dim;
+    const size_t floats = (size_t)rows * (d_pad + 2);
+    auto part = [&](int p) { return a.parts + ((size_t)(blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * floats; };
+    for (int idx = threadIdx.x; idx < rows * (d / 2); idx += blockDim.x) {
+        const int r = idx / (d / 2), col = 2 * (idx % (d / 2)), row = tile * rows + r, i = row / a.group;
+        if (i >= a.rows) continue;
+        float m = -INFINITY;
+        for (int p = 0; p < pieces; ++p) m = fmaxf(m, part(p)[rows * d_pad + r]);
+        const float b = m == -INFINITY ? 0.f : m;
+        float x = 0.f, y = 0.f, l = 0.f;
+        for (int p = 0; p < pieces; ++p) {
+            const float *f = part(p);
+            const float w = exp2f(f[rows * d_pad + r] - b);
+            const float2 v = *reinterpret_cast<const float2 *>(f + r * d_pad + col);
+            x += w * v.x;
+            y += w * v.y;
+            l += w * f[rows * d_pad + rows + r];
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col)) = l == 0.f || i >= info.w ? 0u : pack2<BF16>(x * inv, y * inv);
+    }
+}
+
+template <int D, int WM, bool BF16> static int launch_shape(zq_ctx *ctx, AttnArgs &a, zq_error *err) {
+    using S = AttnShape<D, WM>;
+    a.tiles = (a.rows * a.group + S::kRows - 1) / S::kRows;
+    const size_t ctas = (size_t)ctx->sm_count, bytes = ctas * 2 * S::kPartFloats * sizeof(float);
+    LaunchScratch scratch;
+    int rc = scratch.take(ctx, bytes + ctas * sizeof(int4), err);
+    if (rc) return rc;
+    a.parts = static_cast<float *>(scratch.p);
+    a.info = reinterpret_cast<int4 *>(static_cast<uint8_t *>(scratch.p) + bytes);
+    ZQ_CUDA_CHECK(cudaFuncSetAttribute(tree_attention_kernel<D, WM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), err);
+    rc = launch_pdl(ctx, tree_attention_kernel<D, WM, BF16>, dim3((unsigned)ctas), dim3(S::kThreads), S::kSmem, err, a);
+    if (rc) return rc;
+    return launch_pdl(ctx, attention_join_kernel<BF16>, dim3((unsigned)ctas), dim3(256), 0, err, a, S::kRows, D);
+}
+template <int D, bool BF16> static int launch_rows(zq_ctx *ctx, AttnArgs &a, zq_error *err) {
+    const int rows = a.rows * a.group;
+    return rows <= 16 ? launch_shape<D, 1, BF16>(ctx, a, err) : rows <= 32 ? launch_shape<D, 2, BF16>(ctx, a, err) : launch_shape<D, 4, BF16>(ctx, a, err);
+}
+template <bool BF16> static int launch_dim(zq_ctx *ctx, AttnArgs &a, zq_error *err) {
+    const int d = a.c.head_dim;
+    return d <= 64 ? launch_rows<64, BF16>(ctx, a, err) : d <= 96 ? launch_rows<96, BF16>(ctx, a, err) : d <= 128 ? launch_rows<128, BF16>(ctx, a, err) : d <= 192 ? launch_rows<192, BF16>(ctx, a, err) : launch_rows<256, BF16>(ctx, a, err);
+}
+
+}  // namespace zq
+
+using namespace zq;
+
+extern "C" int zq_tree_attention(zq_ctx *ctx, const void *dev_q, size_t q_heads, size_t q_stride, size_t rows, const zq_kv_cache *cache, const uint64_t *dev_mask, const int32_t *dev_draft_lens, float scale, void *dev_out, zq_error *err) {
+    if (!ctx || !dev_q || !dev_out) return set_error(err, ZQ_ERR_ARG, "zq_tree_attention: null argument");
+    AttnArgs a = {};
+    int rc = cache_args("zq_tree_attention", cache, a.c, err);
+    if (rc) return rc;
+    if (rows == 0 || rows > kMaxDraftRows) return set_error(err, ZQ_ERR_SHAPE, "zq_tree_attention: %zu rows of a sequence (1..%d)", rows, kMaxDraftRows);
+    if (q_heads == 0 || q_heads % cache->heads || q_heads > 65536) return set_error(err, ZQ_ERR_SHAPE, "zq_tree_attention: %zu query heads for %zu heads of the cache", q_heads, cache->heads);
+    if (q_stride < q_heads * cache->head_dim || q_stride % 2 || q_stride > (size_t)INT32_MAX) return set_error(err, ZQ_ERR_SHAPE, "zq_tree_attention: rows of q %zu values apart for %zu values", q_stride, q_heads * cache->head_dim);
+    if (!(scale > 0) || scale > 1e30f) return set_error(err, ZQ_ERR_ARG, "zq_tree_attention: scale %g (positive)", (double)scale);
+    if ((reinterpret_cast<uintptr_t>(dev_q) | reinterpret_cast<uintptr_t>(dev_out)) & 3) return set_error(err, ZQ_ERR_ARG, "zq_tree_attention: q or the output is not 4-byte aligned");
+    if ((uint64_t)cache->max_blocks * cache->page_size > (uint64_t)INT32_MAX - 4096) return set_error(err, ZQ_ERR_SHAPE, "zq_tree_attention: %zu blocks of %zu positions", cache->max_blocks, cache->page_size);
+    if ((rc = use_device(ctx, err))) return rc;
+    a.q = static_cast<const uint8_t *>(dev_q);
+    a.mask = reinterpret_cast<const unsigned long long *>(dev_mask);
+    a.lens = dev_draft_lens;
+    a.out = static_cast<uint8_t *>(dev_out);
+    a.q_stride = (int64_t)q_stride;
+    a.batch = (int)cache->batch;
+    a.rows = (int)rows;
+    a.group = (int)(q_heads / cache->heads);
+    a.words = (int)((rows + 63) / 64);
+    a.scale = scale * kLog2e;
+    a.status = ctx->status_dev;
+    return cache->dtype == ZQ_BF16 ? launch_dim<true>(ctx, a, err) : launch_dim<false>(ctx, a, err);
+}

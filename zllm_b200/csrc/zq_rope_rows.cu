@@ -1,0 +1,291 @@
+// Rotary positions of single rows, from frequencies: the rows of a drafted tree, batches of sequences of unequal length, contexts
+// longer than a table; optionally with the keys and values written to a paged cache.
+//
+//     (re, im) <- factor * (re cos t - im sin t, im cos t + re sin t),   t = position * inv_freq[pair]
+//
+// t reaches 1e6 and more, where an f32 product is off by tenths of a radian; here the product is exact (24 + 24 bits in f64), its whole
+// turns come off in f64, and the rest of it, at most half a turn, goes through sincospif: 1e-7 at any position.
+//
+// Bound by memory, each value read and written once.  A CTA takes as many rows as fill its 256 threads; a thread asks for its first two
+// vectors before the angles are computed, so that these hide under the loads, and the sines of a row are shared by all its heads.
+#include <cmath>
+
+#include "zq_draft.cuh"
+
+namespace zq {
+
+struct RopeRowsArgs {
+    const uint8_t *q, *k, *v;
+    uint8_t *q_out, *k_out;
+    const int32_t *positions, *lens;
+    const float *inv_freq;
+    CacheArgs cache;  // cache.k null: keys go to k_out
+    int64_t q_stride, k_stride, v_stride;  // values between rows
+    int64_t rows;
+    int rows_per_seq, q_heads, k_heads, v_heads, head_dim, rotary, start, interleaved, inverse;
+    float factor;
+    int threads;        // of one row
+    int pair_items, copy_items, copy_all;  // work items of a head: that turn pairs, outside the turned part; of a head of V
+    uint32_t *status;
+};
+
+template <class T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <class T, int N> struct alignas(sizeof(T) * N) Vec {
+    T v[N];
+};
+
+// VEC values per access: 16 bytes where head, turned part, strides and addresses allow, else one value (a pair, where pairs lie side by side).
+// An item is VEC pairs (two vectors, of which an interleaved one is the other's neighbour) or 2 VEC values that are copied.
+template <class T, int VEC> __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeRowsArgs a) {
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    extern __shared__ float2 s_turn[];
+    using V = Vec<T, VEC>;
+    const int lane = threadIdx.x % a.threads, slot = threadIdx.x / a.threads, half = a.rotary / 2;
+    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / a.threads) + slot;
+    const bool here = row < a.rows;
+    const int position = here ? a.positions[row] : -1;
+    int64_t keep = -1;  // the cache row, or -1
+    if (a.cache.k && here && position >= 0) {
+        const int seq = (int)(row / a.rows_per_seq), i = (int)(row % a.rows_per_seq);
+        if (i < draft_len(a.lens, seq, a.rows_per_seq, a.status)) {
+            const int start = a.cache.lens[seq];
+            keep = start < 0 ? -1 : cache_row(a.cache, seq, (int64_t)start + i);
+            if (keep < 0) atomicMax(a.status, (uint32_t)kStatusBadIndex);
+        }
+    }
+    const int head_items = a.pair_items + a.copy_items, turned = (a.q_heads + a.k_heads) * head_items, items = here ? turned + a.v_heads * a.copy_all : 0;
+    const bool to_cache = a.cache.k != nullptr;
+
+    struct Item {
+        const T *src;
+        T *dst;
+        int first, second, pair;  // offsets of the two vectors from the head's start (second: head_dim where there is none); their first pair, or -1
+    };
+    auto item_of = [&](int i) {
+        Item it;
+        if (i >= turned) {
+            const int head = (i - turned) / a.copy_all, c = (i - turned) % a.copy_all;
+            it.src = reinterpret_cast<const T *>(a.v) + row * a.v_stride + head * a.head_dim;
+            it.dst = keep < 0 ? nullptr : reinterpret_cast<T *>(a.cache.v) + keep + head * a.head_dim;
+            it.first = 2 * VEC * c;
+            it.second = it.first + VEC;
+            it.pair = -1;
+            return it;
+        }
+        const int head = i / head_items, c = i % head_items;
+        if (head < a.q_heads) {
+            it.src = reinterpret_cast<const T *>(a.q) + row * a.q_stride + head * a.head_dim;
+            it.dst = reinterpret_cast<T *>(a.q_out) + (row * a.q_heads + head) * a.head_dim;
+        } else {
+            const int h = head - a.q_heads;
+            it.src = reinterpret_cast<const T *>(a.k) + row * a.k_stride + h * a.head_dim;
+            it.dst = !to_cache ? reinterpret_cast<T *>(a.k_out) + (row * a.k_heads + h) * a.head_dim : keep < 0 ? nullptr : reinterpret_cast<T *>(a.cache.k) + keep + h * a.head_dim;
+        }
+        if (c < a.pair_items) {
+            it.pair = c * VEC;
+            it.first = a.start + (a.interleaved ? 2 * VEC * c : VEC * c);
+            it.second = a.interleaved ? it.first + VEC : it.first + half;
+        } else {
+            it.pair = -1;
+            const int at = 2 * VEC * (c - a.pair_items);
+            it.first = a.start ? at : a.rotary + at;  // in front of the turned part or behind it
+            it.second = it.first + VEC < (a.start ? a.start : a.head_dim) ? it.first + VEC : a.head_dim;
+        }
+        return it;
+    };
+    auto load = [&](const Item &it, V &x, V &y) {
+        x = *reinterpret_cast<const V *>(it.src + it.first);
+        if (it.second < a.head_dim) y = *reinterpret_cast<const V *>(it.src + it.second);
+    };
+
+    V x, y;
+    Item it{};
+    if (lane < items) {
+        it = item_of(lane);
+        load(it, x, y);
+    }
+    float2 *turn = s_turn + slot * half;
+    if (here && position >= 0) {
+        for (int p = lane; p < half; p += a.threads) {
+            double t = (double)position * (double)a.inv_freq[p] * 0.15915494309189533577;  // in turns
+            t -= rint(t);
+            float s, c;
+            sincospif(2.f * (float)t, &s, &c);
+            turn[p] = make_float2(c * a.factor, a.inverse ? -s * a.factor : s * a.factor);
+        }
+    }
+    __syncthreads();
+    for (int i = lane; i < items; i += a.threads) {
+        if (i != lane) {
+            it = item_of(i);
+            load(it, x, y);
+        }
+        if (it.pair >= 0 && position >= 0) {
+            if (a.interleaved && VEC > 1) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    V &w = 2 * j < VEC ? x : y;
+                    const int at = 2 * j % VEC;
+                    const float2 cs = turn[it.pair + j];
+                    const float re = to_f32(w.v[at]), im = to_f32(w.v[(at + 1) % VEC]);
+                    w.v[at] = from_f32<T>(re * cs.x - im * cs.y);
+                    w.v[(at + 1) % VEC] = from_f32<T>(im * cs.x + re * cs.y);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float2 cs = turn[it.pair + j];
+                    const float re = to_f32(x.v[j]), im = to_f32(y.v[j]);
+                    x.v[j] = from_f32<T>(re * cs.x - im * cs.y);
+                    y.v[j] = from_f32<T>(im * cs.x + re * cs.y);
+                }
+            }
+        }
+        if (it.dst) {
+            *reinterpret_cast<V *>(it.dst + it.first) = x;
+            if (it.second < a.head_dim) *reinterpret_cast<V *>(it.dst + it.second) = y;
+        }
+    }
+}
+
+static int rope_checks(const char *who, zq_ctx *ctx, const RopeRowsArgs &a, int dtype, size_t q_heads, size_t q_stride, size_t k_heads, size_t k_stride, size_t v_stride, size_t rows, size_t head_dim, size_t rotary, int layout, int placement,
+                       float factor, zq_error *err) {
+    if (!ctx || !a.q || !a.q_out || !a.positions || !a.inv_freq) return set_error(err, ZQ_ERR_ARG, "%s: null argument", who);
+    if (dtype != ZQ_F32 && dtype != ZQ_F16 && dtype != ZQ_BF16) return set_error(err, ZQ_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    if ((layout != ZQ_ROPE_SPLIT_HALF && layout != ZQ_ROPE_INTERLEAVED) || (placement != ZQ_ROPE_PREFIX && placement != ZQ_ROPE_SUFFIX)) return set_error(err, ZQ_ERR_ARG, "%s: unknown layout %d or placement %d", who, layout, placement);
+    if (q_heads == 0 || rotary == 0 || rotary % 2 || head_dim == 0 || head_dim > 4096) return set_error(err, ZQ_ERR_SHAPE, "%s: heads=%zu head_dim=%zu rotary=%zu (rotary must be even and positive)", who, q_heads, head_dim, rotary);
+    if (rotary > head_dim) return set_error(err, ZQ_ERR_SHAPE, "%s: rotary=%zu exceeds head_dim=%zu", who, rotary, head_dim);
+    if (rows == 0 || rows > (size_t)INT32_MAX) return set_error(err, ZQ_ERR_SHAPE, "%s: %zu rows", who, rows);
+    if (q_heads > 65536 || k_heads > 65536) return set_error(err, ZQ_ERR_SHAPE, "%s: shape too large", who);
+    if (q_stride < q_heads * head_dim || (a.k && k_stride < k_heads * head_dim) || (a.v && v_stride < k_heads * head_dim)) return set_error(err, ZQ_ERR_SHAPE, "%s: rows overlap (strides %zu, %zu, %zu)", who, q_stride, k_stride, v_stride);
+    if (q_stride > (size_t)INT32_MAX || k_stride > (size_t)INT32_MAX || v_stride > (size_t)INT32_MAX) return set_error(err, ZQ_ERR_SHAPE, "%s: shape too large", who);
+    if ((a.q_out == a.q && q_stride != q_heads * head_dim) || (a.k && a.k_out == a.k && k_stride != k_heads * head_dim)) return set_error(err, ZQ_ERR_ARG, "%s: in place only where the rows are dense", who);
+    if (!std::isfinite(factor)) return set_error(err, ZQ_ERR_ARG, "%s: the factor is not finite", who);
+    return ZQ_OK;
+}
+
+template <class T> static int launch_rope_rows(zq_ctx *ctx, RopeRowsArgs &a, zq_error *err) {
+    constexpr int kWide = 16 / sizeof(T);
+    // pairs of an item lie in two vectors: half a turned part (split halves) or two neighbours (interleaved)
+    const int half = a.rotary / 2, rest = a.head_dim - a.rotary;
+    bool wide = a.head_dim % kWide == 0 && a.rotary % (2 * kWide) == 0 && a.start % kWide == 0 && a.q_stride % kWide == 0 && (!a.k || a.k_stride % kWide == 0) && (!a.v || a.v_stride % kWide == 0);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k_out);
+    wide = wide && (at & 15) == 0;
+    const int vec = wide ? kWide : 1;
+    a.pair_items = half / vec;
+    a.copy_items = (rest + 2 * vec - 1) / (2 * vec);
+    a.copy_all = (a.head_dim + 2 * vec - 1) / (2 * vec);
+    const int64_t items = (int64_t)(a.q_heads + a.k_heads) * (a.pair_items + a.copy_items) + (int64_t)a.v_heads * a.copy_all;
+    a.threads = 32;
+    while (a.threads < 256 && a.threads < items) a.threads *= 2;
+    const int per_cta = 256 / a.threads;
+    const dim3 grid((unsigned)((a.rows + per_cta - 1) / per_cta));
+    const size_t smem = (size_t)per_cta * half * sizeof(float2);
+    return wide ? launch_pdl(ctx, rope_rows_kernel<T, kWide>, grid, dim3(256), smem, err, a) : launch_pdl(ctx, rope_rows_kernel<T, 1>, grid, dim3(256), smem, err, a);
+}
+
+static int launch_rope_rows(zq_ctx *ctx, RopeRowsArgs &a, int dtype, zq_error *err) {
+    int rc = use_device(ctx, err);
+    if (rc) return rc;
+    a.status = ctx->status_dev;
+    return dtype == ZQ_F32 ? launch_rope_rows<float>(ctx, a, err) : dtype == ZQ_F16 ? launch_rope_rows<__half>(ctx, a, err) : launch_rope_rows<__nv_bfloat16>(ctx, a, err);
+}
+
+}  // namespace zq
+
+using namespace zq;
+
+extern "C" int zq_rope_frequencies(size_t rotary_dim, double base, int scaling, double factor, double original_context, double beta_slow, double beta_fast, const float *pair_factors, float *out_inv_freq, float *out_factor, zq_error *err) {
+    if (!out_inv_freq || !out_factor) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: null argument");
+    if (rotary_dim == 0 || rotary_dim % 2 || rotary_dim > 4096) return set_error(err, ZQ_ERR_SHAPE, "zq_rope_frequencies: rotary=%zu (rotary must be even and positive)", rotary_dim);
+    if (scaling != ZQ_ROPE_SCALE_NONE && scaling != ZQ_ROPE_SCALE_LINEAR && scaling != ZQ_ROPE_SCALE_YARN) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: unknown scaling %d", scaling);
+    if (!(base > 0) || !std::isfinite(base)) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: base %g", base);
+    if (scaling != ZQ_ROPE_SCALE_NONE && (!(factor > 0) || !std::isfinite(factor))) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: factor %g", factor);
+    if (scaling == ZQ_ROPE_SCALE_YARN && (!(original_context > 0) || !std::isfinite(original_context) || !(beta_fast > beta_slow) || !std::isfinite(beta_fast) || !std::isfinite(beta_slow)))
+        return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: original context %g, turns %g to %g", original_context, beta_slow, beta_fast);
+    const size_t half = rotary_dim / 2;
+    for (size_t i = 0; i < half; ++i) {
+        double f = std::pow(base, -(double)i / (double)half);
+        if (pair_factors) {
+            if (!(pair_factors[i] > 0)) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: pair factor %g", (double)pair_factors[i]);
+            f /= (double)pair_factors[i];
+        }
+        if (scaling == ZQ_ROPE_SCALE_LINEAR) f /= factor;
+        if (scaling == ZQ_ROPE_SCALE_YARN) {
+            const double turns = original_context * f / 6.28318530717958647692;
+            double keep = (turns - beta_slow) / (beta_fast - beta_slow);
+            keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
+            f = f * keep + f / factor * (1 - keep);
+        }
+        out_inv_freq[i] = (float)f;
+    }
+    *out_factor = scaling == ZQ_ROPE_SCALE_YARN && factor > 1 ? (float)(0.1 * std::log(factor) + 1.0) : 1.f;
+    return ZQ_OK;
+}
+
+extern "C" int zq_rope_rows(zq_ctx *ctx, const void *dev_q, size_t q_heads, size_t q_stride, const void *dev_k, size_t k_heads, size_t k_stride, int dtype, size_t rows, size_t head_dim, size_t rotary_dim, int layout, int placement,
+                            const int32_t *dev_positions, const float *dev_inv_freq, float factor, int inverse, void *dev_q_out, void *dev_k_out, zq_error *err) {
+    RopeRowsArgs a = {};
+    a.q = static_cast<const uint8_t *>(dev_q);
+    a.k = static_cast<const uint8_t *>(dev_k);
+    a.q_out = static_cast<uint8_t *>(dev_q_out);
+    a.k_out = static_cast<uint8_t *>(dev_k_out);
+    a.positions = dev_positions;
+    a.inv_freq = dev_inv_freq;
+    int rc = rope_checks("zq_rope_rows", ctx, a, dtype, q_heads, q_stride, k_heads, k_stride, 0, rows, head_dim, rotary_dim, layout, placement, factor, err);
+    if (rc) return rc;
+    if (dev_k && (!dev_k_out || k_heads == 0)) return set_error(err, ZQ_ERR_ARG, "zq_rope_rows: key given without heads or without an output");
+    a.q_stride = (int64_t)q_stride;
+    a.k_stride = (int64_t)k_stride;
+    a.rows = (int64_t)rows;
+    a.rows_per_seq = 1;
+    a.q_heads = (int)q_heads;
+    a.k_heads = dev_k ? (int)k_heads : 0;
+    a.head_dim = (int)head_dim;
+    a.rotary = (int)rotary_dim;
+    a.start = placement == ZQ_ROPE_SUFFIX ? (int)(head_dim - rotary_dim) : 0;
+    a.interleaved = layout == ZQ_ROPE_INTERLEAVED;
+    a.inverse = inverse;
+    a.factor = factor;
+    return launch_rope_rows(ctx, a, dtype, err);
+}
+
+extern "C" int zq_rope_append(zq_ctx *ctx, const void *dev_q, size_t q_heads, size_t q_stride, const void *dev_k, size_t k_stride, const void *dev_v, size_t v_stride, size_t rows_per_seq, const zq_kv_cache *cache, const int32_t *dev_draft_lens,
+                              size_t rotary_dim, int layout, int placement, const int32_t *dev_positions, const float *dev_inv_freq, float factor, void *dev_q_out, zq_error *err) {
+    if (!dev_k || !dev_v) return set_error(err, ZQ_ERR_ARG, "zq_rope_append: null argument");
+    RopeRowsArgs a = {};
+    int rc = cache_args("zq_rope_append", cache, a.cache, err);
+    if (rc) return rc;
+    a.q = static_cast<const uint8_t *>(dev_q);
+    a.k = static_cast<const uint8_t *>(dev_k);
+    a.v = static_cast<const uint8_t *>(dev_v);
+    a.q_out = static_cast<uint8_t *>(dev_q_out);
+    a.positions = dev_positions;
+    a.lens = dev_draft_lens;
+    a.inv_freq = dev_inv_freq;
+    if (rows_per_seq == 0 || rows_per_seq > (size_t(1) << 20)) return set_error(err, ZQ_ERR_SHAPE, "zq_rope_append: %zu rows of a sequence", rows_per_seq);
+    rc = rope_checks("zq_rope_append", ctx, a, cache->dtype, q_heads, q_stride, cache->heads, k_stride, v_stride, rows_per_seq * cache->batch, cache->head_dim, rotary_dim, layout, placement, factor, err);
+    if (rc) return rc;
+    a.q_stride = (int64_t)q_stride;
+    a.k_stride = (int64_t)k_stride;
+    a.v_stride = (int64_t)v_stride;
+    a.rows = (int64_t)(rows_per_seq * cache->batch);
+    a.rows_per_seq = (int)rows_per_seq;
+    a.q_heads = (int)q_heads;
+    a.k_heads = a.v_heads = (int)cache->heads;
+    a.head_dim = (int)cache->head_dim;
+    a.rotary = (int)rotary_dim;
+    a.start = placement == ZQ_ROPE_SUFFIX ? (int)(cache->head_dim - rotary_dim) : 0;
+    a.interleaved = layout == ZQ_ROPE_INTERLEAVED;
+    a.factor = factor;
+    return launch_rope_rows(ctx, a, cache->dtype, err);
+}

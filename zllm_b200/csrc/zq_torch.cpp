@@ -17,6 +17,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <vector>
 
 #include "../../include/zq_b200.h"
@@ -139,7 +140,7 @@ template <class Fn> PyObject *guarded(Fn fn) {
 template <class Tensors> PyObject *wrap_list(Tensors &ys) {
     PyObject *out = PyList_New((Py_ssize_t)ys.size());
     if (!out) throw PyError();
-    for (size_t i = 0; i < ys.size(); ++i) PyList_SET_ITEM(out, (Py_ssize_t)i, THPVariable_Wrap(std::move(ys[i])));
+    for (size_t i = 0; i < ys.size(); ++i) PyList_SET_ITEM(out, (Py_ssize_t)i, THPVariable_Wrap(std::move(ys[i])));  // None for one that was never made
     return out;
 }
 // The items of a sequence for the time of a call.
@@ -426,6 +427,281 @@ PyObject *py_linear_host_batch(PyObject *, PyObject *const *a, Py_ssize_t) {
     });
 }
 
+// ---- drafted tokens over a paged cache.  Tensors of these operators are checked for their device too: (ctx, device index, ...).
+int device_of(PyObject *o) {
+    const long d = PyLong_AsLong(o);
+    if (d == -1 && PyErr_Occurred()) throw PyError();
+    return (int)d;
+}
+at::Tensor on_device(PyObject *o, int device, const char *what) {
+    at::Tensor t = tensor_of(o);
+    if (!t.is_cuda() || t.get_device() != device) fail(4, std::string(what) + " is not on the context's device cuda:" + std::to_string(device));
+    return t;
+}
+std::string sizes_of(const at::Tensor &t) {
+    std::string s = "[";
+    for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+    return s + "]";
+}
+// A tensor of plain values: its type and how many it holds.
+at::Tensor values(PyObject *o, int device, const char *what, at::ScalarType type, int64_t count) {
+    at::Tensor t = on_device(o, device, what);
+    if (t.scalar_type() != type) type_error(std::string(what) + " is " + dtype_name(type) + ", not " + dtype_name(t.scalar_type()));
+    if (t.numel() != count) fail(1, std::string(what) + " of shape " + sizes_of(t) + ": " + std::to_string(count) + " values are needed");
+    return contiguous(t);
+}
+// Rows of [heads, head_dim] values at one distance: the tensor itself, or a dense copy where its strides are others.
+struct Rows {
+    at::Tensor t;
+    int64_t rows, heads, dim, stride;
+};
+Rows rows_3d(PyObject *o, int device, const char *what) {
+    Rows r{on_device(o, device, what), 1, 0, 0, 0};
+    if (r.t.dim() < 3) fail(1, std::string(what) + " of shape " + sizes_of(r.t) + ": [..., heads, head_dim] is needed");
+    const int64_t n = r.t.dim();
+    r.heads = r.t.size(n - 2);
+    r.dim = r.t.size(n - 1);
+    for (int64_t i = 0; i < n - 2; ++i) r.rows *= r.t.size(i);
+    if (r.rows == 0 || r.heads == 0 || r.dim == 0) fail(1, std::string(what) + " of shape " + sizes_of(r.t) + " is empty");
+    bool one = (r.dim == 1 || r.t.stride(n - 1) == 1) && (r.heads == 1 || r.t.stride(n - 2) == r.dim);
+    int64_t step = 0, inner = 1;  // the leading dimensions as one
+    for (int64_t i = n - 3; i >= 0 && one; --i) {
+        if (r.t.size(i) == 1) continue;
+        if (!step) step = r.t.stride(i);
+        else one = r.t.stride(i) == step * inner;
+        inner *= r.t.size(i);
+    }
+    if (!step) step = r.heads * r.dim;
+    if (!one || step < r.heads * r.dim) {
+        r.t = contiguous(r.t);
+        step = r.heads * r.dim;
+    }
+    r.stride = step;
+    return r;
+}
+struct Cache {
+    at::Tensor k, v, blocks, lens;
+    zq_kv_cache c;
+};
+Cache cache_of(PyObject *k, PyObject *v, PyObject *blocks, PyObject *lens, int device, bool layers) {
+    Cache s;
+    s.k = on_device(k, device, "k_pages");
+    s.v = on_device(v, device, "v_pages");
+    const int64_t n = s.k.dim();
+    if (n != 4 && !(layers && n == 5)) fail(1, "k_pages of shape " + sizes_of(s.k) + ": [pages, page_size, heads, head_dim] is needed" + (layers ? ", or that behind a dimension of layers" : ""));
+    if (s.k.scalar_type() != s.v.scalar_type()) type_error("k_pages is " + dtype_name(s.k.scalar_type()) + " and v_pages " + dtype_name(s.v.scalar_type()));
+    if (s.k.sizes() != s.v.sizes() || s.k.strides() != s.v.strides()) fail(1, "k_pages and v_pages differ in shape or strides: " + sizes_of(s.k) + ", " + sizes_of(s.v));
+    if (s.k.numel() == 0) fail(1, "k_pages of shape " + sizes_of(s.k) + " is empty");
+    const int64_t heads = s.k.size(n - 2), dim = s.k.size(n - 1), size = s.k.size(n - 3);
+    if ((dim > 1 && s.k.stride(n - 1) != 1) || (heads > 1 && s.k.stride(n - 2) != dim) || (size > 1 && s.k.stride(n - 3) != heads * dim)) fail(1, "a page of the cache is not dense");
+    s.blocks = on_device(blocks, device, "block_table");
+    if (s.blocks.scalar_type() != at::kInt) type_error("block_table is torch.int32, not " + dtype_name(s.blocks.scalar_type()));
+    if (s.blocks.dim() != 2 || s.blocks.numel() == 0) fail(1, "block_table of shape " + sizes_of(s.blocks) + ": [sequences, blocks] is needed");
+    s.blocks = contiguous(s.blocks);
+    s.lens = values(lens, device, "context_lens", at::kInt, s.blocks.size(0));
+    const int64_t pages = s.k.size(n - 4), page = size * heads * dim, page_stride = pages > 1 ? s.k.stride(n - 4) : page;
+    if (page_stride < page) fail(1, "the pages of the cache overlap");
+    const int64_t n_layers = n == 5 ? s.k.size(0) : 1;
+    const int64_t layer_stride = n_layers > 1 ? s.k.stride(0) : 0;
+    if (n_layers > 1 && layer_stride < page) fail(1, "the layers of the cache overlap");
+    s.c = {s.k.data_ptr(), s.v.data_ptr(), zq_dtype(s.k.scalar_type()), (size_t)pages, (size_t)size, (size_t)heads, (size_t)dim, (size_t)page_stride, (size_t)n_layers, (size_t)layer_stride,
+           s.blocks.data_ptr<int>(), (size_t)s.blocks.size(0), (size_t)s.blocks.size(1), s.lens.data_ptr<int>()};
+    return s;
+}
+at::Tensor optional_lens(PyObject *o, int device, const char *what, int64_t count) { return is_none(o) ? at::Tensor() : values(o, device, what, at::kInt, count); }
+const int32_t *ints_or_null(const at::Tensor &t) { return t.defined() ? t.data_ptr<int>() : nullptr; }
+bool truth(PyObject *o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw PyError();
+    return v != 0;
+}
+double number(PyObject *o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw PyError();
+    return v;
+}
+at::Tensor empty_like_sizes(const at::Tensor &like, at::IntArrayRef sizes, at::ScalarType t) { return at::empty(sizes, like.options().dtype(t).memory_format(at::MemoryFormat::Contiguous)); }
+
+// parents: [rows] for all sequences or [sequences, rows]
+struct Parents {
+    at::Tensor t;
+    bool shared;
+};
+Parents parents_of(PyObject *o, int device, int64_t batch, int64_t rows) {
+    at::Tensor t = on_device(o, device, "parents");
+    if (t.scalar_type() != at::kInt) type_error("parents is torch.int32, not " + dtype_name(t.scalar_type()));
+    const bool shared = t.dim() == 1;
+    if ((t.dim() != 1 && t.dim() != 2) || t.size(-1) != rows || (!shared && t.size(0) != batch)) fail(1, "parents of shape " + sizes_of(t) + " for " + std::to_string(batch) + " sequences of " + std::to_string(rows) + " rows");
+    return {contiguous(t), shared};
+}
+
+// draft_tree(ctx, device, parents, context_lens, draft_lens | None) -> positions, mask
+PyObject *py_draft_tree(PyObject *, PyObject *const *a, Py_ssize_t) {
+    return guarded([&]() -> PyObject * {
+        zq_ctx *ctx = ctx_of(a[0]);
+        const int device = device_of(a[1]);
+        const at::Tensor lens = on_device(a[3], device, "context_lens"), given = on_device(a[2], device, "parents");
+        const int64_t batch = lens.numel(), rows = given.dim() ? given.size(-1) : 0;
+        const Parents parents = parents_of(a[2], device, batch, rows);
+        const at::Tensor context = values(a[3], device, "context_lens", at::kInt, batch), drafted = optional_lens(a[4], device, "draft_lens", batch);
+        std::vector<at::Tensor> out(2);
+        zq_error err;
+        int rc;
+        {
+            NoGil g;
+            out[0] = empty_like_sizes(context, {batch, rows}, at::kInt);
+            out[1] = empty_like_sizes(context, {batch, rows, (rows + 63) / 64}, at::kLong);
+            rc = zq_draft_tree(ctx, parents.t.data_ptr<int>(), parents.shared, (size_t)batch, (size_t)rows, context.data_ptr<int>(), ints_or_null(drafted), out[0].data_ptr<int>(), reinterpret_cast<uint64_t *>(out[1].data_ptr<int64_t>()), &err);
+        }
+        check(rc, err);
+        return wrap_list(out);
+    });
+}
+
+// rope_rows(ctx, device, query, key | None, positions, inv_freq, interleaved, suffix, factor, inverse) -> query, key
+PyObject *py_rope_rows(PyObject *, PyObject *const *a, Py_ssize_t) {
+    return guarded([&]() -> PyObject * {
+        zq_ctx *ctx = ctx_of(a[0]);
+        const int device = device_of(a[1]);
+        const Rows q = rows_3d(a[2], device, "query");
+        Rows k{};
+        if (!is_none(a[3])) {
+            k = rows_3d(a[3], device, "key");
+            if (k.rows != q.rows || k.dim != q.dim || k.t.scalar_type() != q.t.scalar_type()) fail(1, "rope_rows: key of shape " + sizes_of(k.t) + " or its dtype does not match the query's " + sizes_of(q.t));
+        }
+        const int d = in_dtype(q.t);
+        const at::Tensor positions = values(a[4], device, "positions", at::kInt, q.rows);
+        const at::Tensor freq = on_device(a[5], device, "inv_freq");
+        const at::Tensor inv_freq = values(a[5], device, "inv_freq", at::kFloat, freq.numel());
+        const bool interleaved = truth(a[6]), suffix = truth(a[7]), inverse = truth(a[9]);
+        const float factor = (float)number(a[8]);
+        std::vector<at::Tensor> out(2);
+        zq_error err;
+        int rc;
+        {
+            NoGil g;
+            out[0] = empty_like_sizes(q.t, q.t.sizes(), q.t.scalar_type());
+            if (k.t.defined()) out[1] = empty_like_sizes(k.t, k.t.sizes(), k.t.scalar_type());
+            rc = zq_rope_rows(ctx, q.t.data_ptr(), (size_t)q.heads, (size_t)q.stride, k.t.defined() ? k.t.data_ptr() : nullptr, (size_t)k.heads, (size_t)k.stride, d, (size_t)q.rows, (size_t)q.dim, (size_t)(2 * inv_freq.numel()), interleaved, suffix,
+                              positions.data_ptr<int>(), inv_freq.data_ptr<float>(), factor, inverse, out[0].data_ptr(), k.t.defined() ? out[1].data_ptr() : nullptr, &err);
+        }
+        check(rc, err);
+        return wrap_list(out);
+    });
+}
+
+// rope_append(ctx, device, query, key, value, k_pages, v_pages, block_table, context_lens, positions, inv_freq, draft_lens | None, interleaved, suffix, factor) -> query
+PyObject *py_rope_append(PyObject *, PyObject *const *a, Py_ssize_t) {
+    return guarded([&]() -> PyObject * {
+        zq_ctx *ctx = ctx_of(a[0]);
+        const int device = device_of(a[1]);
+        const Rows q = rows_3d(a[2], device, "query"), k = rows_3d(a[3], device, "key"), v = rows_3d(a[4], device, "value");
+        const Cache cache = cache_of(a[5], a[6], a[7], a[8], device, false);
+        const int64_t batch = (int64_t)cache.c.batch;
+        if (q.rows % batch || k.rows != q.rows || v.rows != q.rows) fail(1, "rope_append: " + std::to_string(q.rows) + " / " + std::to_string(k.rows) + " / " + std::to_string(v.rows) + " rows for " + std::to_string(batch) + " sequences");
+        if (q.dim != (int64_t)cache.c.head_dim || k.dim != q.dim || v.dim != q.dim || k.heads != (int64_t)cache.c.heads || v.heads != k.heads) fail(1, "rope_append: heads of key " + sizes_of(k.t) + " or value " + sizes_of(v.t) + " are not the cache's " + sizes_of(cache.k));
+        if (q.t.scalar_type() != cache.k.scalar_type() || k.t.scalar_type() != q.t.scalar_type() || v.t.scalar_type() != q.t.scalar_type()) type_error("rope_append: query, key and value have the cache's dtype " + dtype_name(cache.k.scalar_type()));
+        const at::Tensor positions = values(a[9], device, "positions", at::kInt, q.rows);
+        const at::Tensor freq = on_device(a[10], device, "inv_freq");
+        const at::Tensor inv_freq = values(a[10], device, "inv_freq", at::kFloat, freq.numel()), drafted = optional_lens(a[11], device, "draft_lens", batch);
+        const bool interleaved = truth(a[12]), suffix = truth(a[13]);
+        const float factor = (float)number(a[14]);
+        at::Tensor out;
+        zq_error err;
+        int rc;
+        {
+            NoGil g;
+            out = empty_like_sizes(q.t, q.t.sizes(), q.t.scalar_type());
+            rc = zq_rope_append(ctx, q.t.data_ptr(), (size_t)q.heads, (size_t)q.stride, k.t.data_ptr(), (size_t)k.stride, v.t.data_ptr(), (size_t)v.stride, (size_t)(q.rows / batch), &cache.c, ints_or_null(drafted), (size_t)(2 * inv_freq.numel()),
+                                interleaved, suffix, positions.data_ptr<int>(), inv_freq.data_ptr<float>(), factor, out.data_ptr(), &err);
+        }
+        check(rc, err);
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// tree_attention(ctx, device, query, k_pages, v_pages, block_table, context_lens, mask | None, draft_lens | None, scale | None) -> rows
+PyObject *py_tree_attention(PyObject *, PyObject *const *a, Py_ssize_t) {
+    return guarded([&]() -> PyObject * {
+        zq_ctx *ctx = ctx_of(a[0]);
+        const int device = device_of(a[1]);
+        const Rows q = rows_3d(a[2], device, "query");
+        const Cache cache = cache_of(a[3], a[4], a[5], a[6], device, false);
+        const int64_t batch = (int64_t)cache.c.batch, rows = q.rows / batch;
+        if (q.rows % batch || q.dim != (int64_t)cache.c.head_dim) fail(1, "tree_attention: query of shape " + sizes_of(q.t) + " for " + std::to_string(batch) + " sequences of a cache of " + sizes_of(cache.k));
+        if (q.t.scalar_type() != cache.k.scalar_type()) type_error("tree_attention: the query has the cache's dtype " + dtype_name(cache.k.scalar_type()) + ", not " + dtype_name(q.t.scalar_type()));
+        at::Tensor mask;
+        if (!is_none(a[7])) mask = values(a[7], device, "mask", at::kLong, batch * rows * ((rows + 63) / 64));
+        const at::Tensor drafted = optional_lens(a[8], device, "draft_lens", batch);
+        const float scale = is_none(a[9]) ? (float)(1.0 / std::sqrt((double)q.dim)) : (float)number(a[9]);
+        at::Tensor out;
+        zq_error err;
+        int rc;
+        {
+            NoGil g;
+            out = empty_like_sizes(q.t, q.t.sizes(), q.t.scalar_type());
+            rc = zq_tree_attention(ctx, q.t.data_ptr(), (size_t)q.heads, (size_t)q.stride, (size_t)rows, &cache.c, mask.defined() ? reinterpret_cast<const uint64_t *>(mask.data_ptr<int64_t>()) : nullptr, ints_or_null(drafted), scale, out.data_ptr(),
+                                   &err);
+        }
+        check(rc, err);
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// verify_draft(ctx, device, logits, tokens, parents, accept_u, sample_u, temperature, draft_logits | None, draft_lens | None) -> path, accepted, token
+PyObject *py_verify_draft(PyObject *, PyObject *const *a, Py_ssize_t) {
+    return guarded([&]() -> PyObject * {
+        zq_ctx *ctx = ctx_of(a[0]);
+        const int device = device_of(a[1]);
+        const at::Tensor logits = contiguous(on_device(a[2], device, "logits"));
+        if (logits.dim() != 3 || logits.numel() == 0) fail(1, "logits of shape " + sizes_of(logits) + ": [sequences, rows, vocabulary] is needed");
+        const int64_t batch = logits.size(0), rows = logits.size(1);
+        const int d = in_dtype(logits);
+        const at::Tensor tokens = values(a[3], device, "tokens", at::kInt, batch * rows);
+        const Parents parents = parents_of(a[4], device, batch, rows);
+        const at::Tensor accept_u = values(a[5], device, "accept_u", at::kFloat, batch * rows), sample_u = values(a[6], device, "sample_u", at::kFloat, batch), heat = values(a[7], device, "temperature", at::kFloat, batch);
+        at::Tensor draft;
+        if (!is_none(a[8])) {
+            draft = values(a[8], device, "draft_logits", logits.scalar_type(), logits.numel());
+            if (tensor_of(a[8]).sizes() != logits.sizes()) fail(1, "draft_logits of shape " + sizes_of(draft) + " for logits of " + sizes_of(logits));
+        }
+        const at::Tensor drafted = optional_lens(a[9], device, "draft_lens", batch);
+        std::vector<at::Tensor> out(3);
+        zq_error err;
+        int rc;
+        {
+            NoGil g;
+            out[0] = empty_like_sizes(logits, {batch, rows}, at::kInt);
+            out[1] = empty_like_sizes(logits, {batch}, at::kInt);
+            out[2] = empty_like_sizes(logits, {batch}, at::kInt);
+            rc = zq_verify_draft(ctx, logits.data_ptr(), draft.defined() ? draft.data_ptr() : nullptr, d, (size_t)batch, (size_t)rows, (size_t)logits.size(2), tokens.data_ptr<int>(), parents.t.data_ptr<int>(), parents.shared, accept_u.data_ptr<float>(),
+                                 sample_u.data_ptr<float>(), heat.data_ptr<float>(), ints_or_null(drafted), out[0].data_ptr<int>(), out[1].data_ptr<int>(), out[2].data_ptr<int>(), &err);
+        }
+        check(rc, err);
+        return wrap_list(out);
+    });
+}
+
+// cache_keep_path(ctx, device, k_pages, v_pages, block_table, context_lens, path, accepted)
+PyObject *py_cache_keep_path(PyObject *, PyObject *const *a, Py_ssize_t) {
+    return guarded([&]() -> PyObject * {
+        zq_ctx *ctx = ctx_of(a[0]);
+        const int device = device_of(a[1]);
+        const Cache cache = cache_of(a[2], a[3], a[4], a[5], device, true);
+        const at::Tensor given = on_device(a[6], device, "path");
+        if (given.dim() != 2 || given.size(0) != (int64_t)cache.c.batch) fail(1, "path of shape " + sizes_of(given) + " for " + std::to_string(cache.c.batch) + " sequences");
+        const at::Tensor path = values(a[6], device, "path", at::kInt, given.numel()), accepted = values(a[7], device, "accepted", at::kInt, (int64_t)cache.c.batch);
+        zq_error err;
+        int rc;
+        {
+            NoGil g;
+            rc = zq_cache_keep_path(ctx, &cache.c, path.data_ptr<int>(), (size_t)path.size(1), accepted.data_ptr<int>(), &err);
+        }
+        check(rc, err);
+        Py_RETURN_NONE;
+    });
+}
+
 PyObject *py_setup(PyObject *, PyObject *failure) {
     Py_INCREF(failure);
     Py_XSETREF(g_failure, failure);
@@ -442,7 +718,9 @@ template <Py_ssize_t N, PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t
 #define ZQ_FAST(name, n, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&counted<n, fn>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     ZQ_FAST("linear", 5, py_linear), ZQ_FAST("linear_batch", 3, py_linear_batch), ZQ_FAST("linear_multi", 7, py_linear_multi), ZQ_FAST("gated", 7, py_gated),
-    ZQ_FAST("rope", 11, py_rope), ZQ_FAST("gather_rows", 4, py_gather_rows), ZQ_FAST("linear_host_batch", 2, py_linear_host_batch), {"setup", py_setup, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr},
+    ZQ_FAST("rope", 11, py_rope), ZQ_FAST("gather_rows", 4, py_gather_rows), ZQ_FAST("linear_host_batch", 2, py_linear_host_batch),
+    ZQ_FAST("draft_tree", 5, py_draft_tree), ZQ_FAST("rope_rows", 10, py_rope_rows), ZQ_FAST("rope_append", 15, py_rope_append), ZQ_FAST("tree_attention", 10, py_tree_attention), ZQ_FAST("verify_draft", 10, py_verify_draft),
+    ZQ_FAST("cache_keep_path", 8, py_cache_keep_path), {"setup", py_setup, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_zq_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

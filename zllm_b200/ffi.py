@@ -15,6 +15,7 @@ Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, IQ4_NL = 2, 8, 12, 13, 14, 20
 Q5_0, Q5_1, Q3_K, IQ4_XS = 6, 7, 11, 23
 F32, F16, BF16 = 0, 1, 2
 JOB_ROW_PARALLEL = 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_YARN = 0, 1, 2
 ROUTE_SOFTMAX, ROUTE_SIGMOID_BIAS, ROUTE_SQRT_SOFTPLUS_BIAS = 0, 1, 2
 MOE_NO_ROUTE = 0xFFFFFFFF  # ZQ_MOE_NO_ROUTE: an expert id that means "no route in this place"
 DIST_HANDLE_BYTES = 80
@@ -32,7 +33,7 @@ class ZqFailure(RuntimeError):
         self.message = message
 
 
-_vp, _sz, _u32, _i, _f = C.c_void_p, C.c_size_t, C.c_uint32, C.c_int, C.c_float
+_vp, _sz, _u32, _i, _f, _d = C.c_void_p, C.c_size_t, C.c_uint32, C.c_int, C.c_float, C.c_double
 
 
 class ZqLinearJob(C.Structure):
@@ -45,6 +46,13 @@ class ZqLinearHostJob(C.Structure):
     """``zq_linear_host_job``: one host-buffer projection of a ``zq_linear_host_batch`` call."""
 
     _fields_ = [("w", C.c_void_p), ("host_x", C.c_void_p), ("m", C.c_size_t), ("host_y", C.c_void_p)]
+
+
+class ZqKvCache(C.Structure):
+    """``zq_kv_cache``: the pages of a cache, the sequences' block table and their lengths."""
+
+    _fields_ = [("dev_k", C.c_void_p), ("dev_v", C.c_void_p), ("dtype", C.c_int), ("pages", C.c_size_t), ("page_size", C.c_size_t), ("heads", C.c_size_t), ("head_dim", C.c_size_t), ("page_stride", C.c_size_t),
+                ("layers", C.c_size_t), ("layer_stride", C.c_size_t), ("dev_blocks", C.c_void_p), ("batch", C.c_size_t), ("max_blocks", C.c_size_t), ("dev_context_lens", C.c_void_p)]
 
 
 _err = C.POINTER(ZqError)
@@ -80,6 +88,13 @@ PROTOTYPES = {
     "zq_linear_multi": (_i, [_vp, C.POINTER(_vp), _sz, _vp, _i, _sz, C.POINTER(_vp), _i, _err]),
     "zq_rmsnorm_linear": (_i, [_vp, C.POINTER(_vp), _sz, _vp, _i, _sz, _vp, C.c_float, C.c_float, C.POINTER(_vp), _i, _err]),
     "zq_rope_qk": (_i, [_vp, _vp, _sz, _vp, _sz, _i, _sz, _sz, _sz, _i, _i, _sz, _vp, _vp, _sz, _err]),
+    "zq_rope_frequencies": (_i, [_sz, _d, _i, _d, _d, _d, _d, C.POINTER(_f), C.POINTER(_f), C.POINTER(_f), _err]),
+    "zq_rope_rows": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _sz, _i, _sz, _sz, _sz, _i, _i, _vp, _vp, _f, _i, _vp, _vp, _err]),
+    "zq_rope_append": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, C.POINTER(ZqKvCache), _vp, _sz, _i, _i, _vp, _vp, _f, _vp, _err]),
+    "zq_draft_tree": (_i, [_vp, _vp, _i, _sz, _sz, _vp, _vp, _vp, _vp, _err]),
+    "zq_tree_attention": (_i, [_vp, _vp, _sz, _sz, _sz, C.POINTER(ZqKvCache), _vp, _vp, _f, _vp, _err]),
+    "zq_verify_draft": (_i, [_vp, _vp, _vp, _i, _sz, _sz, _sz, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _err]),
+    "zq_cache_keep_path": (_i, [_vp, C.POINTER(ZqKvCache), _vp, _sz, _vp, _err]),
     "zq_gated_silu": (_i, [_vp, _vp, _vp, _vp, _i, _sz, _vp, _i, _err]),
     "zq_gated_mlp": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _sz, _vp, _i, _vp, _err]),
     "zq_linear_noalloc": (_i, [_vp, _vp, _vp, _i, _sz, _vp, _i, _err]),
