@@ -38,24 +38,6 @@ template <bool BF16> __device__ __forceinline__ void mma16(float (&d)[4], const 
     else
         mma_16816(d, a[0], a[1], a[2], a[3], b0, b1);
 }
-template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    if (BF16) {
-        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<uint32_t *>(&v);
-    }
-    __half2 v = __floats2half2_rn(lo, hi);
-    return h2_as_u32(v);
-}
-template <bool BF16> __device__ __forceinline__ float unpack16(uint32_t bits) { return BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits)); }
-// Values of a word whose exponent is all ones (infinities, NaN) become zero; true if there was one.
-template <bool BF16> __device__ __forceinline__ bool drop_nonfinite(uint32_t &w) {
-    const uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-    const bool lo = (w & e) == e, hi = (w >> 16 & e) == e;
-    if (lo) w &= 0xffff0000u;
-    if (hi) w &= 0x0000ffffu;
-    return lo || hi;
-}
-
 // Shape of the kernel for a head of up to D values and WM warps of 16 rows.
 template <int D, int WM> struct AttnShape {
     static constexpr int kGroups = WM == 4 ? 2 : 4;              // key groups of a CTA
@@ -72,63 +54,6 @@ template <int D, int WM> struct AttnShape {
     static constexpr int kPartFloats = kRows * (D + 2);
     static_assert(kStages >= 2 && kSmem <= 227 << 10, "ring");
 };
-
-struct Share {
-    int64_t first, last, total;  // units of this CTA; of all
-    int ctas;                    // with a share
-    int seq;                     // of the first unit
-    int64_t seq_first;           // first unit of that sequence
-};
-
-__device__ __forceinline__ int units_of(const SeqLen &s, int unit) {
-    return s.rows ? (s.context + s.rows + unit - 1) / unit : 1;  // a sequence without rows has its output set to zero by its one unit
-}
-
-// The CTA's share of the units.  Every thread adds up some sequences, the thread whose sequences hold the first unit looks for it.
-template <int kThreads> __device__ Share find_share(const AttnArgs &a, int unit, uint8_t *scratch) {
-    int64_t *s_sum = reinterpret_cast<int64_t *>(scratch);  // [kThreads / 32 + 3]
-    const int tid = threadIdx.x, lane = tid & 31, per = (a.batch + kThreads - 1) / kThreads;
-    const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
-    const int64_t items = (int64_t)a.c.heads * a.tiles;
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += units_of(seq_len(a, b), unit) * items;
-    int64_t incl = mine;
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-    }
-    if (lane == 31) s_sum[tid / 32] = incl;
-    __syncthreads();
-    int64_t before = 0, total = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < tid / 32) before += s_sum[w];
-        total += s_sum[w];
-    }
-    int64_t at = before + incl - mine;
-    Share s;
-    s.total = total;
-    s.ctas = (int)min((int64_t)gridDim.x, total);
-    const int64_t c = blockIdx.x;
-    s.first = c < s.ctas ? c * total / s.ctas : total;
-    s.last = c < s.ctas ? (c + 1) * total / s.ctas : total;
-    int64_t *s_found = s_sum + kThreads / 32;
-    if (s.first >= at && s.first < at + mine) {
-        for (int b = b0; b < b1; ++b) {
-            const int64_t n = units_of(seq_len(a, b), unit) * items;
-            if (s.first < at + n) {
-                s_found[0] = b;
-                s_found[1] = at;
-                break;
-            }
-            at += n;
-        }
-    }
-    __syncthreads();
-    s.seq = s.first < total ? (int)s_found[0] : 0;
-    s.seq_first = s.first < total ? s_found[1] : 0;
-    __syncthreads();
-    return s;
-}
 
 template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<D, WM>::kThreads, 1) tree_attention_kernel(const AttnArgs a) {
     using S = AttnShape<D, WM>;
@@ -401,7 +326,7 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
 }
 
 // Joins the parts of the item that starts in CTA blockIdx.x's share, in the order of its keys.
-template <bool BF16> __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, int rows, int d_pad) {
+template <bool BF16> __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, int rows, int d_pad) {  // blockIdx.y: sixteen rows
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int4 info = a.info[blockIdx.x];
@@ -409,8 +334,8 @@ template <bool BF16> __global__ void __launch_bounds__(256) attention_join_kerne
     const int seq = info.x, head = info.y / a.tiles, tile = info.y % a.tiles, pieces = info.z, d = a.c.head_dim;
     const size_t floats = (size_t)rows * (d_pad + 2);
     auto part = [&](int p) { return a.parts + ((size_t)(blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * floats; };
-    for (int idx = threadIdx.x; idx < rows * (d / 2); idx += blockDim.x) {
-        const int r = idx / (d / 2), col = 2 * (idx % (d / 2)), row = tile * rows + r, i = row / a.group;
+    for (int idx = threadIdx.x; idx < 16 * (d / 2); idx += blockDim.x) {
+        const int r = 16 * blockIdx.y + idx / (d / 2), col = 2 * (idx % (d / 2)), row = tile * rows + r, i = row / a.group;
         if (i >= a.rows) continue;
         float m = -INFINITY;
         for (int p = 0; p < pieces; ++p) m = fmaxf(m, part(p)[rows * d_pad + r]);
@@ -429,6 +354,10 @@ template <bool BF16> __global__ void __launch_bounds__(256) attention_join_kerne
     }
 }
 
+int launch_attention_join(zq_ctx *ctx, const AttnArgs &a, bool bf16, int ctas, int rows, int d_pad, zq_error *err) {
+    return launch_pdl(ctx, bf16 ? attention_join_kernel<true> : attention_join_kernel<false>, dim3((unsigned)ctas, (unsigned)(rows / 16)), dim3(256), 0, err, a, rows, d_pad);
+}
+
 template <int D, int WM, bool BF16> static int launch_shape(zq_ctx *ctx, AttnArgs &a, zq_error *err) {
     using S = AttnShape<D, WM>;
     a.tiles = (a.rows * a.group + S::kRows - 1) / S::kRows;
@@ -441,7 +370,7 @@ template <int D, int WM, bool BF16> static int launch_shape(zq_ctx *ctx, AttnArg
     ZQ_CUDA_CHECK(cudaFuncSetAttribute(tree_attention_kernel<D, WM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), err);
     rc = launch_pdl(ctx, tree_attention_kernel<D, WM, BF16>, dim3((unsigned)ctas), dim3(S::kThreads), S::kSmem, err, a);
     if (rc) return rc;
-    return launch_pdl(ctx, attention_join_kernel<BF16>, dim3((unsigned)ctas), dim3(256), 0, err, a, S::kRows, D);
+    return launch_attention_join(ctx, a, BF16, (int)ctas, S::kRows, D, err);
 }
 template <int D, bool BF16> static int launch_rows(zq_ctx *ctx, AttnArgs &a, zq_error *err) {
     const int rows = a.rows * a.group;
@@ -479,5 +408,8 @@ extern "C" int zq_tree_attention(zq_ctx *ctx, const void *dev_q, size_t q_heads,
     a.words = (int)((rows + 63) / 64);
     a.scale = scale * kLog2e;
     a.status = ctx->status_dev;
+    bool taken = false;
+    rc = launch_attention_wide(ctx, a, cache, taken, err);
+    if (rc || taken) return rc;
     return cache->dtype == ZQ_BF16 ? launch_dim<true>(ctx, a, err) : launch_dim<false>(ctx, a, err);
 }

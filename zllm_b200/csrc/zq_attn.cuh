@@ -38,4 +38,89 @@ __device__ __forceinline__ bool sees(const AttnArgs &a, int seq, int i, int j) {
     return a.mask[((size_t)seq * a.rows + i) * a.words + (j >> 6)] >> (j & 63) & 1;
 }
 
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if (BF16) {
+        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t *>(&v);
+    }
+    __half2 v = __floats2half2_rn(lo, hi);
+    return h2_as_u32(v);
+}
+template <bool BF16> __device__ __forceinline__ float unpack16(uint32_t bits) { return BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits)); }
+// Values of a word whose exponent is all ones (infinities, NaN) become zero; true if there was one.
+template <bool BF16> __device__ __forceinline__ bool drop_nonfinite(uint32_t &w) {
+    const uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+    const bool lo = (w & e) == e, hi = (w >> 16 & e) == e;
+    if (lo) w &= 0xffff0000u;
+    if (hi) w &= 0x0000ffffu;
+    return lo || hi;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+struct Share {
+    int64_t first, last, total;  // units of this CTA; of all
+    int ctas;                    // with a share
+    int seq;                     // of the first unit
+    int64_t seq_first;           // first unit of that sequence
+};
+
+__device__ __forceinline__ int units_of(const SeqLen &s, int unit) {
+    return s.rows ? (s.context + s.rows + unit - 1) / unit : 1;  // a sequence without rows has its output set to zero by its one unit
+}
+
+// The CTA's share of the units.  Every thread adds up some sequences, the thread whose sequences hold the first unit looks for it.
+template <int kThreads> __device__ Share find_share(const AttnArgs &a, int unit, uint8_t *scratch) {
+    int64_t *s_sum = reinterpret_cast<int64_t *>(scratch);  // [kThreads / 32 + 3]
+    const int tid = threadIdx.x, lane = tid & 31, per = (a.batch + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+    const int64_t items = (int64_t)a.c.heads * a.tiles;
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += units_of(seq_len(a, b), unit) * items;
+    int64_t incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 31) s_sum[tid / 32] = incl;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < tid / 32) before += s_sum[w];
+        total += s_sum[w];
+    }
+    int64_t at = before + incl - mine;
+    Share s;
+    s.total = total;
+    s.ctas = (int)min((int64_t)gridDim.x, total);
+    const int64_t c = blockIdx.x;
+    s.first = c < s.ctas ? c * total / s.ctas : total;
+    s.last = c < s.ctas ? (c + 1) * total / s.ctas : total;
+    int64_t *s_found = s_sum + kThreads / 32;
+    if (s.first >= at && s.first < at + mine) {
+        for (int b = b0; b < b1; ++b) {
+            const int64_t n = units_of(seq_len(a, b), unit) * items;
+            if (s.first < at + n) {
+                s_found[0] = b;
+                s_found[1] = at;
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+    s.seq = s.first < total ? (int)s_found[0] : 0;
+    s.seq_first = s.first < total ? s_found[1] : 0;
+    __syncthreads();
+    return s;
+}
+
+// Joins the parts of cut items: in place behind a kernel that left them (a.parts, a.info) with `rows` rows of d_pad values per part.
+int launch_attention_join(zq_ctx *ctx, const AttnArgs &a, bool bf16, int ctas, int rows, int d_pad, zq_error *err);
+// Many rows per key: the kernel on tcgen05 (zq_attn_wide.cu).  `taken` false: not a shape of this kernel.
+int launch_attention_wide(zq_ctx *ctx, AttnArgs &a, const zq_kv_cache *cache, bool &taken, zq_error *err);
+
 }  // namespace zq

@@ -1,0 +1,583 @@
+// Attention of many rows per key (drafted rows times query heads of a cache head) on the 5th-generation tensor cores.
+//
+// The same sums and the same shares as in zq_attn.cu, in tiles of 128 rows by 128 keys: S = Q K^T into tensor memory, the weights from
+// there through registers back into tensor memory (the same columns), O += P V.  A CTA per SM has
+//   warp 8      the copies: TMA boxes of a page by 64 values, K and V tiles in turn through one ring of 128-byte swizzled tiles;
+//   warp 9      the MMAs (tcgen05, one lane);
+//   warps 0..3  slot 0 and warps 4..7 slot 1: a thread has a row of S and O, so largest score and sum need no exchange.
+// The slots take turns at the tensor cores: while one turns scores into weights, the other's products run.  With more than 128 rows (PAIR) they hold two row tiles
+// against the same keys, else the same rows against every other tile of keys, and add up at the end of the item.
+//
+// O stays in tensor memory while the largest score rises by less than 2^8: the weights are taken relative to an older maximum (exact in f32,
+// and the sum with them), so that the sums so far are hardly ever multiplied down.
+//
+// Bytes against tensor cycles: a tile of 128 keys of 128 values is 64 KB, 2850 cycles at an SM's share of the memory rate; its products take 1024
+// cycles per slot of rows and its exponentials as many, so up to 256 rows the copies bound it.
+//
+// Padding and the end of a sequence: boxes are whole pages, and what lies behind the sequence's end must not reach a row (0 * NaN): in tiles that hold
+// drafted rows or the end, a slot's threads clear those rows of V in shared memory, and infinities and NaN of drafted rows, which they
+// add to O of the rows that see them.
+#include "zq_attn.cuh"
+
+namespace zq {
+
+constexpr int kWideThreads = 320, kWideTile = 128;
+
+__device__ __forceinline__ bool wide_elect() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t *bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc) : "memory");
+}
+__device__ __forceinline__ void tm_ld32(uint32_t at, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tm_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+        "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int x, int head, int row, int page) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(head), "r"(row), "r"(page)
+                 : "memory");
+}
+// A tile of 128-byte swizzled rows, eight rows (1024 bytes) from one group to the next.  K-major (Q, K: a row is 64 values of the reduced
+// dimension): the leading offset is not used.  The other way round (V: a row is a key, the reduced dimension): the leading offset leads to the next 64 values.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t leading) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+template <int D> struct WideShape {
+    static constexpr int kBlocks = D / 64;
+    static constexpr int kBlock = kWideTile * 128;      // bytes of 64 values of 128 rows
+    static constexpr int kTileBytes = kBlocks * kBlock;
+    static constexpr int kRing = D == 128 ? 5 : 10;     // K and V tiles
+    static constexpr int kQ = 0, kRingAt = 2 * kTileBytes, kBars = kRingAt + kRing * kTileBytes;
+    static constexpr int kSmem = kBars + 2048 + 1024;   // barriers, maxima and sums of slot 1; alignment
+    static_assert(kSmem <= 227 << 10, "shared memory");
+};
+
+struct WideBars {
+    uint64_t full[10], empty[10], scores[2], weights[2], sums[2], q[2], end;
+    uint32_t tmem, dead, poison[2][4];     // rows of a tile of V that were cleared of infinities and NaN, per slot
+    float top[kWideTile], sum[kWideTile];  // of slot 1's rows, when the slots share rows
+};
+static_assert(sizeof(WideBars) <= 2048, "barriers");
+
+// 32 bits of a row's view of the drafted rows, from row d on (d may be negative: the context, which it sees).
+__device__ __forceinline__ uint32_t view32(const AttnArgs &a, int seq, int i, int d, int rows) {
+    if (i >= rows) return 0u;
+    uint32_t v;
+    if (d <= -32) {
+        v = 0xffffffffu;
+    } else {
+        const int from = d < 0 ? 0 : d, skip = d < 0 ? -d : 0;
+        uint32_t bits;  // drafted rows [from, from + 32)
+        if (!a.mask) {
+            const int n = i - from + 1;
+            bits = n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+        } else {
+            const unsigned long long *m = a.mask + ((size_t)seq * a.rows + i) * a.words;
+            const int w = from >> 6, o = from & 63;
+            unsigned long long x = w < a.words ? m[w] >> o : 0;
+            if (o > 32 && w + 1 < a.words) x |= m[w + 1] << (64 - o);
+            bits = (uint32_t)x;
+        }
+        v = skip ? bits << skip | ((1u << skip) - 1) : bits;
+    }
+    const int n = rows - d;  // keys there are
+    return n <= 0 ? 0u : n >= 32 ? v : v & ((1u << n) - 1);
+}
+
+template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideThreads, 1) wide_attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    using S = WideShape<D>;
+    constexpr int kRows = PAIR ? 2 * kWideTile : kWideTile;
+    extern __shared__ uint8_t raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t base = smem_u32(smem);
+    WideBars &bar = *reinterpret_cast<WideBars *>(smem + S::kBars);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    if (tid == 0) {
+        for (int i = 0; i < S::kRing; ++i) {
+            mbar_init(&bar.full[i], 1);
+            mbar_init(&bar.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.scores[i], 1);
+            mbar_init(&bar.weights[i], kWideTile);
+            mbar_init(&bar.sums[i], 1);
+            mbar_init(&bar.q[i], kWideTile);
+        }
+        mbar_init(&bar.end, 1);
+        bar.dead = 0;
+        fence_mbar_init();
+        a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    const Share share = find_share<kWideThreads>(a, kWideTile, smem);
+    if (share.first >= share.last) return;
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == 8 && wide_elect()) {
+        tma_prefetch_desc(&map_k);
+        tma_prefetch_desc(&map_v);
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = bar.tmem;
+    const int d = a.c.head_dim;
+
+    // Bounded wait of a whole warp.  One that runs out is reported, and from then on the CTA waits for nothing and walks to its end.
+    auto wait = [&](uint64_t *b, uint32_t parity, uint32_t code) {
+        bool ok = false;
+        for (uint32_t i = 0; i < (1u << 22) && !ok; ++i) {
+            ok = mbar_try_wait(b, parity);
+            if (!ok && *reinterpret_cast<volatile uint32_t *>(&bar.dead)) break;
+        }
+        if (!__all_sync(0xffffffffu, ok) && lane == 0) {
+            *reinterpret_cast<volatile uint32_t *>(&bar.dead) = 1;
+            atomicMax(a.status, code);
+        }
+        __syncwarp();
+    };
+
+    // The items of this CTA's share, one after the other; every role walks them for itself.
+    int seq = share.seq;
+    int64_t seq_first = share.seq_first, u = share.first;
+    SeqLen len = seq_len(a, seq);
+    int units = units_of(len, kWideTile), head = 0, tile = 0, ua = 0, ub = 0, item = 0, keys = 0;
+    int64_t item_first = 0;
+    auto next_item = [&]() {
+        if (u >= share.last) return false;
+        while (u >= seq_first + (int64_t)units * a.c.heads * a.tiles) {
+            seq_first += (int64_t)units * a.c.heads * a.tiles;
+            len = seq_len(a, ++seq);
+            units = units_of(len, kWideTile);
+        }
+        item = (int)((u - seq_first) / units);
+        item_first = seq_first + (int64_t)item * units;
+        head = item / a.tiles;
+        tile = item % a.tiles;
+        ua = (int)(u - item_first);
+        ub = (int)min((int64_t)units, share.last - item_first);
+        keys = len.rows ? len.context + len.rows : 0;
+        u = item_first + ub;
+        return true;
+    };
+
+    if (warp == 8) {
+        // ---- copies
+        const int box_shift = min(a.c.page_shift, 7), boxes = kWideTile >> box_shift, box_rows = 1 << box_shift;
+        uint32_t at = 0, phase = 0;  // ring place; how often round
+        while (next_item()) {
+            auto page_of = [&](int t) {
+                const int key = t * kWideTile + lane * box_rows;
+                if (lane >= boxes || t >= ub || key >= keys) return a.c.pages;  // no page: zeros
+                const int page = a.c.blocks[(size_t)seq * a.c.max_blocks + (key >> a.c.page_shift)];
+                if (page >= 0 && page < a.c.pages) return page;
+                atomicMax(a.status, (uint32_t)kStatusBadIndex);
+                return a.c.pages;
+            };
+            int ahead = page_of(ua);
+            for (int t = ua; t < ub; ++t) {
+                const int page = ahead, row = (t * kWideTile + lane * box_rows) & ((1 << a.c.page_shift) - 1);
+                ahead = page_of(t + 1);
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    if (phase) wait(&bar.empty[at], (phase - 1) & 1, kStatusMmaTimeout);
+                    if (wide_elect()) mbar_expect_tx(&bar.full[at], S::kTileBytes);
+                    __syncwarp();
+                    if (lane < boxes) {
+                        const uint32_t dst = base + S::kRingAt + at * S::kTileBytes + lane * box_rows * 128;
+#pragma unroll
+                        for (int b = 0; b < S::kBlocks; ++b) tma_load_page(dst + b * S::kBlock, kv ? &map_v : &map_k, &bar.full[at], 64 * b, head, row, page);
+                    }
+                    if (++at == S::kRing) {
+                        at = 0;
+                        ++phase;
+                    }
+                }
+            }
+        }
+        // where waits ran out, nobody has waited for the last copies
+        if (*reinterpret_cast<volatile uint32_t *>(&bar.dead)) {
+            for (int i = 0; i < S::kRing; ++i) {
+                const uint32_t rounds = phase + (i < (int)at ? 1 : 0);
+                if (rounds) mbar_wait_bounded(&bar.full[i], (rounds - 1) & 1);
+            }
+        }
+    } else if (warp == 9) {
+        // ---- MMAs
+        const uint32_t type = BF16 ? 1u << 7 | 1u << 10 : 0u;
+        const uint32_t idesc_s = 1u << 4 | type | (uint32_t)(kWideTile >> 3) << 17 | (uint32_t)(kWideTile >> 4) << 24;
+        const uint32_t idesc_o = 1u << 4 | type | 1u << 16 | (uint32_t)(D >> 3) << 17 | (uint32_t)(kWideTile >> 4) << 24;
+        const int k_steps = (d + 15) / 16;
+        uint32_t first = 0;  // tiles of the ring used by earlier items
+        uint32_t q_phase = 0, w_phase[2] = {0, 0};
+        auto slot_of = [&](uint32_t n) { return n % S::kRing; };
+        auto wait_tile = [&](uint32_t n) { wait(&bar.full[n % S::kRing], n / S::kRing & 1, kStatusTmaTimeout); };
+        while (next_item()) {
+            const int n = ub - ua, jobs = PAIR ? 2 * n : n;
+            wait(&bar.q[0], q_phase, kStatusMmaTimeout);
+            if (PAIR) wait(&bar.q[1], q_phase, kStatusMmaTimeout);
+            q_phase ^= 1;
+            auto scores = [&](int j) {
+                const int i = PAIR ? j >> 1 : j, s = j & 1;
+                const uint32_t k_tile = first + 2 * i;
+                if (!PAIR || s == 0) wait_tile(k_tile);
+                tc_after();
+                const uint64_t qd = sw128_desc(base + S::kQ + (PAIR ? s : 0) * S::kTileBytes, 16), kd = sw128_desc(base + S::kRingAt + slot_of(k_tile) * S::kTileBytes, 16);
+                if (wide_elect()) {
+                    for (int k = 0; k < k_steps; ++k) {
+                        const uint32_t off = (k >> 2) * (S::kBlock / 16) + (k & 3) * 2;
+                        mma_ss(tmem + s * 256, qd + off, kd + off, idesc_s, k > 0);
+                    }
+                    tc_commit(&bar.scores[s]);
+                    if (!PAIR || s == 1) tc_commit(&bar.empty[slot_of(k_tile)]);
+                }
+                __syncwarp();
+            };
+            if (jobs > 0) scores(0);
+            if (jobs > 1) scores(1);
+            for (int j = 0; j < jobs; ++j) {
+                const int i = PAIR ? j >> 1 : j, s = j & 1;
+                const uint32_t v_tile = first + 2 * i + 1;
+                if (!PAIR || s == 0) wait_tile(v_tile);
+                wait(&bar.weights[s], w_phase[s], kStatusMmaTimeout);
+                w_phase[s] ^= 1;
+                tc_after();
+                const uint64_t vd = sw128_desc(base + S::kRingAt + slot_of(v_tile) * S::kTileBytes, S::kBlock);
+                if (wide_elect()) {
+#pragma unroll
+                    for (int k = 0; k < kWideTile / 16; ++k) mma_ts(tmem + s * 256 + 128, tmem + s * 256 + 8 * k, vd + k * (2048 / 16), idesc_o);
+                    tc_commit(&bar.sums[s]);
+                    if (!PAIR || s == 1) tc_commit(&bar.empty[slot_of(v_tile)]);
+                }
+                __syncwarp();
+                if (j + 2 < jobs) scores(j + 2);
+            }
+            first += 2 * n;
+        }
+        if (wide_elect()) tc_commit(&bar.end);
+        __syncwarp();
+        wait(&bar.end, 0, kStatusMmaTimeout);
+    } else {
+        // ---- scores to weights
+        const int s = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16, t_s = tmem + s * 256 + lanes, t_o = t_s + 128;
+        uint32_t s_phase = 0;
+        uint32_t n_sums = 0;   // products that this slot has been through
+        uint32_t first = 0;
+        const int chunks = d / 8;
+        while (next_item()) {
+            const int n = ub - ua, mine = PAIR ? n : (n + 1 - s) / 2;
+            // ---- this slot's rows of Q
+            if (PAIR || s == 0) {
+                uint8_t *q_tile = smem + S::kQ + s * S::kTileBytes;
+                const int r0 = tile * kRows + s * kWideTile, n_rows = len.rows * a.group;
+                for (int idx = row; idx < kWideTile * (D / 8); idx += kWideTile) {
+                    const int r = idx / (D / 8), c = idx % (D / 8), q_row = r0 + r;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (q_row < n_rows && c < chunks)
+                        v = *reinterpret_cast<const uint4 *>(a.q + 2 * (((int64_t)seq * a.rows + q_row / a.group) * a.q_stride + (int64_t)(head * a.group + q_row % a.group) * d + 8 * c));
+                    *reinterpret_cast<uint4 *>(q_tile + (c >> 3) * S::kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+                }
+                fence_proxy_async();
+            }
+            uint32_t zero[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) zero[e] = 0;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) tm_st32(t_o + 32 * c, zero);
+            tm_st_wait();
+            if (PAIR || s == 0) mbar_arrive(&bar.q[s]);
+            const int q_row = tile * kRows + (PAIR ? s * kWideTile : 0) + row, i = q_row / a.group;
+            float top = -INFINITY, sum = 0.f;  // top: what the weights are relative to, in scores as they come
+
+            for (int job = 0; job < mine; ++job) {
+                const int step = PAIR ? job : 2 * job + s, key0 = (ua + step) * kWideTile;
+                const bool masked = key0 + kWideTile > (len.rows ? len.context : 0);
+                uint32_t seen[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                if (masked) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) seen[c] = view32(a, seq, i, key0 + 32 * c - len.context, len.rows);
+                }
+                wait(&bar.scores[s], s_phase, kStatusMmaTimeout);
+                s_phase ^= 1;
+                tc_after();
+                float m = -INFINITY;
+                uint32_t x[32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tm_ld32(t_s + 32 * c, x);
+                    tm_ld_wait();
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(seen[c] >> e & 1)) x[e] = 0xff800000u;
+                    }
+                    float part[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) part[e & 3] = fmaxf(part[e & 3], __uint_as_float(x[e]));
+                    m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+                }
+                // rises by less than 2^8 stay in the weights
+                const bool rise = m > top && (top == -INFINITY || (m - top) * a.scale > 8.f);
+                if (__any_sync(0xffffffffu, rise && top != -INFINITY)) {
+                    const float down = rise && top != -INFINITY ? ex2((top - m) * a.scale) : 1.f;
+                    if (job) wait(&bar.sums[s], (n_sums - 1) & 1, kStatusMmaTimeout);
+                    tc_after();
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        tm_ld32(t_o + 32 * c, x);
+                        tm_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
+                        tm_st32(t_o + 32 * c, x);
+                    }
+                    tm_st_wait();
+                    sum *= down;
+                }
+                if (rise) top = m;
+                const float off = top == -INFINITY ? 0.f : top * a.scale;
+                float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tm_ld32(t_s + 32 * c, x);
+                    tm_ld_wait();
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float lo = ex2(fmaf(__uint_as_float(x[e]), a.scale, -off)), hi = ex2(fmaf(__uint_as_float(x[e + 1]), a.scale, -off));
+                        if (masked) {
+                            if (!(seen[c] >> e & 1)) lo = 0.f;
+                            if (!(seen[c] >> (e + 1) & 1)) hi = 0.f;
+                        }
+                        sums[e >> 1 & 3] += lo + hi;
+                        p[e >> 1] = pack2<BF16>(lo, hi);
+                    }
+                    tm_st16(t_s + 16 * c, p);  // over the first half of scores that are read already
+                }
+                tm_st_wait();
+                sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+
+                if (masked) {
+                    // clear what nobody may meet in V; slot 0 does it for both where they share the keys
+                    const uint32_t v_tile = first + 2 * step + 1;
+                    uint8_t *v = smem + S::kRingAt + v_tile % S::kRing * S::kTileBytes;
+                    if (!PAIR || s == 0) {
+                        wait(&bar.full[v_tile % S::kRing], v_tile / S::kRing & 1, kStatusTmaTimeout);
+                        bool dropped = false;
+                        const int key = key0 + row;
+                        if (key >= (len.rows ? len.context : 0)) {
+#pragma unroll 1
+                            for (int c = 0; c < D / 8; ++c) {
+                                uint4 *w = reinterpret_cast<uint4 *>(v + (c >> 3) * S::kBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+                                uint4 y = *w;
+                                if (key >= keys) {
+                                    *w = make_uint4(0, 0, 0, 0);
+                                } else {
+                                    bool some = drop_nonfinite<BF16>(y.x);
+                                    some |= drop_nonfinite<BF16>(y.y);
+                                    some |= drop_nonfinite<BF16>(y.z);
+                                    some |= drop_nonfinite<BF16>(y.w);
+                                    if (some) *w = y;
+                                    dropped |= some;
+                                }
+                            }
+                            fence_proxy_async();
+                        }
+                        const uint32_t rows = __ballot_sync(0xffffffffu, dropped);
+                        if (lane == 0) bar.poison[s][warp & 3] = rows;
+                    }
+                    asm volatile("bar.sync %0, %1;" ::"r"(PAIR ? 1 : 2 + s), "n"(PAIR ? 2 * kWideTile : kWideTile) : "memory");
+                    // the rows that see such a value have it in their sums
+                    uint32_t poison[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) poison[c] = bar.poison[PAIR ? 0 : s][c];
+                    if (poison[0] | poison[1] | poison[2] | poison[3]) {
+                        if (job) wait(&bar.sums[s], (n_sums - 1) & 1, kStatusMmaTimeout);
+                        tc_after();
+                        for (int r = 0; r < kWideTile; ++r) {
+                            const uint32_t bad = r < 32 ? poison[0] : r < 64 ? poison[1] : r < 96 ? poison[2] : poison[3], view = r < 32 ? seen[0] : r < 64 ? seen[1] : r < 96 ? seen[2] : seen[3];
+                            if (!(bad >> (r & 31) & 1)) continue;
+                            const bool mine_too = view >> (r & 31) & 1;
+                            const int64_t at = cache_row(a.c, seq, key0 + r);
+                            if (at < 0) continue;
+                            const uint16_t *from = reinterpret_cast<const uint16_t *>(a.c.v) + at + (int64_t)head * d;
+#pragma unroll 1
+                            for (int c = 0; c < (d + 31) / 32; ++c) {
+                                tm_ld32(t_o + 32 * c, x);
+                                tm_ld_wait();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) {
+                                    if (32 * c + e < d && mine_too) {
+                                        const float y = unpack16<BF16>(from[32 * c + e]);
+                                        if (!isfinite(y)) x[e] = __float_as_uint(__uint_as_float(x[e]) + y);
+                                    }
+                                }
+                                tm_st32(t_o + 32 * c, x);
+                            }
+                        }
+                        tm_st_wait();
+                    }
+                    asm volatile("bar.sync %0, %1;" ::"r"(PAIR ? 1 : 2 + s), "n"(PAIR ? 2 * kWideTile : kWideTile) : "memory");
+                }
+                tc_before();
+                mbar_arrive(&bar.weights[s]);
+                ++n_sums;
+            }
+            if (mine) wait(&bar.sums[s], (n_sums - 1) & 1, kStatusMmaTimeout);
+            tc_after();
+            first += 2 * n;
+
+            // ---- the item's sums
+            float log_top = top == -INFINITY ? -INFINITY : top * a.scale, scale = 1.f;
+            const bool whole = ua == 0 && ub == units;
+            float *part = a.parts + ((size_t)blockIdx.x * 2 + (ua == 0 ? 1 : 0)) * (size_t)(kRows * (D + 2));
+            const int part_row = PAIR ? s * kWideTile + row : row;
+            auto put = [&](int col, uint32_t (&v)[32]) {  // 32 columns of the row
+                if (whole) {
+                    const float inv = sum == 0.f || i >= len.rows ? 0.f : 1.f / sum;
+                    const bool none = sum == 0.f || i >= len.rows;
+                    if (i < a.rows) {
+                        uint8_t *out = a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + q_row % a.group) * d + col);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2)
+                            if (col + e < d) *reinterpret_cast<uint32_t *>(out + 2 * e) = none ? 0u : pack2<BF16>(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv);
+                    }
+                } else if (i < a.rows) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(part + part_row * D + col + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                }
+            };
+            uint32_t x[32];
+            if (PAIR) {
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    tm_ld32(t_o + 32 * c, x);
+                    tm_ld_wait();
+                    put(32 * c, x);
+                }
+            } else {
+                // slot 1 hands its sums to slot 0, half of the columns at a time, through the place of a second Q tile
+                float *hand = reinterpret_cast<float *>(smem + S::kTileBytes);  // [D / 2][128]
+                if (s == 1) {
+                    bar.top[row] = log_top;
+                    bar.sum[row] = sum;
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                float from1 = 0.f;
+                if (s == 0) {
+                    const float top1 = bar.top[row], both = fmaxf(log_top, top1), b = both == -INFINITY ? 0.f : both;
+                    scale = ex2(log_top - b);
+                    from1 = ex2(top1 - b);
+                    sum = sum * scale + bar.sum[row] * from1;
+                    log_top = both;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (s == 1) {
+#pragma unroll
+                        for (int c = 0; c < D / 64; ++c) {
+                            tm_ld32(t_o + h * (D / 2) + 32 * c, x);
+                            tm_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) hand[(32 * c + e) * kWideTile + row] = __uint_as_float(x[e]);
+                        }
+                    }
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    if (s == 0) {
+#pragma unroll
+                        for (int c = 0; c < D / 64; ++c) {
+                            tm_ld32(t_o + h * (D / 2) + 32 * c, x);
+                            tm_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * scale + hand[(32 * c + e) * kWideTile + row] * from1);
+                            put(h * (D / 2) + 32 * c, x);
+                        }
+                    }
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                }
+            }
+            if (!whole && (PAIR || s == 0)) {
+                part[kRows * D + part_row] = log_top;
+                part[kRows * D + kRows + part_row] = sum;
+            }
+            if (tid == 0 && ua == 0 && ub < units) {
+                const int64_t end = item_first + units;
+                a.info[blockIdx.x] = make_int4(seq, item, (int)((end * share.ctas - 1) / share.total) - (int)blockIdx.x + 1, len.rows);
+            }
+        }
+        tc_before();
+    }
+    __syncthreads();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+static int page_map(const zq_kv_cache *c, void *data, int box_rows, CUtensorMap *out, zq_error *err) {
+    EncodeTiledFn encode = get_encode_tiled(err);
+    if (!encode) return ZQ_ERR_CUDA;
+    const cuuint64_t dims[4] = {c->head_dim, c->heads, c->page_size, c->pages};
+    const cuuint64_t strides[3] = {c->head_dim * 2, c->heads * c->head_dim * 2, c->page_stride * 2};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)box_rows, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = encode(out, c->dtype == ZQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(err, ZQ_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d (cache of %zu pages of %zu x %zu x %zu)", (int)r, c->pages, c->page_size, c->heads, c->head_dim);
+    return ZQ_OK;
+}
+
+template <int D, bool BF16, bool PAIR> static int launch_wide(zq_ctx *ctx, AttnArgs &a, const zq_kv_cache *cache, zq_error *err) {
+    constexpr int kRows = PAIR ? 2 * kWideTile : kWideTile;
+    CUtensorMap map_k, map_v;
+    const int box_rows = cache->page_size < kWideTile ? (int)cache->page_size : kWideTile;
+    int rc = page_map(cache, cache->dev_k, box_rows, &map_k, err);
+    if (rc || (rc = page_map(cache, cache->dev_v, box_rows, &map_v, err))) return rc;
+    a.tiles = (a.rows * a.group + kRows - 1) / kRows;
+    const size_t ctas = (size_t)ctx->sm_count, bytes = ctas * 2 * kRows * (D + 2) * sizeof(float);
+    LaunchScratch scratch;
+    if ((rc = scratch.take(ctx, bytes + ctas * sizeof(int4), err))) return rc;
+    a.parts = static_cast<float *>(scratch.p);
+    a.info = reinterpret_cast<int4 *>(static_cast<uint8_t *>(scratch.p) + bytes);
+    ZQ_CUDA_CHECK(cudaFuncSetAttribute(wide_attention_kernel<D, BF16, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, WideShape<D>::kSmem), err);
+    rc = launch_pdl(ctx, wide_attention_kernel<D, BF16, PAIR>, dim3((unsigned)ctas), dim3(kWideThreads), WideShape<D>::kSmem, err, a, map_k, map_v);
+    if (rc) return rc;
+    return launch_attention_join(ctx, a, BF16, (int)ctas, kRows, D, err);
+}
+
+int launch_attention_wide(zq_ctx *ctx, AttnArgs &a, const zq_kv_cache *cache, bool &taken, zq_error *err) {
+    const int rows = a.rows * a.group, d = a.c.head_dim;
+    taken = rows > 16 && d >= 64 && d <= 128 && cache->page_size >= 8 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_stride % 8 == 0;
+    if (!taken) return ZQ_OK;
+    const bool bf16 = cache->dtype == ZQ_BF16, pair = rows > kWideTile;
+    if (d == 64) return bf16 ? (pair ? launch_wide<64, true, true>(ctx, a, cache, err) : launch_wide<64, true, false>(ctx, a, cache, err)) : pair ? launch_wide<64, false, true>(ctx, a, cache, err) : launch_wide<64, false, false>(ctx, a, cache, err);
+    return bf16 ? (pair ? launch_wide<128, true, true>(ctx, a, cache, err) : launch_wide<128, true, false>(ctx, a, cache, err)) : pair ? launch_wide<128, false, true>(ctx, a, cache, err) : launch_wide<128, false, false>(ctx, a, cache, err);
+}
+
+}  // namespace zq

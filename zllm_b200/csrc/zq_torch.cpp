@@ -107,14 +107,17 @@ struct NoGil {
 // without the GIL.  On the GPU from torch's allocator directly (0.4 us instead of the 0.8 of at::empty), by way of its hooks, so that this library
 // needs no CUDA build of torch to load, unless something is on that would see the call (dispatch modes, tracing, function transforms, autocast, the callbacks of
 // profilers) or fill the tensor.
-at::Tensor new_rows(const at::Tensor &like, size_t m, size_t n, at::ScalarType t) {
-    const int64_t size[2] = {(int64_t)m, (int64_t)n};
+at::Tensor new_tensor(const at::Tensor &like, at::IntArrayRef size, at::ScalarType t) {
     const bool watched = !(c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set).empty() || at::getStepCallbacksUnlessEmpty(at::RecordScope::FUNCTION).has_value();
     if (like.is_cuda() && !watched && !at::globalContext().deterministicAlgorithms()) {
         const c10::DeviceGuard on(like.device());
         return at::Tensor(at::detail::empty_generic(size, at::detail::getCUDAHooks().getCUDADeviceAllocator(), c10::DispatchKeySet(c10::DispatchKey::CUDA), t, std::nullopt));
     }
     return at::empty(size, like.options().dtype(t));
+}
+at::Tensor new_rows(const at::Tensor &like, size_t m, size_t n, at::ScalarType t) {
+    const int64_t size[2] = {(int64_t)m, (int64_t)n};
+    return new_tensor(like, size, t);
 }
 at::Tensor contiguous(const at::Tensor &t) {
     if (t.is_contiguous()) return t;
@@ -520,7 +523,6 @@ double number(PyObject *o) {
     if (v == -1.0 && PyErr_Occurred()) throw PyError();
     return v;
 }
-at::Tensor empty_like_sizes(const at::Tensor &like, at::IntArrayRef sizes, at::ScalarType t) { return at::empty(sizes, like.options().dtype(t).memory_format(at::MemoryFormat::Contiguous)); }
 
 // parents: [rows] for all sequences or [sequences, rows]
 struct Parents {
@@ -549,8 +551,8 @@ PyObject *py_draft_tree(PyObject *, PyObject *const *a, Py_ssize_t) {
         int rc;
         {
             NoGil g;
-            out[0] = empty_like_sizes(context, {batch, rows}, at::kInt);
-            out[1] = empty_like_sizes(context, {batch, rows, (rows + 63) / 64}, at::kLong);
+            out[0] = new_tensor(context, {batch, rows}, at::kInt);
+            out[1] = new_tensor(context, {batch, rows, (rows + 63) / 64}, at::kLong);
             rc = zq_draft_tree(ctx, parents.t.data_ptr<int>(), parents.shared, (size_t)batch, (size_t)rows, context.data_ptr<int>(), ints_or_null(drafted), out[0].data_ptr<int>(), reinterpret_cast<uint64_t *>(out[1].data_ptr<int64_t>()), &err);
         }
         check(rc, err);
@@ -580,8 +582,8 @@ PyObject *py_rope_rows(PyObject *, PyObject *const *a, Py_ssize_t) {
         int rc;
         {
             NoGil g;
-            out[0] = empty_like_sizes(q.t, q.t.sizes(), q.t.scalar_type());
-            if (k.t.defined()) out[1] = empty_like_sizes(k.t, k.t.sizes(), k.t.scalar_type());
+            out[0] = new_tensor(q.t, q.t.sizes(), q.t.scalar_type());
+            if (k.t.defined()) out[1] = new_tensor(k.t, k.t.sizes(), k.t.scalar_type());
             rc = zq_rope_rows(ctx, q.t.data_ptr(), (size_t)q.heads, (size_t)q.stride, k.t.defined() ? k.t.data_ptr() : nullptr, (size_t)k.heads, (size_t)k.stride, d, (size_t)q.rows, (size_t)q.dim, (size_t)(2 * inv_freq.numel()), interleaved, suffix,
                               positions.data_ptr<int>(), inv_freq.data_ptr<float>(), factor, inverse, out[0].data_ptr(), k.t.defined() ? out[1].data_ptr() : nullptr, &err);
         }
@@ -611,7 +613,7 @@ PyObject *py_rope_append(PyObject *, PyObject *const *a, Py_ssize_t) {
         int rc;
         {
             NoGil g;
-            out = empty_like_sizes(q.t, q.t.sizes(), q.t.scalar_type());
+            out = new_tensor(q.t, q.t.sizes(), q.t.scalar_type());
             rc = zq_rope_append(ctx, q.t.data_ptr(), (size_t)q.heads, (size_t)q.stride, k.t.data_ptr(), (size_t)k.stride, v.t.data_ptr(), (size_t)v.stride, (size_t)(q.rows / batch), &cache.c, ints_or_null(drafted), (size_t)(2 * inv_freq.numel()),
                                 interleaved, suffix, positions.data_ptr<int>(), inv_freq.data_ptr<float>(), factor, out.data_ptr(), &err);
         }
@@ -639,7 +641,7 @@ PyObject *py_tree_attention(PyObject *, PyObject *const *a, Py_ssize_t) {
         int rc;
         {
             NoGil g;
-            out = empty_like_sizes(q.t, q.t.sizes(), q.t.scalar_type());
+            out = new_tensor(q.t, q.t.sizes(), q.t.scalar_type());
             rc = zq_tree_attention(ctx, q.t.data_ptr(), (size_t)q.heads, (size_t)q.stride, (size_t)rows, &cache.c, mask.defined() ? reinterpret_cast<const uint64_t *>(mask.data_ptr<int64_t>()) : nullptr, ints_or_null(drafted), scale, out.data_ptr(),
                                    &err);
         }
@@ -671,9 +673,9 @@ PyObject *py_verify_draft(PyObject *, PyObject *const *a, Py_ssize_t) {
         int rc;
         {
             NoGil g;
-            out[0] = empty_like_sizes(logits, {batch, rows}, at::kInt);
-            out[1] = empty_like_sizes(logits, {batch}, at::kInt);
-            out[2] = empty_like_sizes(logits, {batch}, at::kInt);
+            out[0] = new_tensor(logits, {batch, rows}, at::kInt);
+            out[1] = new_tensor(logits, {batch}, at::kInt);
+            out[2] = new_tensor(logits, {batch}, at::kInt);
             rc = zq_verify_draft(ctx, logits.data_ptr(), draft.defined() ? draft.data_ptr() : nullptr, d, (size_t)batch, (size_t)rows, (size_t)logits.size(2), tokens.data_ptr<int>(), parents.t.data_ptr<int>(), parents.shared, accept_u.data_ptr<float>(),
                                  sample_u.data_ptr<float>(), heat.data_ptr<float>(), ints_or_null(drafted), out[0].data_ptr<int>(), out[1].data_ptr<int>(), out[2].data_ptr<int>(), &err);
         }

@@ -4,12 +4,16 @@
 // max(p - q, 0) / Z and the next child is tried.  Kept or drawn, tokens are then distributed as the target alone would draw them.
 //
 // The token drawn at the end is a whole number that a random number picks among a vocabulary's running sums, most of which lie closer
-// together than f32 tells apart (two f32 sums of 128 000 weights disagree about one pick in a hundred): weights and sums are f64.
+// together than f32 tells apart (two f32 sums of 128 000 weights disagree about one pick in a hundred): the weights of that pick and their sums
+// are f64, exact to 2e-12 (of the lightest tokens: in f32, see Weights).  A child's test has one border only; while none was rejected at a row, its sums are f32 inside a thread.
 //
 // Only rows on the walk are read, so the work is latency more than bytes: a cluster of CTAs per sequence shares a row (each CTA a
-// run of the vocabulary) and walks in step.  Each CTA takes its own largest logit, then its weights relative to that, kept as one sum per
-// segment of 256 tokens; the CTAs exchange two numbers per row through distributed shared memory and all come to the same
-// decision.  The pick looks for its CTA, then its segment, then its token, and evaluates one segment again.
+// run of the vocabulary) and walks in step: all CTAs exchange their sums through distributed shared memory, one barrier each time, and come to
+// the same decision.  A row is read once for its largest logit and sum (f32); where the walk ends, once more (from L2) for f64 weights,
+// kept as one sum per segment of tokens.  The pick looks for its CTA, then its segment, then its token, and evaluates one segment again.
+//
+// What rejections of drawn children leave has a closed form: after k of them p is (p - m q)+ / Z with m = 1 at first and m + Z after each, Z the
+// sum of (p - m q)+.  So a rejection is one pass, in f32 for the test of the next child and, for those of the last row only, in f64.
 #include <cooperative_groups.h>
 
 #include "zq_draft.cuh"
@@ -18,7 +22,10 @@ namespace zq {
 
 namespace cg = cooperative_groups;
 
-constexpr int kVerifyThreads = 1024, kVerifyWarps = kVerifyThreads / 32, kSegment = 256, kMaxCluster = 16;
+// 1024 threads of an SM in four CTAs: each pass waits for memory and for chains of dependent operations more than for issue slots (with 512 threads of
+// twice the tokens at a time 64 sequences of 128 003 tokens took 235 us, so 170).
+constexpr int kVerifyThreads = 256, kVerifyCtas = 4, kVerifyWarps = kVerifyThreads / 32, kMaxCluster = 16, kSegment = 256;  // tokens that a warp takes at a time and whose sum is kept
+constexpr float kHeavy = -18.f;  // weights above 2^kHeavy of the largest are evaluated in f64
 
 struct VerifyArgs {
     const uint8_t *logits, *draft;
@@ -30,21 +37,20 @@ struct VerifyArgs {
     uint32_t *status;
 };
 
-// What the CTAs of a cluster tell each other about a row.
+// A row's largest logit (NaN if the row holds one), its first place, and the sum of its weights relative to it.
 struct RowPart {
-    float top;    // largest logit of the CTA's run (NaN if it holds one)
-    int32_t at;   // its first place, greedy
-    double sum;   // of the weights relative to `top`
+    float top;
+    int32_t at;
+    double sum;
 };
 
 struct VerifyShared {
-    RowPart part[2][2][kMaxCluster];  // [exchange parity][target, draft]
-    double z[kMaxDraftRows];          // normalisers of the rejections at this row (drawn children)
+    RowPart part[2][2][kMaxCluster];  // [exchanges in turn][target, draft]: what the CTAs of the cluster tell each other
+    RowPart warp_part[2][kVerifyWarps];
     int32_t gone[kMaxDraftRows];      // rejected tokens at this row (chosen children)
-    double red[kVerifyWarps];
-    float red_top[kVerifyWarps];
-    int32_t red_at[kVerifyWarps];
-    int32_t pick;
+    int32_t parent[kMaxDraftRows], token[kMaxDraftRows];
+    float u[kMaxDraftRows];
+    float2 list[kVerifyWarps][kSegment];
 };
 
 template <class T> __device__ __forceinline__ float logit(const T *row, int64_t v) {
@@ -54,234 +60,343 @@ template <class T> __device__ __forceinline__ float logit(const T *row, int64_t 
 }
 
 // The eight values of a row from place v on; places outside [0, vocab) give -infinity.  v is a multiple of 8 less the row's
-// distance from a 16-byte boundary, so that whole vectors are aligned.
-template <class T> __device__ __forceinline__ void eight(const T *row, int64_t v, int64_t vocab, bool wide, float (&x)[8]) {
-    if (wide && v >= 0 && v + 8 <= vocab) {
-        constexpr int kPer = 16 / sizeof(T);
+// distance from a 16-byte boundary, so that whole vectors are aligned (wide).
+template <class T> struct Eight {
+    static constexpr int kPer = 16 / sizeof(T);
+    uint4 w[8 / kPer];
+    __device__ __forceinline__ void load(const T *row, int64_t v, int64_t vocab, bool wide) {
+        if (wide && v >= 0 && v + 8 <= vocab) {
 #pragma unroll
-        for (int j = 0; j < 8 / kPer; ++j) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(row + v + j * kPer);
-            const T *t = reinterpret_cast<const T *>(&w);
+            for (int j = 0; j < 8 / kPer; ++j) w[j] = *reinterpret_cast<const uint4 *>(row + v + j * kPer);
+        } else {
+            T x[8];
+            const float low = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) x[j * kPer + e] = logit(t, e);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = v + e >= 0 && v + e < vocab ? logit(row, v + e) : -INFINITY;
-    }
-}
-
-template <class T> struct Walk {
-    const VerifyArgs &a;
-    VerifyShared &s;
-    double *seg;  // sums of this CTA's segments
-    const T *row, *qrow;
-    double inv_t, p_top, p_inv, q_top, q_inv;  // 1 / temperature; largest logit and 1 / sum of the row's weights
-    int64_t shift, first, last;                // the row's distance from its boundary; this CTA's segments
-    int n_gone, n_z;
-    bool wide, q_wide, drawn;
-
-    __device__ double weight(float l, double top) const { return l == -INFINITY ? 0.0 : exp(((double)l - top) * inv_t); }
-    // What is left at the row of token v, up to a factor: z[0..n) have been divided by, one more subtraction with `open`.
-    __device__ double left(float l, float ql, int n, bool open) const {
-        double r = weight(l, p_top) * p_inv;
-        if (n == 0 && !open) return r;
-        const double q = weight(ql, q_top) * q_inv;
-        for (int i = 0; i < n; ++i) r = fmax(r - q, 0.0) / s.z[i];
-        return open ? fmax(r - q, 0.0) : r;
-    }
-    __device__ bool is_gone(int64_t v) const {
-        for (int i = 0; i < n_gone; ++i)
-            if (s.gone[i] == v) return true;
-        return false;
-    }
-    // Values of lane `lane` of segment g.
-    __device__ int64_t place(int64_t g, int lane) const { return g * kSegment + lane * 8 - shift; }
-    __device__ void lane_weights(int64_t g, int lane, int n, bool open, double (&w)[8]) const {
-        float x[8], y[8];
-        const int64_t v = place(g, lane);
-        eight(row, v, a.vocab, wide, x);
-        if (drawn && (n || open)) eight(qrow, v, a.vocab, q_wide, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            w[e] = n_gone && is_gone(v + e) ? 0.0 : left(x[e], drawn && (n || open) ? y[e] : 0.f, n, open);
+            for (int e = 0; e < 8; ++e) {
+                if (v + e >= 0 && v + e < vocab) x[e] = row[v + e];
+                else if constexpr (sizeof(T) == 4) x[e] = low;
+                else if constexpr (std::is_same<T, __half>::value) x[e] = __float2half_rn(low);
+                else x[e] = __float2bfloat16_rn(low);
+            }
+            memcpy(w, x, sizeof(x));
         }
     }
-    __device__ double block_sum(double x) const {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        __syncthreads();
-        if (lane == 0) s.red[warp] = x;
-        __syncthreads();
-        double t = 0;
-        for (int w = 0; w < kVerifyWarps; ++w) t += s.red[w];
-        return t;
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        T t[8];
+        memcpy(t, w, sizeof(t));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = logit(t, e);
     }
 };
 
-template <class T> __global__ void __launch_bounds__(kVerifyThreads, 1) verify_draft_kernel(const VerifyArgs a) {
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ double warp_sum(double x) {
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+// 2^((l - top) c) to 2e-12 of itself: 2^(n + j / 32 + r), |r| <= 1 / 64, with 2^(j / 32) from lane j of the warp and a Taylor sum of degree 4 for
+// 2^r; 11 f64 operations.  Below `low` (2^-900 of the largest) it is 0.  All lanes of the warp call it.
+//
+// light(): the same in f32, the argument to twice f32's bits, off by 2^-21 of the weight.  Of weights below 2^-18 of the largest that is
+// 2^-39 each, and of either sign: 128 000 of them move a running sum by less than 1e-9 of a border's usual distance.
+struct Weights {
+    double c, top;
+    float low, c_hi, c_lo, top32, least;
+    __device__ void set(double scale, float largest) {
+        c = scale;
+        top = (double)largest;
+        low = fmaxf((float)(top - 900.0 / c), -3.4028235e38f);
+        top32 = largest;
+        c_hi = (float)fmin(scale, 1e30);
+        c_lo = (float)(fmin(scale, 1e30) - (double)c_hi);
+        least = fmaxf(-200.f / c_hi, -3.4028235e38f);
+    }
+    __device__ __forceinline__ bool heavy(float l) const { return (l - top32) * c_hi > kHeavy; }
+    __device__ __forceinline__ float light(float l) const {
+        const float d = fmaxf(l - top32, least), y = d * c_hi;
+        float w = ex2(y);
+        w = fmaf(w * 0.69314718f, fmaf(d, c_lo, fmaf(d, c_hi, -y)), w);
+        return l == -INFINITY ? 0.f : w;
+    }
+    __device__ __forceinline__ double operator()(float l, double root) const {
+        constexpr double kMagic = 6755399441055744.0 / 32;  // 1.5 * 2^52 / 32: adding it leaves the number of 32nds in the low bits
+        const bool none = !(l >= low);
+        const double y = none ? 0.0 : ((double)l - top) * c;
+        const double t = y + kMagic;
+        const int k = __double2loint(t);
+        const double r = y - (t - kMagic);
+        double s = fma(r, 9.618129107628477e-3, 5.550410866482158e-2);
+        s = fma(r, s, 2.402265069591007e-1);
+        s = fma(r, s, 6.931471805599453e-1);
+        s = fma(r, s, 1.0);
+        s *= __shfl_sync(0xffffffffu, root, k & 31);
+        s = __hiloint2double(__double2hiint(s) + ((k >> 5) << 20), __double2loint(s));
+        return none ? 0.0 : s;
+    }
+};
+
+// The sum over a lane's tokens of `value` in f64 where a weight is heavy and of `light` elsewhere.  Few tokens are heavy: the warp lists them
+// and takes 32 at a time.
+template <class Heavy, class Value, class Light> __device__ __forceinline__ double lane_sum(float2 *list, const float (&l)[8], const float (&ql)[8], Heavy heavy, Value value, Light light) {
+    const int lane = threadIdx.x & 31;
+    unsigned heavies = 0;
+    float some = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float w = light(l[e], ql[e]);
+        const bool h = heavy(l[e], ql[e]);
+        if (h) heavies |= 1u << e;
+        some += h ? 0.f : w;
+    }
+    double t = (double)some;
+    const int mine = __popc(heavies);
+    int incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    if (total == 0) return t;
+    int at = incl - mine;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (heavies >> e & 1) list[at++] = make_float2(l[e], ql[e]);
+    __syncwarp();
+    for (int i = lane; i - lane < total; i += 32) {
+        const float2 x = list[min(i, total - 1)];
+        const double v = value(x.x, x.y);
+        if (i < total) t += v;
+    }
+    __syncwarp();
+    return t;
+}
+
+template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) verify_draft_kernel(const VerifyArgs a) {
     pdl_launch_dependents();
-    pdl_wait_prior_grid();
-    extern __shared__ double s_seg[];
+    extern __shared__ double s_seg[];  // sums of this CTA's segments
     __shared__ VerifyShared s;
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), seq = blockIdx.x / ctas;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const double root = exp2(lane / 32.0);
+    pdl_wait_prior_grid();
     const int n = draft_len(a.lens, seq, a.rows, a.status);
     const size_t row0 = (size_t)seq * a.rows;
-    const int32_t *parents = a.parents + (a.shared_parents ? 0 : row0);
     const float heat = a.temperature[seq];
-    const bool greedy = heat == 0.f;
-    Walk<T> w{a, s, s_seg};
-    w.inv_t = greedy ? 1.0 : 1.0 / (double)heat;
-    w.first = (int64_t)rank * a.segments;
-    w.last = w.first + a.segments;
-    w.drawn = a.draft != nullptr && !greedy;
+    for (int i = tid; i < n; i += kVerifyThreads) {
+        s.parent[i] = a.parents[(a.shared_parents ? 0 : row0) + i];
+        s.token[i] = a.tokens[row0 + i];
+        s.u[i] = a.accept_u[row0 + i];
+    }
+    __syncthreads();
+    const bool greedy = heat == 0.f, drawn = a.draft != nullptr && !greedy;
+    const double scale = 1.4426950408889634074 / (greedy ? 1.0 : (double)heat);
+    const float scale32 = (float)fmin(scale, 1e30);
+    const int64_t first = (int64_t)rank * a.segments, last = first + a.segments;
     int parity = 0, node = 0, count = 0, token = -1;
     bool bad = n > 0 && !(heat >= 0.f && heat < INFINITY);
 
-    // Largest logit (and its first place) of this CTA's run of a row.
-    auto find_top = [&](const T *row, int64_t shift, bool wide, float &top, int32_t &at) {
-        float m = -INFINITY;
-        int32_t where = 0x7fffffff;
-        bool nan = false;
-        for (int64_t g = w.first + warp; g < w.last; g += kVerifyWarps) {
-            float x[8];
-            const int64_t v = g * kSegment + lane * 8 - shift;
-            eight(row, v, a.vocab, wide, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                nan |= isnan(x[e]);
-                if (x[e] > m) {
-                    m = x[e];
-                    where = (int32_t)(v + e);
-                }
-            }
-        }
-        if (nan) m = NAN;
+    const T *row = nullptr, *qrow = nullptr;
+    int64_t shift = 0;
+    bool wide = false, q_wide = false;
+    Weights pw, qw;
+    double p_inv = 0, q_inv = 0;  // 1 / sum of weights
+    double m = 0, rest = 1;         // drawn children: p is (p - m q)+ / rest
+    int n_gone = 0;
+
+    // Joins (largest, place, sum) of the lanes of a warp; a NaN stays.
+    auto join_lanes = [&](RowPart p) {
+        RowPart m = p;
         for (int o = 16; o > 0; o >>= 1) {
-            const float om = __shfl_xor_sync(0xffffffffu, m, o);
-            const int32_t ow = __shfl_xor_sync(0xffffffffu, where, o);
-            if (isnan(om) || om > m || (om == m && ow < where)) {
-                m = om;
-                where = ow;
+            const float top = __shfl_xor_sync(0xffffffffu, m.top, o);
+            const int32_t at = __shfl_xor_sync(0xffffffffu, m.at, o);
+            if (isnan(top) || top > m.top || (top == m.top && at < m.at)) {
+                m.top = top;
+                m.at = at;
             }
         }
-        __syncthreads();
-        if (lane == 0) {
-            s.red_top[warp] = m;
-            s.red_at[warp] = where;
-        }
-        __syncthreads();
-        m = s.red_top[0];
-        where = s.red_at[0];
-        for (int i = 1; i < kVerifyWarps; ++i) {
-            const float om = s.red_top[i];
-            const int32_t ow = s.red_at[i];
-            if (isnan(om) || om > m || (om == m && ow < where)) {
-                m = om;
-                where = ow;
-            }
-        }
-        top = m;
-        at = where;
+        m.sum = warp_sum(p.top == -INFINITY ? 0.0 : p.sum * (double)exp2f((p.top - m.top) * scale32));
+        return m;
     };
-    // Sums of this CTA's segments of what is left at the row; their sum.
-    auto fill_segments = [&](int n_z, bool open) {
-        double mine = 0;
-        for (int64_t g = w.first + warp; g < w.last; g += kVerifyWarps) {
-            double x[8], t = 0;
-            w.lane_weights(g, lane, n_z, open, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t += x[e];
-            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-            if (lane == 0) {
-                s_seg[g - w.first] = t;
-                mine += t;
-            }
-        }
-        return w.block_sum(lane == 0 ? mine : 0.0);
-    };
-    // Every CTA gets every CTA's part; one barrier, two sets of places in turn.
-    auto exchange = [&](const RowPart &p, const RowPart &q) {
+    // Every CTA gets every CTA's part: the warps' parts are joined by the first warp, which stores the result into all CTAs.
+    auto exchange = [&](bool both, bool sums_only) {
         parity ^= 1;
-        if (tid < ctas) {
-            VerifyShared *other = cluster.map_shared_rank(&s, tid);
-            other->part[parity][0][rank] = p;
-            other->part[parity][1][rank] = q;
+        __syncthreads();
+        if (warp < (both ? 2 : 1)) {
+            RowPart p = lane < kVerifyWarps ? s.warp_part[warp][lane] : RowPart{-INFINITY, 0x7fffffff, 0.0};
+            if (sums_only) p.sum = warp_sum(p.sum);
+            else p = join_lanes(p);
+            if (lane < ctas) cluster.map_shared_rank(&s, lane)->part[parity][warp][rank] = p;
         }
         cluster.sync();
     };
-    // Largest logit and 1 / sum of a row from all CTAs' parts.
-    auto joined = [&](int which, double &top, double &inv, int32_t &at) {
-        float m = -INFINITY;
-        at = 0x7fffffff;
-        for (int i = 0; i < ctas; ++i) {
-            const RowPart &p = s.part[parity][which][i];
-            if (isnan(p.top) || p.top > m) {
-                m = p.top;
-                at = p.at;
-            }
-            if (isnan(m)) break;
-        }
-        top = m;
-        double sum = 0;
-        for (int i = 0; i < ctas; ++i) sum += s.part[parity][which][i].sum * w.weight(s.part[parity][which][i].top, top);
-        inv = 1.0 / sum;
-        return isfinite(m);
+    // Largest logit, its place and 1 / sum of a row from all CTAs' parts.
+    auto joined = [&](int which, Weights &w, double &inv, int32_t &at) {
+        const RowPart p = join_lanes(lane < ctas ? s.part[parity][which][lane] : RowPart{-INFINITY, 0x7fffffff, 0.0});
+        at = p.at;
+        inv = 1.0 / p.sum;
+        w.set(scale, p.top);
+        return isfinite(p.top);
     };
-    auto local_sum = [&](const T *row, int64_t shift, bool wide, float top, bool keep) {
-        double mine = 0;
-        for (int64_t g = w.first + warp; g < w.last; g += kVerifyWarps) {
-            float x[8];
-            eight(row, g * kSegment + lane * 8 - shift, a.vocab, wide, x);
-            double t = 0;
+    auto total_of = [&](int which) { return warp_sum(lane < ctas ? s.part[parity][which][lane].sum : 0.0); };
+    auto place = [&](int64_t g) { return g * kSegment + lane * 8 - shift; };
+    auto load = [&](const T *r, bool w, int64_t g, float (&l)[8]) {
+        Eight<T> x;
+        x.load(r, place(g), a.vocab, w);
+        x.get(l);
+    };
+    // The largest logit and the sum of weights of this CTA's run of a row, in f32 inside a thread.  A NaN makes the sum one.
+    struct Run {
+        float top = -INFINITY, sum = 0.f;
+        int32_t at = 0x7fffffff;
+    };
+    auto take = [&](Run &run, const float (&l)[8], int64_t g) {
+        float most = l[0];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) t += w.weight(x[e], top);
-            if (keep) {
-                for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-                if (lane == 0) s_seg[g - w.first] = t;
-                if (lane) t = 0;
+        for (int e = 1; e < 8; ++e) most = fmaxf(most, l[e]);
+        if (most > run.top) {
+            run.sum *= ex2((run.top - most) * scale32);
+            run.top = most;
+            int e0 = 7;
+#pragma unroll
+            for (int e = 7; e >= 0; --e)
+                if (l[e] == most) e0 = e;
+            run.at = (int32_t)(place(g) + e0);
+        }
+        const float base = run.top == -INFINITY ? 0.f : run.top;
+        float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[e & 3] += ex2((l[e] - base) * scale32);
+        run.sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    };
+    auto scan = [&](bool both) {
+        Run p, q;
+        for (int64_t g = first + warp; g < last; g += kVerifyWarps) {
+            Eight<T> x, y;
+            x.load(row, place(g), a.vocab, wide);
+            if (both) y.load(qrow, place(g), a.vocab, q_wide);
+            float l[8];
+            x.get(l);
+            take(p, l, g);
+            if (both) {
+                y.get(l);
+                take(q, l, g);
             }
+        }
+        const RowPart jp = join_lanes({isnan(p.sum) ? NAN : p.top, p.at, (double)p.sum});
+        if (lane == 0) s.warp_part[0][warp] = jp;
+        if (both) {
+            const RowPart jq = join_lanes({isnan(q.sum) ? NAN : q.top, q.at, (double)q.sum});
+            if (lane == 0) s.warp_part[1][warp] = jq;
+        }
+    };
+    // What is left of p at a token, times `rest`.  All lanes call it.
+    auto left = [&](float l, float ql, bool two) {
+        const double p = pw(l, root) * p_inv;
+        return two ? fmax(p - m * (qw(ql, root) * q_inv), 0.0) : p;
+    };
+    // Sum of a row's weights (its largest logit is known).
+    auto precise_sum = [&](const T *r, bool w, const Weights &weight, int which) {
+        double mine = 0;
+        for (int64_t g = first + warp; g < last; g += kVerifyWarps) {
+            float l[8];
+            load(r, w, g, l);
+            mine += lane_sum(s.list[warp], l, l, [&](float v, float) { return weight.heavy(v); }, [&](float v, float) { return weight(v, root); }, [&](float v, float) { return weight.light(v); });
+        }
+        mine = warp_sum(mine);
+        if (lane == 0) s.warp_part[which][warp] = {0.f, 0, mine};
+    };
+    // Takes the rejected tokens out of a lane's tokens of segment g.
+    auto drop_gone = [&](float (&l)[8], int64_t g) {
+        for (int i0 = 0; i0 < n_gone; i0 += 32) {
+            const int64_t d = i0 + lane < n_gone ? s.gone[i0 + lane] - (g * kSegment - shift) : -1;
+            unsigned hits = __ballot_sync(0xffffffffu, d >= 0 && d < kSegment);
+            while (hits) {
+                const int at = __shfl_sync(0xffffffffu, (int)d, __ffs(hits) - 1);
+                hits &= hits - 1;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (at == lane * 8 + e) l[e] = -INFINITY;
+            }
+        }
+    };
+    // The sums of the segments of what is left, times `rest`; of all of them, over the cluster.
+    auto fill_segments = [&](bool two) {
+        double mine = 0;
+        const float p32 = (float)p_inv, mq32 = (float)(m * q_inv);
+        for (int64_t g = first + warp; g < last; g += kVerifyWarps) {
+            float l[8];
+            double t;
+            load(row, wide, g, l);
+            if (two) {
+                float ql[8];
+                load(qrow, q_wide, g, ql);
+                t = lane_sum(s.list[warp], l, ql, [&](float v, float w) { return pw.heavy(v) || qw.heavy(w); }, [&](float v, float w) { return left(v, w, true); },
+                             [&](float v, float w) { return fmaxf(fmaf(-mq32, qw.light(w), p32 * pw.light(v)), 0.f); });
+            } else {
+                drop_gone(l, g);
+                t = lane_sum(s.list[warp], l, l, [&](float v, float) { return pw.heavy(v); }, [&](float v, float) { return left(v, v, false); }, [&](float v, float) { return p32 * pw.light(v); });
+            }
+            t = warp_sum(t);
+            if (lane == 0) s_seg[g - first] = t;
             mine += t;
         }
-        return w.block_sum(mine);
+        if (lane == 0) s.warp_part[0][warp] = {0.f, 0, mine};
+        exchange(false, true);
+        return total_of(0);
+    };
+    // The sum of what a rejection leaves, in f32 inside a thread.
+    auto light_rest = [&] {
+        float mine = 0.f;
+        const float p32 = (float)p_inv, mq32 = (float)(m * q_inv);
+        for (int64_t g = first + warp; g < last; g += kVerifyWarps) {
+            float l[8], ql[8];
+            load(row, wide, g, l);
+            load(qrow, q_wide, g, ql);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mine += fmaxf(fmaf(-mq32, ex2((ql[e] - qw.top32) * scale32), p32 * ex2((l[e] - pw.top32) * scale32)), 0.f);
+        }
+        const double t = warp_sum((double)mine);
+        if (lane == 0) s.warp_part[0][warp] = {0.f, 0, t};
+        exchange(false, true);
+        return total_of(0);
     };
 
     if (n > 0 && !bad) {
         count = 1;
         if (rank == 0 && tid == 0) a.path[row0] = 0;
         while (true) {
-            // ---- the row of the target, and of the draft where it has children
-            w.row = reinterpret_cast<const T *>(a.logits) + (row0 + node) * a.vocab;
-            w.shift = (int64_t)((reinterpret_cast<uintptr_t>(w.row) & 15) / sizeof(T));
-            w.wide = (reinterpret_cast<uintptr_t>(w.row) & (sizeof(T) - 1)) == 0;
-            w.n_gone = w.n_z = 0;
+            row = reinterpret_cast<const T *>(a.logits) + (row0 + node) * a.vocab;
+            shift = (int64_t)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+            wide = true;
+            n_gone = 0;
+            m = 0;
+            rest = 1;
             bool child = false;
-            for (int j = node + 1; j < n && !child; ++j) child = parents[j] == node;
-            RowPart p{-INFINITY, 0, 0}, q{-INFINITY, 0, 0};
-            find_top(w.row, w.shift, w.wide, p.top, p.at);
-            if (!greedy && p.top < INFINITY) p.sum = local_sum(w.row, w.shift, w.wide, p.top, true);
-            const bool use_q = w.drawn && child;
+            for (int j = node + 1; j < n && !child; ++j) child = s.parent[j] == node;
+            const bool use_q = drawn && child;
             if (use_q) {
-                w.qrow = reinterpret_cast<const T *>(a.draft) + (row0 + node) * a.vocab;
-                w.q_wide = ((reinterpret_cast<uintptr_t>(w.qrow) ^ reinterpret_cast<uintptr_t>(w.row)) & 15) == 0;
-                find_top(w.qrow, w.shift, w.q_wide, q.top, q.at);
-                if (q.top < INFINITY) q.sum = local_sum(w.qrow, w.shift, w.q_wide, q.top, false);
+                qrow = reinterpret_cast<const T *>(a.draft) + (row0 + node) * a.vocab;
+                q_wide = ((reinterpret_cast<uintptr_t>(qrow) ^ reinterpret_cast<uintptr_t>(row)) & 15) == 0;
             }
-            exchange(p, q);
+            scan(use_q);
+            exchange(use_q, false);
             int32_t best, unused;
-            bad = !joined(0, w.p_top, w.p_inv, best);
-            if (use_q) bad |= !joined(1, w.q_top, w.q_inv, unused);
+            bad = !joined(0, pw, p_inv, best);
+            if (use_q) bad |= !joined(1, qw, q_inv, unused);
             if (bad) break;
 
-            // ---- its children
             int next = -1;
-            bool stale = false;        // s_seg holds something else than what is left
-            double gone = 0;           // chosen children: what the rejected ones had of p
+            int rejected = 0;  // drawn children
+            double gone = 0;   // what the rejected chosen children had of p
             for (int j = node + 1; j < n; ++j) {
-                if (parents[j] != node) continue;
-                const int t = a.tokens[row0 + j];
+                if (s.parent[j] != node) continue;
+                const int t = s.token[j];
                 if (t < 0 || t >= a.vocab) {
                     if (tid == 0 && rank == 0) atomicMax(a.status, (uint32_t)kStatusBadIndex);
                     continue;
@@ -291,38 +406,35 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, 1) verify_d
                     if (next >= 0) break;
                     continue;
                 }
-                const double u = (double)a.accept_u[row0 + j];
-                const float l = logit(w.row, t);
-                if (w.drawn) {
-                    const float ql = logit(w.qrow, t);
-                    if (u * w.weight(ql, w.q_top) * w.q_inv < w.left(l, ql, w.n_z, false)) {
+                const double u = (double)s.u[j];
+                const float l = logit(row, t);
+                if (drawn) {
+                    const float ql = logit(qrow, t);
+                    if (u * qw(ql, root) * q_inv * rest < left(l, ql, true)) {
                         next = j;
                         break;
                     }
-                    const double mine = fill_segments(w.n_z, true);
-                    RowPart z{0, 0, mine};
-                    exchange(z, z);
-                    double sum = 0;
-                    for (int i = 0; i < ctas; ++i) sum += s.part[parity][0][i].sum;
-                    stale = !(sum > 0);
-                    if (sum > 0) {
-                        if (tid == 0) s.z[w.n_z] = sum;
-                        ++w.n_z;
-                    }
-                    __syncthreads();
+                    const double before = m;
+                    m += rest;
+                    const double sum = light_rest();
+                    if (sum > 0) rest = sum;
+                    else m = before;  // nothing left: p stays as it was
+                    ++rejected;
                 } else {
-                    const double chance = w.is_gone(t) ? 0.0 : w.weight(l, w.p_top) * w.p_inv;
+                    bool again = false;
+                    for (int i = 0; i < n_gone; ++i) again |= s.gone[i] == t;
+                    const double chance = again ? 0.0 : pw(l, root) * p_inv;
                     if (u < chance / (1.0 - gone)) {
                         next = j;
                         break;
                     }
-                    __syncthreads();
-                    if (tid == 0) s.gone[w.n_gone] = t;
-                    if (1.0 - gone - chance > 0) {
+                    if (!again && 1.0 - gone - chance > 0) {
+                        __syncthreads();
+                        if (tid == 0) s.gone[n_gone] = t;
                         gone += chance;
-                        ++w.n_gone;
+                        ++n_gone;
+                        __syncthreads();
                     }
-                    __syncthreads();
                 }
             }
             if (next >= 0) {
@@ -336,31 +448,28 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, 1) verify_d
                 break;
             }
             // ---- nobody kept: a token from what is left
-            __syncthreads();
-            if (stale) fill_segments(w.n_z, false);  // the last rejection left nothing, and p as it was before
-            double scale = 1.0;  // of the CTA's segments
-            if (!stale && w.n_z) {
-                scale = 1.0 / s.z[w.n_z - 1];
-            } else if (!stale) {     // those of p are relative to the CTA's own largest logit
-                scale = w.weight(p.top, w.p_top) * w.p_inv;
-                for (int i = warp; i < w.n_gone; i += kVerifyWarps) {  // without the rejected tokens
-                    const int64_t g = (s.gone[i] + w.shift) / kSegment;
-                    if (g >= w.first && g < w.last) {
-                        double x[8], t = 0;
-                        w.lane_weights(g, lane, 0, false, x);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) t += x[e];
-                        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-                        if (lane == 0) s_seg[g - w.first] = scale > 0 ? t / scale : 0.0;
+            bool filled = false;
+            if (rejected) {  // the rejections once more, in f64
+                precise_sum(row, wide, pw, 0);
+                precise_sum(qrow, q_wide, qw, 1);
+                exchange(true, true);
+                p_inv = 1.0 / total_of(0);
+                q_inv = 1.0 / total_of(1);
+                m = 0;
+                rest = 1;
+                for (int i = 0; i < rejected; ++i) {
+                    const double before = m;
+                    m += rest;
+                    const double sum = fill_segments(true);
+                    filled = sum > 0;
+                    if (!filled) {  // and so it would be for the others
+                        m = before;
+                        break;
                     }
+                    rest = sum;
                 }
             }
-            __syncthreads();
-            double mine = 0;
-            for (int64_t g = tid; g < a.segments; g += kVerifyThreads) mine += s_seg[g];
-            mine = w.block_sum(mine) * scale;
-            RowPart z{0, 0, mine};
-            exchange(z, z);
+            if (!filled) fill_segments(m > 0);
             double total = 0, before = 0, upto = 0;
             int owner = -1, some = 0;
             for (int i = 0; i < ctas; ++i) total += s.part[parity][0][i].sum;
@@ -379,11 +488,10 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, 1) verify_d
                 before = upto - s.part[parity][0][some].sum;
             }
             if (owner == rank && warp == 0) {
-                // the segment, 32 at a time
                 double at = before;
                 int64_t found = -1, likely = 0;
                 for (int64_t g0 = 0; g0 < a.segments && found < 0; g0 += 32) {
-                    const double x = g0 + lane < a.segments ? s_seg[g0 + lane] * scale : 0.0;
+                    const double x = g0 + lane < a.segments ? s_seg[g0 + lane] : 0.0;
                     double incl = x;
                     for (int o = 1; o < 32; o <<= 1) {
                         const double up = __shfl_up_sync(0xffffffffu, incl, o);
@@ -401,28 +509,31 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, 1) verify_d
                 }
                 const bool end = found < 0;
                 if (end) found = likely;
+                float l[8], ql[8];
+                load(row, wide, first + found, l);
+                if (m > 0) load(qrow, q_wide, first + found, ql);
+                drop_gone(l, first + found);
                 double x[8], t = 0;
-                w.lane_weights(w.first + found, lane, w.n_z, false, x);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t += x[e];
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = left(l[e], ql[e], m > 0);
+                    t += x[e];
+                }
                 double incl = t;
                 for (int o = 1; o < 32; o <<= 1) {
                     const double up = __shfl_up_sync(0xffffffffu, incl, o);
                     if (lane >= o) incl += up;
                 }
-                const unsigned over = __ballot_sync(0xffffffffu, !end && t > 0 && at + incl > target), any = __ballot_sync(0xffffffffu, t > 0);
-                const int l = over ? __ffs(over) - 1 : any ? 31 - __clz(any) : 0;
-                if (lane == l) {
-                    double run = at + incl - t;
-                    int pick = -1, last_seen = 0;
+                double run = at + incl - t;
+                int hit = -1, seen = -1;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        run += x[e];
-                        if (x[e] > 0) last_seen = e;
-                        if (pick < 0 && over && x[e] > 0 && run > target) pick = e;
-                    }
-                    a.token[seq] = (int32_t)(w.place(w.first + found, lane) + (pick < 0 ? last_seen : pick));
+                for (int e = 0; e < 8; ++e) {
+                    run += x[e];
+                    if (x[e] > 0) seen = e;
+                    if (hit < 0 && !end && x[e] > 0 && run > target) hit = e;
                 }
+                const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, seen >= 0);
+                if (lane == (hits ? __ffs(hits) - 1 : any ? 31 - __clz(any) : 0)) a.token[seq] = (int32_t)(place(first + found) + (hits ? hit : seen));
             }
             token = -2;  // written by its owner
             break;
@@ -473,9 +584,9 @@ extern "C" int zq_verify_draft(zq_ctx *ctx, const void *dev_logits, const void *
     if ((reinterpret_cast<uintptr_t>(dev_logits) | reinterpret_cast<uintptr_t>(dev_draft_logits)) & (dtype_size(dtype) - 1)) return set_error(err, ZQ_ERR_ARG, "zq_verify_draft: logits are not aligned to their type");
     int rc = use_device(ctx, err);
     if (rc) return rc;
-    // CTAs of a sequence: all SMs at work, at least 16 segments each
+    // CTAs of a sequence: several for each SM, so that the sequences that walk longest have the SMs of the others at the end; at least eight segments each
     int cluster = kMaxCluster;
-    while (cluster > 1 && (batch * cluster > (size_t)ctx->sm_count || vocab < (size_t)cluster * 16 * kSegment)) cluster /= 2;
+    while (cluster > 1 && (batch * cluster > kVerifyCtas * (size_t)ctx->sm_count || vocab < (size_t)cluster * 8 * kSegment)) cluster /= 2;
     VerifyArgs a = {};
     a.logits = static_cast<const uint8_t *>(dev_logits);
     a.draft = static_cast<const uint8_t *>(dev_draft_logits);
