@@ -17,6 +17,9 @@
 // Padding and the end of a sequence: boxes are whole pages, and what lies behind the sequence's end must not reach a row (0 * NaN): in tiles that hold
 // drafted rows or the end, a slot's threads clear those rows of V in shared memory, and infinities and NaN of drafted rows, which they
 // add to O of the rows that see them.
+#include <cstddef>
+#include <type_traits>
+
 #include "zq_attn.cuh"
 
 namespace zq {
@@ -30,7 +33,7 @@ __device__ __forceinline__ bool wide_elect() {
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t *bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
@@ -45,7 +48,12 @@ __device__ __forceinline__ void tm_ld32(uint32_t at, uint32_t (&r)[32]) {
         : "r"(at)
         : "memory");
 }
-__device__ __forceinline__ void tm_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for this thread's loads; the values pass through, so that nothing uses them before.
+__device__ __forceinline__ void tm_ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
 __device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
@@ -63,11 +71,48 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *m
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(head), "r"(row), "r"(page)
                  : "memory");
 }
+// Two f32 operations at once.
+__device__ __forceinline__ uint64_t pair64(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpair64(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t twice(float v) { return pair64(__float_as_uint(v), __float_as_uint(v)); }
+// 2^y of both halves on the FMA units, which have time where the exponential units have not: 2^n (n the nearest whole number) times a polynomial of degree 4
+// in the rest, fitted to the least relative error on [-1/2, 1/2] (2.7e-6, against 2^-12 of a weight's rounding).  y is at most about 8; below -126
+// it counts as -126.
+__device__ __forceinline__ void ex2_fma(uint64_t y, float &lo, float &hi) {
+    unpair64(y, lo, hi);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-126.f));
+    y = pair64(__float_as_uint(lo), __float_as_uint(hi));
+    const uint64_t t = add2(y, twice(12582912.f)), f = fma2(add2(t, twice(-12582912.f)), twice(-1.f), y);
+    uint64_t v = fma2(f, twice(0.0095701022f), twice(0.055917859f));
+    v = fma2(f, v, twice(0.24024744f));
+    v = fma2(f, v, twice(0.69312179f));
+    v = fma2(f, v, twice(0.99999928f));
+    float n_lo, n_hi;
+    unpair64(t, n_lo, n_hi);
+    unpair64(v, lo, hi);
+    lo = __uint_as_float(__float_as_uint(lo) + (__float_as_uint(n_lo) << 23));
+    hi = __uint_as_float(__float_as_uint(hi) + (__float_as_uint(n_hi) << 23));
+}
 // A tile of 128-byte swizzled rows, eight rows (1024 bytes) from one group to the next.  K-major (Q, K: a row is 64 values of the reduced
 // dimension): the leading offset is not used.  The other way round (V: a row is a key, the reduced dimension): the leading offset leads to the next 64 values.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t leading) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
+// sw128_low is the half that holds the address; one lane's value for the warp, so that the MMAs' operands are uniform registers.
+__device__ __forceinline__ uint32_t sw128_low(uint32_t addr, uint32_t leading) { return __shfl_sync(0xffffffffu, (addr & 0x3FFFFu) >> 4 | leading >> 4 << 16, 0); }
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t low) { return (uint64_t)low | (uint64_t)(1024 >> 4 | 1 << 14 | 2u << 29) << 32; }
 
 template <int D> struct WideShape {
     static constexpr int kBlocks = D / 64;
@@ -80,11 +125,12 @@ template <int D> struct WideShape {
 };
 
 struct WideBars {
-    uint64_t full[10], empty[10], scores[2], weights[2], sums[2], q[2], end;
+    uint64_t full[10], empty[10], scores[2], weights[2], sums[2], q[2], end;  // 8 bytes each, at kFull and so on
     uint32_t tmem, dead, poison[2][4];     // rows of a tile of V that were cleared of infinities and NaN, per slot
-    float top[kWideTile], sum[kWideTile];  // of slot 1's rows, when the slots share rows
+    float row[2][kWideTile];               // largest scores, then sums of the slots' rows, when the slots share rows
 };
-static_assert(sizeof(WideBars) <= 2048, "barriers");
+constexpr uint32_t kFull = 0, kEmpty = 80, kScores = 160, kWeights = 176, kSums = 192, kQ = 208, kEnd = 224;
+static_assert(sizeof(WideBars) <= 2048 && offsetof(WideBars, q) == kQ && offsetof(WideBars, end) == kEnd, "barriers");
 
 // 32 bits of a row's view of the drafted rows, from row d on (d may be negative: the context, which it sees).
 __device__ __forceinline__ uint32_t view32(const AttnArgs &a, int seq, int i, int d, int rows) {
@@ -109,6 +155,19 @@ __device__ __forceinline__ uint32_t view32(const AttnArgs &a, int seq, int i, in
     }
     const int n = rows - d;  // keys there are
     return n <= 0 ? 0u : n >= 32 ? v : v & ((1u << n) - 1);
+}
+
+__device__ __forceinline__ bool poll(uint32_t at, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(at), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __noinline__ void wait_on(uint32_t at, uint32_t parity, volatile uint32_t *dead, uint32_t *status, uint32_t code) {
+    for (uint32_t i = 0; i < (1u << 22); ++i) {
+        if (poll(at, parity) || *dead) return;
+    }
+    *dead = 1;
+    atomicMax(status, code);
 }
 
 template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideThreads, 1) wide_attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -150,20 +209,15 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = bar.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, bar.tmem, 0);
     const int d = a.c.head_dim;
 
     // Bounded wait of a whole warp.  One that runs out is reported, and from then on the CTA waits for nothing and walks to its end.
-    auto wait = [&](uint64_t *b, uint32_t parity, uint32_t code) {
-        bool ok = false;
-        for (uint32_t i = 0; i < (1u << 22) && !ok; ++i) {
-            ok = mbar_try_wait(b, parity);
-            if (!ok && *reinterpret_cast<volatile uint32_t *>(&bar.dead)) break;
-        }
-        if (!__all_sync(0xffffffffu, ok) && lane == 0) {
-            *reinterpret_cast<volatile uint32_t *>(&bar.dead) = 1;
-            atomicMax(a.status, code);
-        }
+    // (The first poll is in line and nearly always enough.  The MMA warp shares its scheduler's instruction cache with the long loops of the slots: its
+    // waits took 350 cycles each while they polled, voted and computed the barrier's place in 60 instructions.)
+    const uint32_t bars = base + S::kBars;
+    auto wait = [&](uint32_t offset, uint32_t parity, uint32_t code) {
+        if (!poll(bars + offset, parity)) wait_on(bars + offset, parity, &bar.dead, a.status, code);
         __syncwarp();
     };
 
@@ -210,7 +264,7 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                 ahead = page_of(t + 1);
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
-                    if (phase) wait(&bar.empty[at], (phase - 1) & 1, kStatusMmaTimeout);
+                    if (phase) wait(kEmpty + 8 * at, (phase - 1) & 1, kStatusMmaTimeout);
                     if (wide_elect()) mbar_expect_tx(&bar.full[at], S::kTileBytes);
                     __syncwarp();
                     if (lane < boxes) {
@@ -237,56 +291,71 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
         const uint32_t type = BF16 ? 1u << 7 | 1u << 10 : 0u;
         const uint32_t idesc_s = 1u << 4 | type | (uint32_t)(kWideTile >> 3) << 17 | (uint32_t)(kWideTile >> 4) << 24;
         const uint32_t idesc_o = 1u << 4 | type | 1u << 16 | (uint32_t)(D >> 3) << 17 | (uint32_t)(kWideTile >> 4) << 24;
-        const int k_steps = (d + 15) / 16;
-        uint32_t first = 0;  // tiles of the ring used by earlier items
         uint32_t q_phase = 0, w_phase[2] = {0, 0};
-        auto slot_of = [&](uint32_t n) { return n % S::kRing; };
-        auto wait_tile = [&](uint32_t n) { wait(&bar.full[n % S::kRing], n / S::kRing & 1, kStatusTmaTimeout); };
+        struct Place {  // in the ring: K tiles take every other one, V tiles those between
+            uint32_t slot, parity;
+            __device__ __forceinline__ void step() {
+                slot += 2;
+                if (slot >= S::kRing) {
+                    slot -= S::kRing;
+                    parity ^= 1;
+                }
+            }
+        } k_at{0, 0}, v_at{1, 0};
+        const uint32_t ring_k = sw128_low(base + S::kRingAt, 16), ring_v = sw128_low(base + S::kRingAt, S::kBlock);
+        const uint32_t q_low[2] = {sw128_low(base + S::kQ, 16), sw128_low(base + S::kQ + (PAIR ? S::kTileBytes : 0), 16)};
+        // products of slot s: scores with the K tile at k_at, sums with the V tile at v_at
+        auto scores = [&](int s) {
+            if (!PAIR || s == 0) wait(kFull + 8 * k_at.slot, k_at.parity, kStatusTmaTimeout);
+            tc_after();
+            const uint32_t kd = __shfl_sync(0xffffffffu, ring_k + k_at.slot * (S::kTileBytes / 16), 0), release = bars + kEmpty + 8 * k_at.slot;
+            if (wide_elect()) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k >> 2) * (S::kBlock / 16) + (k & 3) * 2;
+                    mma_ss(tmem + s * 256, sw128_desc(q_low[s] + off), sw128_desc(kd + off), idesc_s, k > 0);
+                }
+                tc_commit(bars + kScores + 8 * s);
+                if (!PAIR || s == 1) tc_commit(release);
+            }
+            __syncwarp();
+            if (!PAIR || s == 1) k_at.step();
+        };
+        auto sums = [&](int s) {
+            if (!PAIR || s == 0) wait(kFull + 8 * v_at.slot, v_at.parity, kStatusTmaTimeout);
+            wait(kWeights + 8 * s, w_phase[s], kStatusMmaTimeout);
+            w_phase[s] ^= 1;
+            tc_after();
+            const uint32_t vd = __shfl_sync(0xffffffffu, ring_v + v_at.slot * (S::kTileBytes / 16), 0), release = bars + kEmpty + 8 * v_at.slot;
+            if (wide_elect()) {
+#pragma unroll
+                for (int k = 0; k < kWideTile / 16; ++k) mma_ts(tmem + s * 256 + 128, tmem + s * 256 + 8 * k, sw128_desc(vd + k * (2048 / 16)), idesc_o);
+                tc_commit(bars + kSums + 8 * s);
+                if (!PAIR || s == 1) tc_commit(release);
+            }
+            __syncwarp();
+            if (!PAIR || s == 1) v_at.step();
+        };
         while (next_item()) {
             const int n = ub - ua, jobs = PAIR ? 2 * n : n;
-            wait(&bar.q[0], q_phase, kStatusMmaTimeout);
-            if (PAIR) wait(&bar.q[1], q_phase, kStatusMmaTimeout);
+            wait(kQ, q_phase, kStatusMmaTimeout);
+            if (PAIR) wait(kQ + 8, q_phase, kStatusMmaTimeout);
             q_phase ^= 1;
-            auto scores = [&](int j) {
-                const int i = PAIR ? j >> 1 : j, s = j & 1;
-                const uint32_t k_tile = first + 2 * i;
-                if (!PAIR || s == 0) wait_tile(k_tile);
-                tc_after();
-                const uint64_t qd = sw128_desc(base + S::kQ + (PAIR ? s : 0) * S::kTileBytes, 16), kd = sw128_desc(base + S::kRingAt + slot_of(k_tile) * S::kTileBytes, 16);
-                if (wide_elect()) {
-                    for (int k = 0; k < k_steps; ++k) {
-                        const uint32_t off = (k >> 2) * (S::kBlock / 16) + (k & 3) * 2;
-                        mma_ss(tmem + s * 256, qd + off, kd + off, idesc_s, k > 0);
-                    }
-                    tc_commit(&bar.scores[s]);
-                    if (!PAIR || s == 1) tc_commit(&bar.empty[slot_of(k_tile)]);
-                }
-                __syncwarp();
-            };
-            if (jobs > 0) scores(0);
+            scores(0);
             if (jobs > 1) scores(1);
-            for (int j = 0; j < jobs; ++j) {
-                const int i = PAIR ? j >> 1 : j, s = j & 1;
-                const uint32_t v_tile = first + 2 * i + 1;
-                if (!PAIR || s == 0) wait_tile(v_tile);
-                wait(&bar.weights[s], w_phase[s], kStatusMmaTimeout);
-                w_phase[s] ^= 1;
-                tc_after();
-                const uint64_t vd = sw128_desc(base + S::kRingAt + slot_of(v_tile) * S::kTileBytes, S::kBlock);
-                if (wide_elect()) {
-#pragma unroll
-                    for (int k = 0; k < kWideTile / 16; ++k) mma_ts(tmem + s * 256 + 128, tmem + s * 256 + 8 * k, vd + k * (2048 / 16), idesc_o);
-                    tc_commit(&bar.sums[s]);
-                    if (!PAIR || s == 1) tc_commit(&bar.empty[slot_of(v_tile)]);
+#pragma unroll 1
+            for (int j = 0; j < jobs; j += 2) {
+                sums(0);
+                if (j + 2 < jobs) scores(0);
+                if (j + 1 < jobs) {
+                    sums(1);
+                    if (j + 3 < jobs) scores(1);
                 }
-                __syncwarp();
-                if (j + 2 < jobs) scores(j + 2);
             }
-            first += 2 * n;
         }
-        if (wide_elect()) tc_commit(&bar.end);
+        if (wide_elect()) tc_commit(bars + kEnd);
         __syncwarp();
-        wait(&bar.end, 0, kStatusMmaTimeout);
+        wait(kEnd, 0, kStatusMmaTimeout);
     } else {
         // ---- scores to weights
         const int s = warp >> 2, row = tid & 127;
@@ -301,12 +370,18 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
             if (PAIR || s == 0) {
                 uint8_t *q_tile = smem + S::kQ + s * S::kTileBytes;
                 const int r0 = tile * kRows + s * kWideTile, n_rows = len.rows * a.group;
-                for (int idx = row; idx < kWideTile * (D / 8); idx += kWideTile) {
-                    const int r = idx / (D / 8), c = idx % (D / 8), q_row = r0 + r;
-                    uint4 v = make_uint4(0, 0, 0, 0);
+                uint4 v[D / 8];
+#pragma unroll
+                for (int k = 0; k < D / 8; ++k) {
+                    const int r = (k * kWideTile + row) / (D / 8), c = row % (D / 8), q_row = r0 + r;
+                    v[k] = make_uint4(0, 0, 0, 0);
                     if (q_row < n_rows && c < chunks)
-                        v = *reinterpret_cast<const uint4 *>(a.q + 2 * (((int64_t)seq * a.rows + q_row / a.group) * a.q_stride + (int64_t)(head * a.group + q_row % a.group) * d + 8 * c));
-                    *reinterpret_cast<uint4 *>(q_tile + (c >> 3) * S::kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+                        v[k] = *reinterpret_cast<const uint4 *>(a.q + 2 * (((int64_t)seq * a.rows + q_row / a.group) * a.q_stride + (int64_t)(head * a.group + q_row % a.group) * d + 8 * c));
+                }
+#pragma unroll
+                for (int k = 0; k < D / 8; ++k) {
+                    const int r = (k * kWideTile + row) / (D / 8), c = row % (D / 8);
+                    *reinterpret_cast<uint4 *>(q_tile + (c >> 3) * S::kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
                 }
                 fence_proxy_async();
             }
@@ -328,71 +403,97 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
 #pragma unroll
                     for (int c = 0; c < 4; ++c) seen[c] = view32(a, seq, i, key0 + 32 * c - len.context, len.rows);
                 }
-                wait(&bar.scores[s], s_phase, kStatusMmaTimeout);
+                wait(kScores + 8 * s, s_phase, kStatusMmaTimeout);
                 s_phase ^= 1;
                 tc_after();
-                float m = -INFINITY;
-                uint32_t x[32];
+                // Four chunks of 32 scores; the next one comes while one is worked on.  The weights are taken relative to the maximum of earlier tiles
+                // and stay in registers until it is clear that this tile's is no more than 2^8 above it, as hardly any is after the first.
+                uint32_t za[32], zb[32], p[64];
+                auto hide = [&](uint32_t (&z)[32], uint32_t view) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tm_ld32(t_s + 32 * c, x);
-                    tm_ld_wait();
-                    if (masked) {
+                    for (int e = 0; e < 32; ++e)
+                        if (!(view >> e & 1)) z[e] = 0xff800000u;
+                };
+                auto most = [&](float m, const uint32_t (&z)[32]) {
+                    float n = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!(seen[c] >> e & 1)) x[e] = 0xff800000u;
+                    for (int e = 0; e < 32; e += 4) {
+                        m = fmaxf(fmaxf(m, __uint_as_float(z[e])), __uint_as_float(z[e + 1]));
+                        n = fmaxf(fmaxf(n, __uint_as_float(z[e + 2])), __uint_as_float(z[e + 3]));
                     }
-                    float part[4] = {m, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) part[e & 3] = fmaxf(part[e & 3], __uint_as_float(x[e]));
-                    m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-                }
-                // rises by less than 2^8 stay in the weights
-                const bool rise = m > top && (top == -INFINITY || (m - top) * a.scale > 8.f);
-                if (__any_sync(0xffffffffu, rise && top != -INFINITY)) {
-                    const float down = rise && top != -INFINITY ? ex2((top - m) * a.scale) : 1.f;
-                    if (job) wait(&bar.sums[s], (n_sums - 1) & 1, kStatusMmaTimeout);
-                    tc_after();
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        tm_ld32(t_o + 32 * c, x);
-                        tm_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
-                        tm_st32(t_o + 32 * c, x);
-                    }
-                    tm_st_wait();
-                    sum *= down;
-                }
-                if (rise) top = m;
-                const float off = top == -INFINITY ? 0.f : top * a.scale;
-                float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tm_ld32(t_s + 32 * c, x);
-                    tm_ld_wait();
-                    uint32_t p[16];
+                    return fmaxf(m, n);
+                };
+                const uint64_t scale2 = twice(a.scale);
+                uint64_t off2, sums[2];
+                auto weigh = [&](const uint32_t (&z)[32], int c, auto partly) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        float lo = ex2(fmaf(__uint_as_float(x[e]), a.scale, -off)), hi = ex2(fmaf(__uint_as_float(x[e + 1]), a.scale, -off));
-                        if (masked) {
-                            if (!(seen[c] >> e & 1)) lo = 0.f;
-                            if (!(seen[c] >> (e + 1) & 1)) hi = 0.f;
+                        const uint64_t y = fma2(pair64(z[e], z[e + 1]), scale2, off2);
+                        float lo, hi;
+                        if ((e & 6) == 6 && !decltype(partly)::value) {
+                            ex2_fma(y, lo, hi);
+                        } else {
+                            unpair64(y, lo, hi);
+                            lo = ex2(lo);
+                            hi = ex2(hi);
                         }
-                        sums[e >> 1 & 3] += lo + hi;
-                        p[e >> 1] = pack2<BF16>(lo, hi);
+                        sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair64(__float_as_uint(lo), __float_as_uint(hi)));
+                        p[16 * c + (e >> 1)] = pack2<BF16>(lo, hi);
                     }
-                    tm_st16(t_s + 16 * c, p);  // over the first half of scores that are read already
+                };
+                float m = -INFINITY;
+                auto pass = [&](auto partly) {
+                    off2 = twice(top == -INFINITY ? 0.f : -top * a.scale);
+                    sums[0] = sums[1] = 0;
+                    tm_ld32(t_s, za);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t(&z)[32] = c & 1 ? zb : za;
+                        tm_ld_wait(z);
+                        if (c < 3) tm_ld32(t_s + 32 * (c + 1), c & 1 ? za : zb);
+                        if (decltype(partly)::value) hide(z, seen[c]);
+                        m = most(m, z);
+                        weigh(z, c, partly);
+                    }
+                };
+#pragma unroll 1
+                while (true) {
+                    if (masked) pass(std::true_type{});
+                    else pass(std::false_type{});
+                    const bool rise = top == -INFINITY ? m > top : (m - top) * a.scale > 8.f;
+                    if (!__any_sync(0xffffffffu, rise)) break;
+                    const float down = rise && top != -INFINITY ? ex2((top - m) * a.scale) : 1.f;
+                    if (__any_sync(0xffffffffu, down != 1.f)) {
+                        if (job) wait(kSums + 8 * s, (n_sums - 1) & 1, kStatusMmaTimeout);
+                        tc_after();
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            tm_ld32(t_o + 32 * c, za);
+                            tm_ld_wait(za);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) za[e] = __float_as_uint(__uint_as_float(za[e]) * down);
+                            tm_st32(t_o + 32 * c, za);
+                        }
+                        tm_st_wait();
+                        sum *= down;
+                    }
+                    if (rise) top = m;
                 }
+                tm_st32(t_s, *reinterpret_cast<uint32_t(*)[32]>(p));
+                tm_st32(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
                 tm_st_wait();
-                sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                {
+                    float lo, hi;
+                    unpair64(add2(sums[0], sums[1]), lo, hi);
+                    sum += lo + hi;
+                }
 
                 if (masked) {
                     // clear what nobody may meet in V; slot 0 does it for both where they share the keys
                     const uint32_t v_tile = first + 2 * step + 1;
                     uint8_t *v = smem + S::kRingAt + v_tile % S::kRing * S::kTileBytes;
                     if (!PAIR || s == 0) {
-                        wait(&bar.full[v_tile % S::kRing], v_tile / S::kRing & 1, kStatusTmaTimeout);
+                        wait(kFull + 8 * (v_tile % S::kRing), v_tile / S::kRing & 1, kStatusTmaTimeout);
                         bool dropped = false;
                         const int key = key0 + row;
                         if (key >= (len.rows ? len.context : 0)) {
@@ -422,7 +523,7 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
 #pragma unroll
                     for (int c = 0; c < 4; ++c) poison[c] = bar.poison[PAIR ? 0 : s][c];
                     if (poison[0] | poison[1] | poison[2] | poison[3]) {
-                        if (job) wait(&bar.sums[s], (n_sums - 1) & 1, kStatusMmaTimeout);
+                        if (job) wait(kSums + 8 * s, (n_sums - 1) & 1, kStatusMmaTimeout);
                         tc_after();
                         for (int r = 0; r < kWideTile; ++r) {
                             const uint32_t bad = r < 32 ? poison[0] : r < 64 ? poison[1] : r < 96 ? poison[2] : poison[3], view = r < 32 ? seen[0] : r < 64 ? seen[1] : r < 96 ? seen[2] : seen[3];
@@ -433,8 +534,9 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                             const uint16_t *from = reinterpret_cast<const uint16_t *>(a.c.v) + at + (int64_t)head * d;
 #pragma unroll 1
                             for (int c = 0; c < (d + 31) / 32; ++c) {
+                                uint32_t x[32];
                                 tm_ld32(t_o + 32 * c, x);
-                                tm_ld_wait();
+                                tm_ld_wait(x);
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) {
                                     if (32 * c + e < d && mine_too) {
@@ -453,83 +555,92 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                 mbar_arrive(&bar.weights[s]);
                 ++n_sums;
             }
-            if (mine) wait(&bar.sums[s], (n_sums - 1) & 1, kStatusMmaTimeout);
+            if (mine) wait(kSums + 8 * s, (n_sums - 1) & 1, kStatusMmaTimeout);
             tc_after();
             first += 2 * n;
 
             // ---- the item's sums
-            float log_top = top == -INFINITY ? -INFINITY : top * a.scale, scale = 1.f;
             const bool whole = ua == 0 && ub == units;
             float *part = a.parts + ((size_t)blockIdx.x * 2 + (ua == 0 ? 1 : 0)) * (size_t)(kRows * (D + 2));
             const int part_row = PAIR ? s * kWideTile + row : row;
-            auto put = [&](int col, uint32_t (&v)[32]) {  // 32 columns of the row
-                if (whole) {
-                    const float inv = sum == 0.f || i >= len.rows ? 0.f : 1.f / sum;
-                    const bool none = sum == 0.f || i >= len.rows;
-                    if (i < a.rows) {
-                        uint8_t *out = a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + q_row % a.group) * d + col);
+            // first value of this thread's row in the output or in the part
+            const int64_t to = i >= a.rows ? -1 : whole ? (((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + q_row % a.group) * d : (int64_t)part_row * D;
+            uint8_t *stage = smem + S::kQ + s * S::kTileBytes;  // of Q, which is through: [128][D / 2] f32, chunks swizzled
+            // Half h of the columns of the warp's 32 rows leaves by way of shared memory, whole lines at a time.
+            auto put = [&](int h, const float (&y)[D / 2]) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2)
-                            if (col + e < d) *reinterpret_cast<uint32_t *>(out + 2 * e) = none ? 0u : pack2<BF16>(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv);
-                    }
-                } else if (i < a.rows) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(part + part_row * D + col + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                for (int c = 0; c < D / 8; ++c) *reinterpret_cast<float4 *>(stage + row * (2 * D) + ((c ^ (row & 7)) << 4)) = make_float4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+                __syncwarp();
+#pragma unroll 8
+                for (int k = 0; k < D / 4; ++k) {
+                    const int r = (32 * k + lane) / (D / 4), c = (32 * k + lane) % (D / 4), col = h * (D / 2) + 2 * c, at_row = (row & ~31) + r;
+                    const int64_t at = __shfl_sync(0xffffffffu, to, r);
+                    const float2 v = *reinterpret_cast<const float2 *>(stage + at_row * (2 * D) + (((c >> 1) ^ (at_row & 7)) << 4) + 8 * (c & 1));
+                    if (at < 0) continue;
+                    if (!whole) *reinterpret_cast<float2 *>(part + at + col) = v;
+                    else if (col < d) *reinterpret_cast<uint32_t *>(a.out + 2 * (at + col)) = pack2<BF16>(v.x, v.y);
                 }
+                __syncwarp();
             };
-            uint32_t x[32];
+            float log_top = top == -INFINITY ? -INFINITY : top * a.scale;
+            float y[D / 2];
             if (PAIR) {
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    tm_ld32(t_o + 32 * c, x);
-                    tm_ld_wait();
-                    put(32 * c, x);
-                }
-            } else {
-                // slot 1 hands its sums to slot 0, half of the columns at a time, through the place of a second Q tile
-                float *hand = reinterpret_cast<float *>(smem + S::kTileBytes);  // [D / 2][128]
-                if (s == 1) {
-                    bar.top[row] = log_top;
-                    bar.sum[row] = sum;
-                }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                float from1 = 0.f;
-                if (s == 0) {
-                    const float top1 = bar.top[row], both = fmaxf(log_top, top1), b = both == -INFINITY ? 0.f : both;
-                    scale = ex2(log_top - b);
-                    from1 = ex2(top1 - b);
-                    sum = sum * scale + bar.sum[row] * from1;
-                    log_top = both;
-                }
+                const float inv = !whole ? 1.f : sum == 0.f || i >= len.rows ? 0.f : 1.f / sum;
+                const bool none = whole && (sum == 0.f || i >= len.rows);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    if (s == 1) {
 #pragma unroll
-                        for (int c = 0; c < D / 64; ++c) {
-                            tm_ld32(t_o + h * (D / 2) + 32 * c, x);
-                            tm_ld_wait();
+                    for (int c = 0; c < D / 64; ++c) {
+                        uint32_t x[32];
+                        tm_ld32(t_o + h * (D / 2) + 32 * c, x);
+                        tm_ld_wait(x);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) hand[(32 * c + e) * kWideTile + row] = __uint_as_float(x[e]);
-                        }
+                        for (int e = 0; e < 32; ++e) y[32 * c + e] = none ? 0.f : __uint_as_float(x[e]) * inv;
                     }
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    if (s == 0) {
-#pragma unroll
-                        for (int c = 0; c < D / 64; ++c) {
-                            tm_ld32(t_o + h * (D / 2) + 32 * c, x);
-                            tm_ld_wait();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * scale + hand[(32 * c + e) * kWideTile + row] * from1);
-                            put(h * (D / 2) + 32 * c, x);
-                        }
-                    }
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    put(h, y);
                 }
+            } else {
+                // each slot finishes half of the columns: it hands the other half of its sums over, relative to both slots' maximum
+                bar.row[s][row] = log_top;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const float both = fmaxf(log_top, bar.row[1 - s][row]), scale = both == -INFINITY ? 0.f : ex2(log_top - both);
+                float *hand = reinterpret_cast<float *>(stage);  // [D / 2][128]
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c) {
+                    uint32_t x[32];
+                    tm_ld32(t_o + (1 - s) * (D / 2) + 32 * c, x);
+                    tm_ld_wait(x);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) hand[(32 * c + e) * kWideTile + row] = scale == 0.f ? 0.f : __uint_as_float(x[e]) * scale;
+                }
+                sum = scale == 0.f ? 0.f : sum * scale;
+                log_top = both;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                bar.row[s][row] = sum;
+                const float *from = reinterpret_cast<const float *>(smem + S::kQ + (1 - s) * S::kTileBytes);
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c) {
+                    uint32_t x[32];
+                    tm_ld32(t_o + s * (D / 2) + 32 * c, x);
+                    tm_ld_wait(x);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) y[32 * c + e] = (scale == 0.f ? 0.f : __uint_as_float(x[e]) * scale) + from[(32 * c + e) * kWideTile + row];
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                sum += bar.row[1 - s][row];
+                if (whole) {
+                    const bool none = sum == 0.f || i >= len.rows;
+                    const float inv = none ? 0.f : 1.f / sum;
+#pragma unroll
+                    for (int e = 0; e < D / 2; ++e) y[e] = none ? 0.f : y[e] * inv;
+                }
+                put(s, y);
             }
             if (!whole && (PAIR || s == 0)) {
                 part[kRows * D + part_row] = log_top;
                 part[kRows * D + kRows + part_row] = sum;
             }
+            asm volatile("bar.sync %0, %1;" ::"r"(PAIR ? 2 + s : 1), "n"(PAIR ? kWideTile : 2 * kWideTile) : "memory");  // the next item's rows of Q and maxima go where these sums were
             if (tid == 0 && ua == 0 && ub < units) {
                 const int64_t end = item_first + units;
                 a.info[blockIdx.x] = make_int4(seq, item, (int)((end * share.ctas - 1) / share.total) - (int)blockIdx.x + 1, len.rows);
@@ -573,7 +684,7 @@ template <int D, bool BF16, bool PAIR> static int launch_wide(zq_ctx *ctx, AttnA
 
 int launch_attention_wide(zq_ctx *ctx, AttnArgs &a, const zq_kv_cache *cache, bool &taken, zq_error *err) {
     const int rows = a.rows * a.group, d = a.c.head_dim;
-    taken = rows > 16 && d >= 64 && d <= 128 && cache->page_size >= 8 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_stride % 8 == 0;
+    taken = rows > 16 && d >= 64 && d <= 128 && cache->page_size >= 8 && ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 && a.q_stride % 8 == 0;
     if (!taken) return ZQ_OK;
     const bool bf16 = cache->dtype == ZQ_BF16, pair = rows > kWideTile;
     if (d == 64) return bf16 ? (pair ? launch_wide<64, true, true>(ctx, a, cache, err) : launch_wide<64, true, false>(ctx, a, cache, err)) : pair ? launch_wide<64, false, true>(ctx, a, cache, err) : launch_wide<64, false, false>(ctx, a, cache, err);
