@@ -120,17 +120,17 @@ template <int D> struct WideShape {
     static constexpr int kTileBytes = kBlocks * kBlock;
     static constexpr int kRing = D == 128 ? 5 : 10;     // K and V tiles
     static constexpr int kQ = 0, kRingAt = 2 * kTileBytes, kBars = kRingAt + kRing * kTileBytes;
-    static constexpr int kSmem = kBars + 2048 + 1024;   // barriers, maxima and sums of slot 1; alignment
+    static constexpr int kSmem = kBars + 3072;          // barriers, maxima and sums of the slots' rows
     static_assert(kSmem <= 227 << 10, "shared memory");
 };
 
 struct WideBars {
     uint64_t full[10], empty[10], scores[2], weights[2], sums[2], q[2], end;  // 8 bytes each, at kFull and so on
     uint32_t tmem, dead, poison[2][4];     // rows of a tile of V that were cleared of infinities and NaN, per slot
-    float row[2][kWideTile];               // largest scores, then sums of the slots' rows, when the slots share rows
+    float top[2][kWideTile], sum[2][kWideTile];  // of the slots' rows, when the slots share rows
 };
 constexpr uint32_t kFull = 0, kEmpty = 80, kScores = 160, kWeights = 176, kSums = 192, kQ = 208, kEnd = 224;
-static_assert(sizeof(WideBars) <= 2048 && offsetof(WideBars, q) == kQ && offsetof(WideBars, end) == kEnd, "barriers");
+static_assert(sizeof(WideBars) <= 3072 && offsetof(WideBars, q) == kQ && offsetof(WideBars, end) == kEnd, "barriers");
 
 // 32 bits of a row's view of the drafted rows, from row d on (d may be negative: the context, which it sees).
 __device__ __forceinline__ uint32_t view32(const AttnArgs &a, int seq, int i, int d, int rows) {
@@ -173,8 +173,7 @@ __device__ __noinline__ void wait_on(uint32_t at, uint32_t parity, volatile uint
 template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideThreads, 1) wide_attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using S = WideShape<D>;
     constexpr int kRows = PAIR ? 2 * kWideTile : kWideTile;
-    extern __shared__ uint8_t raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem);
     WideBars &bar = *reinterpret_cast<WideBars *>(smem + S::kBars);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -195,7 +194,9 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
         bar.dead = 0;
         fence_mbar_init();
         a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (base & 1023) atomicMax(a.status, (uint32_t)kStatusTmaTimeout);  // swizzled tiles begin at multiples of 1024 bytes
     }
+    if (base & 1023) return;
     const Share share = find_share<kWideThreads>(a, kWideTile, smem);
     if (share.first >= share.last) return;
     if (warp == 9) {
@@ -406,14 +407,8 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                 wait(kScores + 8 * s, s_phase, kStatusMmaTimeout);
                 s_phase ^= 1;
                 tc_after();
-                // Four chunks of 32 scores; the next one comes while one is worked on.  The weights are taken relative to the maximum of earlier tiles
-                // and stay in registers until it is clear that this tile's is no more than 2^8 above it, as hardly any is after the first.
-                uint32_t za[32], zb[32], p[64];
-                auto hide = [&](uint32_t (&z)[32], uint32_t view) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (!(view >> e & 1)) z[e] = 0xff800000u;
-                };
+                const uint64_t scale2 = twice(a.scale);
+                uint64_t sums[2] = {0, 0};
                 auto most = [&](float m, const uint32_t (&z)[32]) {
                     float n = -INFINITY;
 #pragma unroll
@@ -423,45 +418,60 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                     }
                     return fmaxf(m, n);
                 };
-                const uint64_t scale2 = twice(a.scale);
-                uint64_t off2, sums[2];
-                auto weigh = [&](const uint32_t (&z)[32], int c, auto partly) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const uint64_t y = fma2(pair64(z[e], z[e + 1]), scale2, off2);
-                        float lo, hi;
-                        if ((e & 6) == 6 && !decltype(partly)::value) {
-                            ex2_fma(y, lo, hi);
-                        } else {
-                            unpair64(y, lo, hi);
-                            lo = ex2(lo);
-                            hi = ex2(hi);
-                        }
-                        sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair64(__float_as_uint(lo), __float_as_uint(hi)));
-                        p[16 * c + (e >> 1)] = pack2<BF16>(lo, hi);
-                    }
-                };
-                float m = -INFINITY;
-                auto pass = [&](auto partly) {
-                    off2 = twice(top == -INFINITY ? 0.f : -top * a.scale);
-                    sums[0] = sums[1] = 0;
+                uint32_t za[32], zb[32];
+                bool done = false;
+                if (!masked && !__any_sync(0xffffffffu, top == -INFINITY)) {
+                    // Four chunks of 32 scores, the next one on its way while one is worked on.  The weights are taken relative to the maximum of earlier tiles
+                    // and stay in registers until it is clear that this tile's is no more than 2^8 above it.
+                    uint32_t p[64];
+                    const uint64_t off2 = twice(-top * a.scale);
+                    float m = -INFINITY;
                     tm_ld32(t_s, za);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t(&z)[32] = c & 1 ? zb : za;
                         tm_ld_wait(z);
                         if (c < 3) tm_ld32(t_s + 32 * (c + 1), c & 1 ? za : zb);
-                        if (decltype(partly)::value) hide(z, seen[c]);
                         m = most(m, z);
-                        weigh(z, c, partly);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const uint64_t y = fma2(pair64(z[e], z[e + 1]), scale2, off2);
+                            float lo, hi;
+                            if ((e & 6) == 6) {
+                                ex2_fma(y, lo, hi);
+                            } else {
+                                unpair64(y, lo, hi);
+                                lo = ex2(lo);
+                                hi = ex2(hi);
+                            }
+                            sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair64(__float_as_uint(lo), __float_as_uint(hi)));
+                            p[16 * c + (e >> 1)] = pack2<BF16>(lo, hi);
+                        }
                     }
-                };
+                    if (!__any_sync(0xffffffffu, (m - top) * a.scale > 8.f)) {
+                        tm_st32(t_s, *reinterpret_cast<uint32_t(*)[32]>(p));
+                        tm_st32(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
+                        done = true;
+                    }
+                }
+                if (!done) {
+                    // The first tile of an item, one with a new maximum, or with keys that not every row sees: maximum first.  Small code, as the instruction
+                    // cache has not seen it for a while.
+                    auto hide = [&](int c) {
+                        const uint32_t view = c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(view >> e & 1)) za[e] = 0xff800000u;
+                    };
+                    float m = -INFINITY;
 #pragma unroll 1
-                while (true) {
-                    if (masked) pass(std::true_type{});
-                    else pass(std::false_type{});
+                    for (int c = 0; c < 4; ++c) {
+                        tm_ld32(t_s + 32 * c, za);
+                        tm_ld_wait(za);
+                        hide(c);
+                        m = most(m, za);
+                    }
                     const bool rise = top == -INFINITY ? m > top : (m - top) * a.scale > 8.f;
-                    if (!__any_sync(0xffffffffu, rise)) break;
                     const float down = rise && top != -INFINITY ? ex2((top - m) * a.scale) : 1.f;
                     if (__any_sync(0xffffffffu, down != 1.f)) {
                         if (job) wait(kSums + 8 * s, (n_sums - 1) & 1, kStatusMmaTimeout);
@@ -474,13 +484,29 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                             for (int e = 0; e < 32; ++e) za[e] = __float_as_uint(__uint_as_float(za[e]) * down);
                             tm_st32(t_o + 32 * c, za);
                         }
-                        tm_st_wait();
                         sum *= down;
                     }
                     if (rise) top = m;
+                    const uint64_t off2 = twice(top == -INFINITY ? 0.f : -top * a.scale);
+                    sums[0] = sums[1] = 0;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        tm_ld32(t_s + 32 * c, za);
+                        tm_ld_wait(za);
+                        hide(c);
+                        uint32_t p[16];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float lo, hi;
+                            unpair64(fma2(pair64(za[e], za[e + 1]), scale2, off2), lo, hi);
+                            lo = ex2(lo);
+                            hi = ex2(hi);
+                            sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair64(__float_as_uint(lo), __float_as_uint(hi)));
+                            p[e >> 1] = pack2<BF16>(lo, hi);
+                        }
+                        tm_st16(t_s + 16 * c, p);  // over scores that are read already
+                    }
                 }
-                tm_st32(t_s, *reinterpret_cast<uint32_t(*)[32]>(p));
-                tm_st32(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
                 tm_st_wait();
                 {
                     float lo, hi;
@@ -565,76 +591,76 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
             const int part_row = PAIR ? s * kWideTile + row : row;
             // first value of this thread's row in the output or in the part
             const int64_t to = i >= a.rows ? -1 : whole ? (((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + q_row % a.group) * d : (int64_t)part_row * D;
-            uint8_t *stage = smem + S::kQ + s * S::kTileBytes;  // of Q, which is through: [128][D / 2] f32, chunks swizzled
-            // Half h of the columns of the warp's 32 rows leaves by way of shared memory, whole lines at a time.
-            auto put = [&](int h, const float (&y)[D / 2]) {
-#pragma unroll
-                for (int c = 0; c < D / 8; ++c) *reinterpret_cast<float4 *>(stage + row * (2 * D) + ((c ^ (row & 7)) << 4)) = make_float4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+            // The sums leave by way of the place of Q, which is through ([128][D / 2] f32, chunks of 16 bytes swizzled), whole lines at a time: 32 columns of the
+            // warp's 32 rows.  Loops, not straight code: it runs once per item, at the pace of instruction fetches.
+            auto chunk_at = [&](uint8_t *region, int r, int c) { return region + r * (2 * D) + ((c ^ (r & 7)) << 4); };
+            auto put = [&](uint8_t *region, int c0, int col) {
                 __syncwarp();
-#pragma unroll 8
-                for (int k = 0; k < D / 4; ++k) {
-                    const int r = (32 * k + lane) / (D / 4), c = (32 * k + lane) % (D / 4), col = h * (D / 2) + 2 * c, at_row = (row & ~31) + r;
+#pragma unroll 2
+                for (int k = 0; k < 8; ++k) {
+                    const int r = 4 * k + (lane >> 3), c = lane & 7;
                     const int64_t at = __shfl_sync(0xffffffffu, to, r);
-                    const float2 v = *reinterpret_cast<const float2 *>(stage + at_row * (2 * D) + (((c >> 1) ^ (at_row & 7)) << 4) + 8 * (c & 1));
+                    const float4 v = *reinterpret_cast<const float4 *>(chunk_at(region, (row & ~31) + r, c0 + c));
                     if (at < 0) continue;
-                    if (!whole) *reinterpret_cast<float2 *>(part + at + col) = v;
-                    else if (col < d) *reinterpret_cast<uint32_t *>(a.out + 2 * (at + col)) = pack2<BF16>(v.x, v.y);
+                    if (!whole) *reinterpret_cast<float4 *>(part + at + col + 4 * c) = v;
+                    else if (col + 4 * c < d) *reinterpret_cast<uint2 *>(a.out + 2 * (at + col + 4 * c)) = make_uint2(pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w));
                 }
                 __syncwarp();
             };
             float log_top = top == -INFINITY ? -INFINITY : top * a.scale;
-            float y[D / 2];
+            uint8_t *stage = smem + S::kQ + s * S::kTileBytes;
+            uint32_t x[32];
             if (PAIR) {
-                const float inv = !whole ? 1.f : sum == 0.f || i >= len.rows ? 0.f : 1.f / sum;
                 const bool none = whole && (sum == 0.f || i >= len.rows);
+                const float inv = !whole ? 1.f : none ? 0.f : 1.f / sum;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    tm_ld32(t_o + 32 * c, x);
+                    tm_ld_wait(x);
+                    const int c0 = (8 * c) % (D / 8);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                    for (int c = 0; c < D / 64; ++c) {
-                        uint32_t x[32];
-                        tm_ld32(t_o + h * (D / 2) + 32 * c, x);
-                        tm_ld_wait(x);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) y[32 * c + e] = none ? 0.f : __uint_as_float(x[e]) * inv;
-                    }
-                    put(h, y);
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4 *>(chunk_at(stage, row, c0 + e / 4)) = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(__uint_as_float(x[e]) * inv, __uint_as_float(x[e + 1]) * inv, __uint_as_float(x[e + 2]) * inv, __uint_as_float(x[e + 3]) * inv);
+                    put(stage, c0, 32 * c);
                 }
             } else {
                 // each slot finishes half of the columns: it hands the other half of its sums over, relative to both slots' maximum
-                bar.row[s][row] = log_top;
+                bar.top[s][row] = log_top;
+                bar.sum[s][row] = sum;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                const float both = fmaxf(log_top, bar.row[1 - s][row]), scale = both == -INFINITY ? 0.f : ex2(log_top - both);
-                float *hand = reinterpret_cast<float *>(stage);  // [D / 2][128]
-#pragma unroll
+                const float other = bar.top[1 - s][row], both = fmaxf(log_top, other), scale = log_top == -INFINITY ? 0.f : ex2(log_top - both);
+#pragma unroll 1
                 for (int c = 0; c < D / 64; ++c) {
-                    uint32_t x[32];
                     tm_ld32(t_o + (1 - s) * (D / 2) + 32 * c, x);
                     tm_ld_wait(x);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) hand[(32 * c + e) * kWideTile + row] = scale == 0.f ? 0.f : __uint_as_float(x[e]) * scale;
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4 *>(chunk_at(stage, row, 8 * c + e / 4)) = scale == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(__uint_as_float(x[e]) * scale, __uint_as_float(x[e + 1]) * scale, __uint_as_float(x[e + 2]) * scale, __uint_as_float(x[e + 3]) * scale);
                 }
-                sum = scale == 0.f ? 0.f : sum * scale;
+                sum = (scale == 0.f ? 0.f : sum * scale) + (other == -INFINITY ? 0.f : bar.sum[1 - s][row] * ex2(other - both));
                 log_top = both;
+                const bool none = whole && (sum == 0.f || i >= len.rows);
+                const float inv = !whole ? 1.f : none ? 0.f : 1.f / sum;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                bar.row[s][row] = sum;
-                const float *from = reinterpret_cast<const float *>(smem + S::kQ + (1 - s) * S::kTileBytes);
-#pragma unroll
+                uint8_t *from = smem + S::kQ + (1 - s) * S::kTileBytes;
+#pragma unroll 1
                 for (int c = 0; c < D / 64; ++c) {
-                    uint32_t x[32];
                     tm_ld32(t_o + s * (D / 2) + 32 * c, x);
                     tm_ld_wait(x);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) y[32 * c + e] = (scale == 0.f ? 0.f : __uint_as_float(x[e]) * scale) + from[(32 * c + e) * kWideTile + row];
+                    for (int e = 0; e < 32; e += 4) {
+                        float4 *at = reinterpret_cast<float4 *>(chunk_at(from, row, 8 * c + e / 4));
+                        float4 v = *at;
+                        if (scale != 0.f) {
+                            v.x += __uint_as_float(x[e]) * scale;
+                            v.y += __uint_as_float(x[e + 1]) * scale;
+                            v.z += __uint_as_float(x[e + 2]) * scale;
+                            v.w += __uint_as_float(x[e + 3]) * scale;
+                        }
+                        *at = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                    }
+                    put(from, 8 * c, s * (D / 2) + 32 * c);
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                sum += bar.row[1 - s][row];
-                if (whole) {
-                    const bool none = sum == 0.f || i >= len.rows;
-                    const float inv = none ? 0.f : 1.f / sum;
-#pragma unroll
-                    for (int e = 0; e < D / 2; ++e) y[e] = none ? 0.f : y[e] * inv;
-                }
-                put(s, y);
             }
             if (!whole && (PAIR || s == 0)) {
                 part[kRows * D + part_row] = log_top;
