@@ -73,7 +73,7 @@ def test_bad_parents_and_lengths_are_left_out_and_reported():
 # ---- rotary positions
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("interleaved,suffix,inverse", [(False, False, False), (True, False, True), (False, True, True), (True, True, False)])
-@pytest.mark.parametrize("rows,heads,kv,dim,rotary", [(1, 24, 8, 64, 64), (5, 3, 1, 10, 6), (9, 4, 4, 80, 32), (2, 1, 1, 128, 8), (33, 5, 1, 72, 72), (3, 40, 8, 256, 250)])
+@pytest.mark.parametrize("rows,heads,kv,dim,rotary", [(1, 24, 8, 64, 64), (5, 3, 1, 10, 6), (9, 4, 4, 80, 32), (2, 1, 1, 128, 8), (33, 5, 1, 72, 72), (3, 40, 8, 256, 250), (7, 6, 2, 16, 16), (4, 3, 3, 2, 2), (2, 64, 64, 128, 128)])
 def test_rope_rows(dtype, interleaved, suffix, inverse, rows, heads, kv, dim, rotary):
     g = gen_of(rows * dim)
     q, k = torch.randn((rows, heads, dim), generator=g).to(dtype), torch.randn((rows, kv, dim), generator=g).to(dtype)

@@ -6,13 +6,17 @@
 // t reaches 1e6 and more, where an f32 product is off by tenths of a radian; here the product is exact (24 + 24 bits in f64), its whole
 // turns come off in f64, and the rest of it, at most half a turn, goes through sincospif: 1e-7 at any position.
 //
-// Bound by memory, each value read and written once.  A CTA takes as many rows as fill its 256 threads; a thread asks for its first two
-// vectors before the angles are computed, so that these hide under the loads, and the sines of a row are shared by all its heads.
+// Bound by memory, each value read and written once.  A CTA takes as many rows as fill its 128 or 256 threads.  A thread has one place in a head (a vector of
+// pairs) and takes it in several heads, so that offsets and sines are computed or read once for all of them; it asks for the first three heads'
+// values before anything else: the look-ups of position and page and the angles hide under the loads.
 #include <cmath>
+#include <type_traits>
 
 #include "zq_draft.cuh"
 
 namespace zq {
+
+constexpr int kAhead = 3, kMaxRopeHead = 512;  // heads a thread asks for at once; values of a head
 
 struct RopeRowsArgs {
     const uint8_t *q, *k, *v;
@@ -24,8 +28,7 @@ struct RopeRowsArgs {
     int64_t rows;
     int rows_per_seq, q_heads, k_heads, v_heads, head_dim, rotary, start, interleaved, inverse;
     float factor;
-    int threads;        // of one row
-    int pair_items, copy_items, copy_all;  // work items of a head: that turn pairs, outside the turned part; of a head of V
+    int log_threads, places, heads;  // threads of a row, places of a head, heads of q, k and v that the threads take at a time
     uint32_t *status;
 };
 
@@ -38,122 +41,130 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two 16-bit values of a word.
+template <class T> __device__ __forceinline__ float2 two_f32(uint32_t w) {
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <class T> __device__ __forceinline__ uint32_t from_two(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+}
+
 template <class T, int N> struct alignas(sizeof(T) * N) Vec {
     T v[N];
 };
 
-// VEC values per access: 16 bytes where head, turned part, strides and addresses allow, else one value (a pair, where pairs lie side by side).
-// An item is VEC pairs (two vectors, of which an interleaved one is the other's neighbour) or 2 VEC values that are copied.
-template <class T, int VEC> __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeRowsArgs a) {
+// VEC values per access: 16 bytes where head, turned part, strides and addresses allow, else one value.  A place is VEC pairs (two vectors, of which an
+// interleaved one is the other's neighbour) or 2 VEC values that are copied; the sines lie so that neighbouring threads read neighbouring ones.
+template <class T, int VEC> __global__ void __launch_bounds__(256, 4) rope_rows_kernel(const RopeRowsArgs a) {
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     extern __shared__ float2 s_turn[];
     using V = Vec<T, VEC>;
-    const int lane = threadIdx.x % a.threads, slot = threadIdx.x / a.threads, half = a.rotary / 2;
-    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / a.threads) + slot;
-    const bool here = row < a.rows;
-    const int position = here ? a.positions[row] : -1;
+    const int lane = threadIdx.x & ((1 << a.log_threads) - 1), slot = threadIdx.x >> a.log_threads, half = a.rotary / 2;
+    const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> a.log_threads) + slot;
+    const int h0 = (int)((unsigned)lane / (unsigned)a.places), c = lane - h0 * a.places, all = a.q_heads + a.k_heads + a.v_heads;
+    const bool here = row < a.rows && h0 < a.heads;
+    // the place in a head of q or k (its first pair, or -1 outside the turned part), and in one of v; a second vector at head_dim is none
+    const int pairs = half / VEC, at = 2 * VEC * (c - pairs);
+    const int pair = c < pairs ? c * VEC : -1;
+    const int first = pair >= 0 ? a.start + (a.interleaved ? 2 * pair : pair) : a.start ? at : a.rotary + at;
+    const int second = pair >= 0 ? first + (a.interleaved ? VEC : half) : first + VEC < (a.start ? a.start : a.head_dim) ? first + VEC : a.head_dim;
+    const T *q = reinterpret_cast<const T *>(a.q) + row * a.q_stride, *k = reinterpret_cast<const T *>(a.k) + row * a.k_stride, *v = reinterpret_cast<const T *>(a.v) + row * a.v_stride;
+
+    auto load = [&](int h, V &x, V &y) {
+        const bool is_v = h >= a.q_heads + a.k_heads;
+        const T *src = h < a.q_heads ? q + h * a.head_dim : is_v ? v + (h - a.q_heads - a.k_heads) * a.head_dim : k + (h - a.q_heads) * a.head_dim;
+        const int i = is_v ? 2 * VEC * c : first, j = is_v ? i + VEC : second;
+        x = *reinterpret_cast<const V *>(src + i);
+        if (j < a.head_dim) y = *reinterpret_cast<const V *>(src + j);
+    };
+    V xs[kAhead], ys[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        if (here && h0 + j * a.heads < all) load(h0 + j * a.heads, xs[j], ys[j]);
+    const int position = row < a.rows ? a.positions[row] : -1;
     int64_t keep = -1;  // the cache row, or -1
-    if (a.cache.k && here && position >= 0) {
-        const int seq = (int)(row / a.rows_per_seq), i = (int)(row % a.rows_per_seq);
-        if (i < draft_len(a.lens, seq, a.rows_per_seq, a.status)) {
-            const int start = a.cache.lens[seq];
+    if (a.cache.k && row < a.rows) {
+        const int seq = (int)((unsigned)row / (unsigned)a.rows_per_seq), i = (int)row - seq * a.rows_per_seq, start = a.cache.lens[seq];
+        if (i < draft_len(a.lens, seq, a.rows_per_seq, a.status) && position >= 0) {
             keep = start < 0 ? -1 : cache_row(a.cache, seq, (int64_t)start + i);
             if (keep < 0) atomicMax(a.status, (uint32_t)kStatusBadIndex);
         }
     }
-    const int head_items = a.pair_items + a.copy_items, turned = (a.q_heads + a.k_heads) * head_items, items = here ? turned + a.v_heads * a.copy_all : 0;
-    const bool to_cache = a.cache.k != nullptr;
-
-    struct Item {
-        const T *src;
-        T *dst;
-        int first, second, pair;  // offsets of the two vectors from the head's start (second: head_dim where there is none); their first pair, or -1
-    };
-    auto item_of = [&](int i) {
-        Item it;
-        if (i >= turned) {
-            const int head = (i - turned) / a.copy_all, c = (i - turned) % a.copy_all;
-            it.src = reinterpret_cast<const T *>(a.v) + row * a.v_stride + head * a.head_dim;
-            it.dst = keep < 0 ? nullptr : reinterpret_cast<T *>(a.cache.v) + keep + head * a.head_dim;
-            it.first = 2 * VEC * c;
-            it.second = it.first + VEC;
-            it.pair = -1;
-            return it;
-        }
-        const int head = i / head_items, c = i % head_items;
-        if (head < a.q_heads) {
-            it.src = reinterpret_cast<const T *>(a.q) + row * a.q_stride + head * a.head_dim;
-            it.dst = reinterpret_cast<T *>(a.q_out) + (row * a.q_heads + head) * a.head_dim;
-        } else {
-            const int h = head - a.q_heads;
-            it.src = reinterpret_cast<const T *>(a.k) + row * a.k_stride + h * a.head_dim;
-            it.dst = !to_cache ? reinterpret_cast<T *>(a.k_out) + (row * a.k_heads + h) * a.head_dim : keep < 0 ? nullptr : reinterpret_cast<T *>(a.cache.k) + keep + h * a.head_dim;
-        }
-        if (c < a.pair_items) {
-            it.pair = c * VEC;
-            it.first = a.start + (a.interleaved ? 2 * VEC * c : VEC * c);
-            it.second = a.interleaved ? it.first + VEC : it.first + half;
-        } else {
-            it.pair = -1;
-            const int at = 2 * VEC * (c - a.pair_items);
-            it.first = a.start ? at : a.rotary + at;  // in front of the turned part or behind it
-            it.second = it.first + VEC < (a.start ? a.start : a.head_dim) ? it.first + VEC : a.head_dim;
-        }
-        return it;
-    };
-    auto load = [&](const Item &it, V &x, V &y) {
-        x = *reinterpret_cast<const V *>(it.src + it.first);
-        if (it.second < a.head_dim) y = *reinterpret_cast<const V *>(it.src + it.second);
-    };
-
-    V x, y;
-    Item it{};
-    if (lane < items) {
-        it = item_of(lane);
-        load(it, x, y);
-    }
     float2 *turn = s_turn + slot * half;
-    if (here && position >= 0) {
-        for (int p = lane; p < half; p += a.threads) {
+    if (position >= 0) {
+        for (int p = lane; p < half; p += 1 << a.log_threads) {
             double t = (double)position * (double)a.inv_freq[p] * 0.15915494309189533577;  // in turns
             t -= rint(t);
             float s, c;
             sincospif(2.f * (float)t, &s, &c);
-            turn[p] = make_float2(c * a.factor, a.inverse ? -s * a.factor : s * a.factor);
+            turn[p % VEC * (half / VEC) + p / VEC] = make_float2(c * a.factor, a.inverse ? -s * a.factor : s * a.factor);
         }
     }
     __syncthreads();
-    for (int i = lane; i < items; i += a.threads) {
-        if (i != lane) {
-            it = item_of(i);
-            load(it, x, y);
-        }
-        if (it.pair >= 0 && position >= 0) {
-            if (a.interleaved && VEC > 1) {
+    if (!here) return;
+    float2 sines[VEC];
+    const bool turns = pair >= 0 && position >= 0;
+    if (turns) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    V &w = 2 * j < VEC ? x : y;
-                    const int at = 2 * j % VEC;
-                    const float2 cs = turn[it.pair + j];
-                    const float re = to_f32(w.v[at]), im = to_f32(w.v[(at + 1) % VEC]);
-                    w.v[at] = from_f32<T>(re * cs.x - im * cs.y);
-                    w.v[(at + 1) % VEC] = from_f32<T>(im * cs.x + re * cs.y);
+        for (int j = 0; j < VEC; ++j) sines[j] = turn[j * pairs + c];
+    }
+    T *q_out = reinterpret_cast<T *>(a.q_out) + row * a.q_heads * a.head_dim, *k_out = a.cache.k ? reinterpret_cast<T *>(a.cache.k) + keep : reinterpret_cast<T *>(a.k_out) + row * a.k_heads * a.head_dim,
+      *v_out = reinterpret_cast<T *>(a.cache.v) + keep;
+    auto finish = [&](int h, V x, V y) {
+        const bool is_v = h >= a.q_heads + a.k_heads;
+        if (h >= a.q_heads && a.cache.k && keep < 0) return;
+        if (turns && !is_v) {
+            if constexpr (sizeof(T) == 2 && VEC > 1) {
+                uint32_t xw[VEC / 2], yw[VEC / 2];
+                memcpy(xw, &x, sizeof(x));
+                memcpy(yw, &y, sizeof(y));
+#pragma unroll
+                for (int j = 0; j < VEC; j += 2) {
+                    const float2 a0 = sines[j], a1 = sines[j + 1];
+                    if (a.interleaved) {  // words 0..VEC/2 are x's pairs, the others y's
+                        uint32_t &w0 = j < VEC / 2 ? xw[j] : yw[j - VEC / 2], &w1 = j < VEC / 2 ? xw[j + 1] : yw[j + 1 - VEC / 2];
+                        const float2 s = two_f32<T>(w0), t = two_f32<T>(w1);
+                        w0 = from_two<T>(s.x * a0.x - s.y * a0.y, s.y * a0.x + s.x * a0.y);
+                        w1 = from_two<T>(t.x * a1.x - t.y * a1.y, t.y * a1.x + t.x * a1.y);
+                    } else {
+                        const float2 re = two_f32<T>(xw[j / 2]), im = two_f32<T>(yw[j / 2]);
+                        xw[j / 2] = from_two<T>(re.x * a0.x - im.x * a0.y, re.y * a1.x - im.y * a1.y);
+                        yw[j / 2] = from_two<T>(im.x * a0.x + re.x * a0.y, im.y * a1.x + re.y * a1.y);
+                    }
                 }
+                memcpy(&x, xw, sizeof(x));
+                memcpy(&y, yw, sizeof(y));
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float2 cs = turn[it.pair + j];
-                    const float re = to_f32(x.v[j]), im = to_f32(y.v[j]);
-                    x.v[j] = from_f32<T>(re * cs.x - im * cs.y);
-                    y.v[j] = from_f32<T>(im * cs.x + re * cs.y);
+                    const bool beside = a.interleaved && VEC > 1;
+                    T &r = beside ? (2 * j < VEC ? x : y).v[2 * j % VEC] : x.v[j], &i = beside ? (2 * j < VEC ? x : y).v[(2 * j + 1) % VEC] : y.v[j];
+                    const float re = to_f32(r), im = to_f32(i);
+                    r = from_f32<T>(re * sines[j].x - im * sines[j].y);
+                    i = from_f32<T>(im * sines[j].x + re * sines[j].y);
                 }
             }
         }
-        if (it.dst) {
-            *reinterpret_cast<V *>(it.dst + it.first) = x;
-            if (it.second < a.head_dim) *reinterpret_cast<V *>(it.dst + it.second) = y;
-        }
+        T *dst = h < a.q_heads ? q_out + h * a.head_dim : is_v ? v_out + (h - a.q_heads - a.k_heads) * a.head_dim : k_out + (h - a.q_heads) * a.head_dim;
+        const int i = is_v ? 2 * VEC * c : first, j = is_v ? i + VEC : second;
+        *reinterpret_cast<V *>(dst + i) = x;
+        if (j < a.head_dim) *reinterpret_cast<V *>(dst + j) = y;
+    };
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        if (h0 + j * a.heads < all) finish(h0 + j * a.heads, xs[j], ys[j]);
+    for (int h = h0 + kAhead * a.heads; h < all; h += a.heads) {
+        V x, y;
+        load(h, x, y);
+        finish(h, x, y);
     }
 }
 
@@ -162,10 +173,10 @@ static int rope_checks(const char *who, zq_ctx *ctx, const RopeRowsArgs &a, int 
     if (!ctx || !a.q || !a.q_out || !a.positions || !a.inv_freq) return set_error(err, ZQ_ERR_ARG, "%s: null argument", who);
     if (dtype != ZQ_F32 && dtype != ZQ_F16 && dtype != ZQ_BF16) return set_error(err, ZQ_ERR_ARG, "%s: unknown dtype %d", who, dtype);
     if ((layout != ZQ_ROPE_SPLIT_HALF && layout != ZQ_ROPE_INTERLEAVED) || (placement != ZQ_ROPE_PREFIX && placement != ZQ_ROPE_SUFFIX)) return set_error(err, ZQ_ERR_ARG, "%s: unknown layout %d or placement %d", who, layout, placement);
-    if (q_heads == 0 || rotary == 0 || rotary % 2 || head_dim == 0 || head_dim > 4096) return set_error(err, ZQ_ERR_SHAPE, "%s: heads=%zu head_dim=%zu rotary=%zu (rotary must be even and positive)", who, q_heads, head_dim, rotary);
+    if (q_heads == 0 || rotary == 0 || rotary % 2 || head_dim == 0 || head_dim > kMaxRopeHead) return set_error(err, ZQ_ERR_SHAPE, "%s: heads=%zu head_dim=%zu rotary=%zu (a head of up to 512 values, rotary even and positive)", who, q_heads, head_dim, rotary);
     if (rotary > head_dim) return set_error(err, ZQ_ERR_SHAPE, "%s: rotary=%zu exceeds head_dim=%zu", who, rotary, head_dim);
     if (rows == 0 || rows > (size_t)INT32_MAX) return set_error(err, ZQ_ERR_SHAPE, "%s: %zu rows", who, rows);
-    if (q_heads > 65536 || k_heads > 65536) return set_error(err, ZQ_ERR_SHAPE, "%s: shape too large", who);
+    if ((q_heads + 2 * k_heads) * head_dim > (size_t(1) << 20) || q_heads > (size_t(1) << 20) || k_heads > (size_t(1) << 20)) return set_error(err, ZQ_ERR_SHAPE, "%s: rows of %zu and %zu heads of %zu values are too large", who, q_heads, k_heads, head_dim);
     if (q_stride < q_heads * head_dim || (a.k && k_stride < k_heads * head_dim) || (a.v && v_stride < k_heads * head_dim)) return set_error(err, ZQ_ERR_SHAPE, "%s: rows overlap (strides %zu, %zu, %zu)", who, q_stride, k_stride, v_stride);
     if (q_stride > (size_t)INT32_MAX || k_stride > (size_t)INT32_MAX || v_stride > (size_t)INT32_MAX) return set_error(err, ZQ_ERR_SHAPE, "%s: shape too large", who);
     if ((a.q_out == a.q && q_stride != q_heads * head_dim) || (a.k && a.k_out == a.k && k_stride != k_heads * head_dim)) return set_error(err, ZQ_ERR_ARG, "%s: in place only where the rows are dense", who);
@@ -181,16 +192,17 @@ template <class T> static int launch_rope_rows(zq_ctx *ctx, RopeRowsArgs &a, zq_
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k_out);
     wide = wide && (at & 15) == 0;
     const int vec = wide ? kWide : 1;
-    a.pair_items = half / vec;
-    a.copy_items = (rest + 2 * vec - 1) / (2 * vec);
-    a.copy_all = (a.head_dim + 2 * vec - 1) / (2 * vec);
-    const int64_t items = (int64_t)(a.q_heads + a.k_heads) * (a.pair_items + a.copy_items) + (int64_t)a.v_heads * a.copy_all;
-    a.threads = 32;
-    while (a.threads < 256 && a.threads < items) a.threads *= 2;
-    const int per_cta = 256 / a.threads;
+    a.places = half / vec + (rest + 2 * vec - 1) / (2 * vec);  // of v as many: the turned part is whole places
+    const int all = a.q_heads + a.k_heads + a.v_heads;
+    // a row's threads: enough for its heads in three turns where rows are many (their look-ups are then fewer), in one where an SM has few
+    const int64_t turns = a.rows > 4 * ctx->sm_count ? kAhead : 1;
+    a.log_threads = 5;
+    while (a.log_threads < 8 && ((1 << a.log_threads) < a.places || (1 << a.log_threads) / a.places * turns < all)) ++a.log_threads;
+    a.heads = (1 << a.log_threads) / a.places;
+    const int threads = a.log_threads < 7 ? 128 : 1 << a.log_threads, per_cta = threads >> a.log_threads;
     const dim3 grid((unsigned)((a.rows + per_cta - 1) / per_cta));
     const size_t smem = (size_t)per_cta * half * sizeof(float2);
-    return wide ? launch_pdl(ctx, rope_rows_kernel<T, kWide>, grid, dim3(256), smem, err, a) : launch_pdl(ctx, rope_rows_kernel<T, 1>, grid, dim3(256), smem, err, a);
+    return wide ? launch_pdl(ctx, rope_rows_kernel<T, kWide>, grid, dim3((unsigned)threads), smem, err, a) : launch_pdl(ctx, rope_rows_kernel<T, 1>, grid, dim3((unsigned)threads), smem, err, a);
 }
 
 static int launch_rope_rows(zq_ctx *ctx, RopeRowsArgs &a, int dtype, zq_error *err) {
