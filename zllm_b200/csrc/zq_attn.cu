@@ -11,9 +11,14 @@
 // left in parts (largest score, sum of weights and weighted sums per row, f32) which a second, small kernel joins in ascending order:
 // results do not depend on timing.  The lengths are on the device, so each CTA finds its share from them itself.
 //
+// Where all of it takes a few microseconds, the second kernel would be half of the time: there a cluster of CTAs takes an item, in equal
+// runs of its units, and joins its parts through distributed shared memory.
+//
 // A CTA has key groups (its warps of one group share keys, each with 16 rows of its own; the groups take the keys in turn), every one with a ring
 // of its own that cp.async fills: no barrier between groups until the item ends.  Shared memory rows are swizzled by 16-byte chunks so that
 // ldmatrix reads without conflicts.
+#include <cooperative_groups.h>
+
 #include "zq_attn.cuh"
 
 namespace zq {
@@ -50,8 +55,9 @@ template <int D, int WM> struct AttnShape {
     static constexpr int kRows = 16 * WM;
     static constexpr int kRing = kGroups * kStages * kStage;
     static constexpr int kMerge = kGroups * kRows * (D + 2) * 4;  // the groups' sums at the end of an item, in place of the ring
-    static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + 1024;
-    static constexpr int kPartFloats = kRows * (D + 2);
+    static constexpr int kPartFloats = kRows * (D + 2);           // of a part: sums, largest scores, sums of weights
+    static constexpr int kPartAt = kMerge, kNeed = kMerge + kPartFloats * 4;
+    static constexpr int kSmem = (kRing > kNeed ? kRing : kNeed) + 1024;
     static_assert(kStages >= 2 && kSmem <= 227 << 10, "ring");
 };
 
@@ -61,9 +67,22 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
     pdl_wait_prior_grid();
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp / WM, wm = warp % WM, gtid = tid - group * WM * 32;
-    const Share share = find_share<S::kThreads>(a, S::kUnit, smem + S::kSmem - 1024);
-    if (tid == 0) a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
-    if (share.first >= share.last) return;
+    namespace cg = cooperative_groups;
+    Share share;
+    if (a.split) {
+        const int per_seq = a.c.heads * a.tiles, id = blockIdx.x / a.split, rank = blockIdx.x % a.split, item = id % per_seq;
+        share.seq = id / per_seq;
+        share.seq_first = 0;
+        const int64_t n = units_of(seq_len(a, share.seq), S::kUnit);
+        share.first = item * n + rank * n / a.split;
+        share.last = item * n + (rank + 1) * n / a.split;
+        share.total = 0;
+        share.ctas = 0;
+    } else {
+        share = find_share<S::kThreads>(a, S::kUnit, smem + S::kSmem - 1024);
+        if (tid == 0) a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (share.first >= share.last) return;
+    }
     const int d = a.c.head_dim, chunks = d / 8;
     uint8_t *ring = smem + group * S::kStages * S::kStage;
     const uint32_t ring_u32 = smem_u32(ring);
@@ -72,13 +91,13 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
     SeqLen len = seq_len(a, seq);
     int units = units_of(len, S::kUnit);
 
-    for (int64_t u = share.first; u < share.last;) {
-        while (u >= seq_first + (int64_t)units * a.c.heads * a.tiles) {
+    for (int64_t u = share.first; u < share.last || a.split;) {  // in a cluster once, with no units too
+        while (!a.split && u >= seq_first + (int64_t)units * a.c.heads * a.tiles) {
             seq_first += (int64_t)units * a.c.heads * a.tiles;
             len = seq_len(a, ++seq);
             units = units_of(len, S::kUnit);
         }
-        const int item = (int)((u - seq_first) / units);
+        const int item = a.split ? (int)(blockIdx.x / a.split) % (a.c.heads * a.tiles) : (int)((u - seq_first) / units);
         const int64_t item_first = seq_first + (int64_t)item * units;
         const int head = item / a.tiles, tile = item % a.tiles;
         const int ua = (int)(u - item_first), ub = (int)min((int64_t)units, share.last - item_first);
@@ -98,7 +117,7 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
             if (s < steps) {
                 const uint32_t base = ring_u32 + (s % S::kStages) * S::kStage;
                 constexpr int kChunks = D / 8, kCopies = S::kKeys * kChunks;
-#pragma unroll
+#pragma unroll 4
                 for (int i = 0; i < (kCopies + WM * 32 - 1) / (WM * 32); ++i) {
                     const int idx = i * WM * 32 + gtid, key = idx / kChunks, chunk = idx % kChunks;
                     const int64_t at = __shfl_sync(0xffffffffu, mine, key % S::kKeys);
@@ -112,31 +131,30 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
             }
             cp_commit();
         };
-        int64_t ahead[1];
-#pragma unroll
-        for (int s = 0; s < S::kStages - 1; ++s) fill(s, page_of(s));
-        ahead[0] = page_of(S::kStages - 1);
+        int64_t ahead = page_of(0);
+#pragma unroll 1
+        for (int s = 0; s < S::kStages - 1; ++s) {  // small code: it runs once per item, at the pace of instruction fetches
+            const int64_t now = ahead;
+            ahead = page_of(s + 1);
+            fill(s, now);
+        }
 
         // ---- the rows of this warp
         constexpr int kK = D / 16;
         uint32_t qf[kK][4];
-        const int r_lo = row0 + lane / 4, r_hi = r_lo + 8;
+        const int r_lo = row0 + lane / 4, r_hi = r_lo + 8, i_lo = r_lo / a.group, i_hi = r_hi / a.group;
         {
-            auto q_at = [&](int r, int col) -> uint32_t {
-                if (r >= n_rows || col >= d) return 0u;
-                const uint8_t *p = a.q + 2 * (((int64_t)seq * a.rows + r / a.group) * a.q_stride + (int64_t)(head * a.group + r % a.group) * d + col);
-                return *reinterpret_cast<const uint32_t *>(p);
-            };
+            const int g_lo = r_lo % a.group, g_hi = r_hi % a.group;
+            const uint8_t *p_lo = a.q + 2 * (((int64_t)seq * a.rows + i_lo) * a.q_stride + (int64_t)(head * a.group + g_lo) * d), *p_hi = a.q + 2 * (((int64_t)seq * a.rows + i_hi) * a.q_stride + (int64_t)(head * a.group + g_hi) * d);
 #pragma unroll
             for (int k = 0; k < kK; ++k) {
                 const int col = 16 * k + 2 * (lane & 3);
-                qf[k][0] = q_at(r_lo, col);
-                qf[k][1] = q_at(r_hi, col);
-                qf[k][2] = q_at(r_lo, col + 8);
-                qf[k][3] = q_at(r_hi, col + 8);
+                qf[k][0] = r_lo < n_rows && col < d ? *reinterpret_cast<const uint32_t *>(p_lo + 2 * col) : 0u;
+                qf[k][1] = r_hi < n_rows && col < d ? *reinterpret_cast<const uint32_t *>(p_hi + 2 * col) : 0u;
+                qf[k][2] = r_lo < n_rows && col + 8 < d ? *reinterpret_cast<const uint32_t *>(p_lo + 2 * col + 16) : 0u;
+                qf[k][3] = r_hi < n_rows && col + 8 < d ? *reinterpret_cast<const uint32_t *>(p_hi + 2 * col + 16) : 0u;
             }
         }
-        const int i_lo = r_lo / a.group, i_hi = r_hi / a.group;
         float o[D / 8][4];
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -146,8 +164,8 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
             cp_wait<S::kStages - 2>();
             if (WM == 1) __syncwarp();
             else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(WM * 32) : "memory");
-            fill(s + S::kStages - 1, ahead[0]);
-            ahead[0] = page_of(s + S::kStages);
+            fill(s + S::kStages - 1, ahead);
+            ahead = page_of(s + S::kStages);
             const uint32_t kb = ring_u32 + (s % S::kStages) * S::kStage, vb = kb + S::kKeys * S::kPitch;
             const int key0 = (ua + s) * S::kUnit + group * S::kKeys;
 
@@ -173,14 +191,15 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[n][e] *= a.scale;
             }
+            uint32_t view[2] = {0xffffffffu, 0xffffffffu};  // of the keys that the thread's two rows see
             if (masked) {
+                view[0] = view32(a, seq, i_lo, key0 - len.context, len.rows);
+                view[1] = view32(a, seq, i_hi, key0 - len.context, len.rows);
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + n * 8 + 2 * (lane & 3) + (e & 1), i = e < 2 ? i_lo : i_hi;
-                        if (key >= len.context && (key >= keys || i >= len.rows || !sees(a, seq, i, key - len.context))) sc[n][e] = -INFINITY;
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        if (!(view[e >> 1] >> (n * 8 + 2 * (lane & 3) + (e & 1)) & 1)) sc[n][e] = -INFINITY;
                 }
             }
             float base[2];
@@ -215,54 +234,63 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
                 pf[n / 2][(n & 1) * 2] = pack2<BF16>(p[0], p[1]);
                 pf[n / 2][(n & 1) * 2 + 1] = pack2<BF16>(p[2], p[3]);
             }
-            if (!masked) {
-#pragma unroll
-                for (int k = 0; k < S::kKeys / 16; ++k) {
-#pragma unroll
-                    for (int n = 0; n < D / 8; n += 2) {
-                        const int key = k * 16 + (mi & 1) * 8 + mr, chunk = n + (mi >> 1);
-                        uint32_t b[4];
-                        ldmatrix_x4_trans(b, vb + key * S::kPitch + ((chunk ^ (key & 7)) << 4));
-                        mma16<BF16>(o[n], pf[k], b[0], b[1]);
-                        mma16<BF16>(o[n + 1], pf[k], b[2], b[3]);
-                    }
-                }
-            } else {
-                // a weight of zero times an infinity of a row that is not seen would be a NaN: such values leave the product, and come
-                // back for the rows that see them
+            if (masked) {
+                // A weight of zero times an infinity of a row that is not seen would be a NaN: such values leave the tile, and are added to the rows that see
+                // them.  Lane j looks through key j (all warps of the group write the same).
+                uint8_t *v = ring + (s % S::kStages) * S::kStage + S::kKeys * S::kPitch;
                 bool dropped = false;
-#pragma unroll
-                for (int k = 0; k < S::kKeys / 16; ++k) {
-#pragma unroll
-                    for (int n = 0; n < D / 8; n += 2) {
-                        const int key = k * 16 + (mi & 1) * 8 + mr, chunk = n + (mi >> 1);
-                        uint32_t b[4];
-                        ldmatrix_x4_trans(b, vb + key * S::kPitch + ((chunk ^ (key & 7)) << 4));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) dropped |= drop_nonfinite<BF16>(b[e]);
-                        mma16<BF16>(o[n], pf[k], b[0], b[1]);
-                        mma16<BF16>(o[n + 1], pf[k], b[2], b[3]);
+                if (lane < S::kKeys && key0 + lane >= len.context && key0 + lane < keys) {
+#pragma unroll 1
+                    for (int c = 0; c < D / 8; ++c) {
+                        uint4 *at = reinterpret_cast<uint4 *>(v + lane * S::kPitch + ((c ^ (lane & 7)) << 4));
+                        uint4 w = *at;
+                        bool some = drop_nonfinite<BF16>(w.x);
+                        some |= drop_nonfinite<BF16>(w.y);
+                        some |= drop_nonfinite<BF16>(w.z);
+                        some |= drop_nonfinite<BF16>(w.w);
+                        if (some) dropped = true;
                     }
                 }
-                if (__any_sync(0xffffffffu, dropped)) {
-                    const uint8_t *v = ring + (s % S::kStages) * S::kStage + S::kKeys * S::kPitch;
-                    for (int j = 0; j < S::kKeys; ++j) {
-                        const int key = key0 + j;
-                        if (key >= keys) break;
-                        const bool lo = i_lo < len.rows && (key < len.context || sees(a, seq, i_lo, key - len.context));
-                        const bool hi = i_hi < len.rows && (key < len.context || sees(a, seq, i_hi, key - len.context));
+                uint32_t bad = __ballot_sync(0xffffffffu, dropped);
+                if (bad) {
+                    if (WM > 1) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(WM * 32) : "memory");  // every warp has looked
+                    for (uint32_t left = bad; left; left &= left - 1) {
+                        const int j = __ffs(left) - 1;
+                        const int64_t row = cache_row(a.c, seq, key0 + j);
+                        const uint16_t *from = reinterpret_cast<const uint16_t *>(a.c.v) + row + head_off;
+                        const bool lo = view[0] >> j & 1, hi = view[1] >> j & 1;
 #pragma unroll
                         for (int n = 0; n < D / 8; ++n) {
-                            uint32_t w = *reinterpret_cast<const uint32_t *>(v + j * S::kPitch + ((n ^ (j & 7)) << 4) + 4 * (lane & 3));
-                            uint32_t finite = w;
-                            if (!drop_nonfinite<BF16>(finite)) continue;
-                            w &= (finite & 0xffffu) == (w & 0xffffu) ? 0xffff0000u : 0xffffffffu;  // the values that were left out, zero beside them
-                            w &= (finite >> 16) == (w >> 16) ? 0x0000ffffu : 0xffffffffu;
-                            const float x = unpack16<BF16>(w & 0xffffu), y = unpack16<BF16>(w >> 16);
-                            if (lo) o[n][0] += x, o[n][1] += y;
-                            if (hi) o[n][2] += x, o[n][3] += y;
+                            const int col = n * 8 + 2 * (lane & 3);
+                            if (row >= 0 && col < d) {
+                                const float x = unpack16<BF16>(from[col]), y = unpack16<BF16>(from[col + 1]);
+                                if (!isfinite(x)) o[n][0] += lo ? x : 0.f, o[n][2] += hi ? x : 0.f;
+                                if (!isfinite(y)) o[n][1] += lo ? y : 0.f, o[n][3] += hi ? y : 0.f;
+                            }
+                        }
+                        for (int c = lane; c < D / 8; c += 32) {
+                            uint4 *at = reinterpret_cast<uint4 *>(v + j * S::kPitch + ((c ^ (j & 7)) << 4));
+                            uint4 w = *at;
+                            drop_nonfinite<BF16>(w.x);
+                            drop_nonfinite<BF16>(w.y);
+                            drop_nonfinite<BF16>(w.z);
+                            drop_nonfinite<BF16>(w.w);
+                            *at = w;
                         }
                     }
+                    if (WM > 1) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(WM * 32) : "memory");
+                    __syncwarp();
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < S::kKeys / 16; ++k) {
+#pragma unroll
+                for (int n = 0; n < D / 8; n += 2) {
+                    const int key = k * 16 + (mi & 1) * 8 + mr, chunk = n + (mi >> 1);
+                    uint32_t b[4];
+                    ldmatrix_x4_trans(b, vb + key * S::kPitch + ((chunk ^ (key & 7)) << 4));
+                    mma16<BF16>(o[n], pf[k], b[0], b[1]);
+                    mma16<BF16>(o[n + 1], pf[k], b[2], b[3]);
                 }
             }
         }
@@ -284,8 +312,8 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
             }
         }
         __syncthreads();
-        const bool whole = ua == 0 && ub == units;
-        float *part = a.parts + ((size_t)blockIdx.x * 2 + (ua == 0 ? 1 : 0)) * S::kPartFloats;
+        const bool whole = !a.split && ua == 0 && ub == units;
+        float *part = a.split ? reinterpret_cast<float *>(smem + S::kPartAt) : a.parts + ((size_t)blockIdx.x * 2 + (ua == 0 ? 1 : 0)) * S::kPartFloats;  // in a cluster its own memory
         for (int idx = tid; idx < S::kRows * (D / 2); idx += S::kThreads) {
             const int r = idx / (D / 2), col = 2 * (idx % (D / 2)), row = tile * S::kRows + r, i = row / a.group;
             float m = -INFINITY;
@@ -315,6 +343,31 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
                 }
             }
         }
+        if (a.split) {
+            cg::cluster_group cluster = cg::this_cluster();
+            cluster.sync();
+            for (int idx = (int)cluster.block_rank() * S::kThreads + tid; idx < S::kRows * (D / 2); idx += a.split * S::kThreads) {
+                const int r = idx / (D / 2), col = 2 * (idx % (D / 2)), row = tile * S::kRows + r, i = row / a.group;
+                if (i >= a.rows || col >= d) continue;
+                float m = -INFINITY, x = 0.f, y = 0.f, l = 0.f;
+                for (int p = 0; p < a.split; ++p) m = fmaxf(m, cluster.map_shared_rank(part, p)[S::kRows * D + r]);
+                const float b = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+                for (int p = 0; p < a.split; ++p) {
+                    const float *f = cluster.map_shared_rank(part, p);
+                    const float w = exp2f(f[S::kRows * D + r] - b);
+                    const float2 v = *reinterpret_cast<const float2 *>(f + r * D + col);
+                    x += w * v.x;
+                    y += w * v.y;
+                    l += w * f[S::kRows * D + S::kRows + r];
+                }
+                const bool none = l == 0.f || i >= len.rows;
+                const float inv = none ? 0.f : 1.f / l;
+                *reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col)) = none ? 0u : pack2<BF16>(x * inv, y * inv);
+            }
+            cluster.sync();  // no CTA leaves while another reads its part
+            return;
+        }
         if (tid == 0 && ua == 0 && ub < units) {
             const int64_t end = item_first + units;  // the CTA of the item's last unit
             const int last = (int)((end * share.ctas - 1) / share.total);
@@ -325,49 +378,98 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
     }
 }
 
-// Joins the parts of the item that starts in CTA blockIdx.x's share, in the order of its keys.
-template <bool BF16> __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, int rows, int d_pad) {  // blockIdx.y: sixteen rows
+// Joins the parts of the item that starts in CTA blockIdx.x's share, in the order of its keys: four rows per CTA, two warps a row, which take the parts in
+// turn; a lane has four columns.
+constexpr int kJoinRows = 4;
+template <bool BF16> __global__ void __launch_bounds__(64 * kJoinRows) attention_join_kernel(const AttnArgs a, int rows, int d_pad) {
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int4 info = a.info[blockIdx.x];
     if (info.z == 0) return;
+    __shared__ float4 s_sum[kJoinRows][32];
     const int seq = info.x, head = info.y / a.tiles, tile = info.y % a.tiles, pieces = info.z, d = a.c.head_dim;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, which = warp & 1, r = kJoinRows * blockIdx.y + (warp >> 1), row = tile * rows + r, i = row / a.group;
     const size_t floats = (size_t)rows * (d_pad + 2);
     auto part = [&](int p) { return a.parts + ((size_t)(blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * floats; };
-    for (int idx = threadIdx.x; idx < 16 * (d / 2); idx += blockDim.x) {
-        const int r = 16 * blockIdx.y + idx / (d / 2), col = 2 * (idx % (d / 2)), row = tile * rows + r, i = row / a.group;
-        if (i >= a.rows) continue;
-        float m = -INFINITY;
-        for (int p = 0; p < pieces; ++p) m = fmaxf(m, part(p)[rows * d_pad + r]);
-        const float b = m == -INFINITY ? 0.f : m;
-        float x = 0.f, y = 0.f, l = 0.f;
-        for (int p = 0; p < pieces; ++p) {
-            const float *f = part(p);
-            const float w = exp2f(f[rows * d_pad + r] - b);
-            const float2 v = *reinterpret_cast<const float2 *>(f + r * d_pad + col);
-            x += w * v.x;
-            y += w * v.y;
-            l += w * f[rows * d_pad + rows + r];
+    float m = -INFINITY, l = 0.f;
+    if (i < a.rows)
+        for (int p = lane; p < pieces; p += 32) m = fmaxf(m, part(p)[rows * d_pad + r]);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float base = m == -INFINITY ? 0.f : m;
+    if (i < a.rows)
+        for (int p = lane; p < pieces; p += 32) l += exp2f(part(p)[rows * d_pad + r] - base) * part(p)[rows * d_pad + rows + r];
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const bool none = l == 0.f || i >= info.w;
+    const float inv = none ? 0.f : 1.f / l;
+    for (int c0 = 0; c0 < d; c0 += 128) {
+        const int col = c0 + 4 * lane;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < a.rows && col < d) {
+#pragma unroll 8
+            for (int p = which; p < pieces; p += 2) {
+                const float *f = part(p);
+                const float w = exp2f(f[rows * d_pad + r] - base);
+                const float4 v = *reinterpret_cast<const float4 *>(f + (size_t)r * d_pad + col);
+                sum.x += w * v.x;
+                sum.y += w * v.y;
+                sum.z += w * v.z;
+                sum.w += w * v.w;
+            }
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        *reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col)) = l == 0.f || i >= info.w ? 0u : pack2<BF16>(x * inv, y * inv);
+        __syncthreads();
+        if (which) s_sum[warp >> 1][lane] = sum;
+        __syncthreads();
+        if (!which && i < a.rows && col < d) {
+            const float4 v = s_sum[warp >> 1][lane];
+            uint32_t *to = reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col));
+            to[0] = none ? 0u : pack2<BF16>((sum.x + v.x) * inv, (sum.y + v.y) * inv);
+            to[1] = none ? 0u : pack2<BF16>((sum.z + v.z) * inv, (sum.w + v.w) * inv);
+        }
     }
 }
 
 int launch_attention_join(zq_ctx *ctx, const AttnArgs &a, bool bf16, int ctas, int rows, int d_pad, zq_error *err) {
-    return launch_pdl(ctx, bf16 ? attention_join_kernel<true> : attention_join_kernel<false>, dim3((unsigned)ctas, (unsigned)(rows / 16)), dim3(256), 0, err, a, rows, d_pad);
+    return launch_pdl(ctx, bf16 ? attention_join_kernel<true> : attention_join_kernel<false>, dim3((unsigned)ctas, (unsigned)(rows / kJoinRows)), dim3(64 * kJoinRows), 0, err, a, rows, d_pad);
 }
+
+constexpr size_t kClusterBytes = size_t(512) << 10;
 
 template <int D, int WM, bool BF16> static int launch_shape(zq_ctx *ctx, AttnArgs &a, zq_error *err) {
     using S = AttnShape<D, WM>;
     a.tiles = (a.rows * a.group + S::kRows - 1) / S::kRows;
+    ZQ_CUDA_CHECK(cudaFuncSetAttribute(tree_attention_kernel<D, WM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), err);
+    // A cluster per item where that gives each of its CTAs no more of the cache than kClusterBytes, by the room in the block table (the lengths are on the
+    // device): one sequence, 8 cache heads of 128 f16 at 4000 / 8000 / 16000 positions (0.25 / 0.5 / 1 MB a CTA) takes 14.1 / 19.7 / 32.0 us in clusters and
+    // 16.8 / 22.0 / 29.5 with the second kernel, heads of 64 at 1000 / 16000 (0.03 / 0.5 MB) 8.2 / 22.4 and 11.5 / 21.7.  Clusters of at most eight CTAs:
+    // those of sixteen find room one after the other (17.5 us instead of 8.9 at 517 positions).
+    const size_t items = (size_t)a.batch * a.c.heads * a.tiles, positions = (size_t)a.c.max_blocks << a.c.page_shift, units_most = (positions + S::kUnit - 1) / S::kUnit;
+    a.split = 8;
+    while (a.split > 1 && (items * a.split > (size_t)ctx->sm_count || (size_t)a.split >= 2 * units_most)) a.split /= 2;
+    if (items * a.split <= (size_t)ctx->sm_count && positions * a.c.head_dim * 4 <= kClusterBytes * a.split) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(items * a.split));
+        cfg.blockDim = dim3(S::kThreads);
+        cfg.dynamicSmemBytes = S::kSmem;
+        cfg.stream = ctx->stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)a.split;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = ctx->disable_pdl ? 1 : 2;
+        ZQ_CUDA_CHECK(cudaLaunchKernelEx(&cfg, tree_attention_kernel<D, WM, BF16>, a), err);
+        ctx->launches++;
+        return ZQ_OK;
+    }
+    a.split = 0;
     const size_t ctas = (size_t)ctx->sm_count, bytes = ctas * 2 * S::kPartFloats * sizeof(float);
     LaunchScratch scratch;
     int rc = scratch.take(ctx, bytes + ctas * sizeof(int4), err);
     if (rc) return rc;
     a.parts = static_cast<float *>(scratch.p);
     a.info = reinterpret_cast<int4 *>(static_cast<uint8_t *>(scratch.p) + bytes);
-    ZQ_CUDA_CHECK(cudaFuncSetAttribute(tree_attention_kernel<D, WM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), err);
     rc = launch_pdl(ctx, tree_attention_kernel<D, WM, BF16>, dim3((unsigned)ctas), dim3(S::kThreads), S::kSmem, err, a);
     if (rc) return rc;
     return launch_attention_join(ctx, a, BF16, (int)ctas, S::kRows, D, err);

@@ -16,6 +16,7 @@ struct AttnArgs {
     int4 *info;       // [gridDim.x]: {sequence, head * tiles + tile, pieces, rows of the sequence} of the item that starts in this CTA's share and ends in another's
     int64_t q_stride;
     int batch, rows, group, tiles, words;  // tiles: row tiles of a (sequence, head)
+    int split;        // CTAs of a cluster that share an item, 0: shares of all items in one line
     float scale;      // of the scores, log2(e) included
     uint32_t *status;
 };
@@ -32,10 +33,29 @@ __device__ __forceinline__ SeqLen seq_len(const AttnArgs &a, int seq) {
     }
     return s;
 }
-// Does row i of the sequence see its drafted row j?
-__device__ __forceinline__ bool sees(const AttnArgs &a, int seq, int i, int j) {
-    if (!a.mask) return j <= i;
-    return a.mask[((size_t)seq * a.rows + i) * a.words + (j >> 6)] >> (j & 63) & 1;
+// 32 bits of a row's view of the drafted rows, from row d on (d may be negative: the context, which it sees).
+__device__ __forceinline__ uint32_t view32(const AttnArgs &a, int seq, int i, int d, int rows) {
+    if (i >= rows) return 0u;
+    uint32_t v;
+    if (d <= -32) {
+        v = 0xffffffffu;
+    } else {
+        const int from = d < 0 ? 0 : d, skip = d < 0 ? -d : 0;
+        uint32_t bits;  // drafted rows [from, from + 32)
+        if (!a.mask) {
+            const int n = i - from + 1;
+            bits = n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+        } else {
+            const unsigned long long *m = a.mask + ((size_t)seq * a.rows + i) * a.words;
+            const int w = from >> 6, o = from & 63;
+            unsigned long long x = w < a.words ? m[w] >> o : 0;
+            if (o > 32 && w + 1 < a.words) x |= m[w + 1] << (64 - o);
+            bits = (uint32_t)x;
+        }
+        v = skip ? bits << skip | ((1u << skip) - 1) : bits;
+    }
+    const int n = rows - d;  // keys there are
+    return n <= 0 ? 0u : n >= 32 ? v : v & ((1u << n) - 1);
 }
 
 template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {

@@ -132,31 +132,6 @@ struct WideBars {
 constexpr uint32_t kFull = 0, kEmpty = 80, kScores = 160, kWeights = 176, kSums = 192, kQ = 208, kEnd = 224;
 static_assert(sizeof(WideBars) <= 3072 && offsetof(WideBars, q) == kQ && offsetof(WideBars, end) == kEnd, "barriers");
 
-// 32 bits of a row's view of the drafted rows, from row d on (d may be negative: the context, which it sees).
-__device__ __forceinline__ uint32_t view32(const AttnArgs &a, int seq, int i, int d, int rows) {
-    if (i >= rows) return 0u;
-    uint32_t v;
-    if (d <= -32) {
-        v = 0xffffffffu;
-    } else {
-        const int from = d < 0 ? 0 : d, skip = d < 0 ? -d : 0;
-        uint32_t bits;  // drafted rows [from, from + 32)
-        if (!a.mask) {
-            const int n = i - from + 1;
-            bits = n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
-        } else {
-            const unsigned long long *m = a.mask + ((size_t)seq * a.rows + i) * a.words;
-            const int w = from >> 6, o = from & 63;
-            unsigned long long x = w < a.words ? m[w] >> o : 0;
-            if (o > 32 && w + 1 < a.words) x |= m[w + 1] << (64 - o);
-            bits = (uint32_t)x;
-        }
-        v = skip ? bits << skip | ((1u << skip) - 1) : bits;
-    }
-    const int n = rows - d;  // keys there are
-    return n <= 0 ? 0u : n >= 32 ? v : v & ((1u << n) - 1);
-}
-
 __device__ __forceinline__ bool poll(uint32_t at, uint32_t parity) {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(at), "r"(parity) : "memory");
