@@ -43,6 +43,8 @@ template <bool BF16> __device__ __forceinline__ void mma16(float (&d)[4], const 
     else
         mma_16816(d, a[0], a[1], a[2], a[3], b0, b1);
 }
+constexpr int kMaxSplit = 8;  // CTAs of an item in a cluster
+
 // Shape of the kernel for a head of up to D values and WM warps of 16 rows.
 template <int D, int WM> struct AttnShape {
     static constexpr int kGroups = WM == 4 ? 2 : 4;              // key groups of a CTA
@@ -131,14 +133,6 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
             }
             cp_commit();
         };
-        int64_t ahead = page_of(0);
-#pragma unroll 1
-        for (int s = 0; s < S::kStages - 1; ++s) {  // small code: it runs once per item, at the pace of instruction fetches
-            const int64_t now = ahead;
-            ahead = page_of(s + 1);
-            fill(s, now);
-        }
-
         // ---- the rows of this warp
         constexpr int kK = D / 16;
         uint32_t qf[kK][4];
@@ -155,6 +149,14 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
                 qf[k][3] = r_hi < n_rows && col + 8 < d ? *reinterpret_cast<const uint32_t *>(p_hi + 2 * col + 16) : 0u;
             }
         }
+        int64_t ahead = page_of(0);
+#pragma unroll 1
+        for (int s = 0; s < S::kStages - 1; ++s) {  // small code: it runs once per item, at the pace of instruction fetches
+            const int64_t now = ahead;
+            ahead = page_of(s + 1);
+            fill(s, now);
+        }
+
         float o[D / 8][4];
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -314,7 +316,8 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
         __syncthreads();
         const bool whole = !a.split && ua == 0 && ub == units;
         float *part = a.split ? reinterpret_cast<float *>(smem + S::kPartAt) : a.parts + ((size_t)blockIdx.x * 2 + (ua == 0 ? 1 : 0)) * S::kPartFloats;  // in a cluster its own memory
-        for (int idx = tid; idx < S::kRows * (D / 2); idx += S::kThreads) {
+        const int n_out = min(S::kRows, a.rows * a.group - tile * S::kRows) * (D / 2);  // pairs of columns of the tile's rows
+        for (int idx = tid; idx < n_out; idx += S::kThreads) {
             const int r = idx / (D / 2), col = 2 * (idx % (D / 2)), row = tile * S::kRows + r, i = row / a.group;
             float m = -INFINITY;
 #pragma unroll
@@ -346,24 +349,32 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
         if (a.split) {
             cg::cluster_group cluster = cg::this_cluster();
             cluster.sync();
-            for (int idx = (int)cluster.block_rank() * S::kThreads + tid; idx < S::kRows * (D / 2); idx += a.split * S::kThreads) {
+            for (int idx = tid * a.split + (int)cluster.block_rank(); idx < n_out; idx += a.split * S::kThreads) {
                 const int r = idx / (D / 2), col = 2 * (idx % (D / 2)), row = tile * S::kRows + r, i = row / a.group;
-                if (i >= a.rows || col >= d) continue;
-                float m = -INFINITY, x = 0.f, y = 0.f, l = 0.f;
-                for (int p = 0; p < a.split; ++p) m = fmaxf(m, cluster.map_shared_rank(part, p)[S::kRows * D + r]);
+                float top_of[kMaxSplit], sum_of[kMaxSplit], m = -INFINITY, x = 0.f, y = 0.f, l = 0.f;
+                float2 v[kMaxSplit];
+#pragma unroll
+                for (int p = 0; p < kMaxSplit; ++p) {
+                    const float *f = cluster.map_shared_rank(part, p < a.split ? p : 0);
+                    top_of[p] = p < a.split ? f[S::kRows * D + r] : -INFINITY;
+                    sum_of[p] = f[S::kRows * D + S::kRows + r];
+                    v[p] = *reinterpret_cast<const float2 *>(f + r * D + col);
+                }
+#pragma unroll
+                for (int p = 0; p < kMaxSplit; ++p) m = fmaxf(m, top_of[p]);
                 const float b = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-                for (int p = 0; p < a.split; ++p) {
-                    const float *f = cluster.map_shared_rank(part, p);
-                    const float w = exp2f(f[S::kRows * D + r] - b);
-                    const float2 v = *reinterpret_cast<const float2 *>(f + r * D + col);
-                    x += w * v.x;
-                    y += w * v.y;
-                    l += w * f[S::kRows * D + S::kRows + r];
+#pragma unroll
+                for (int p = 0; p < kMaxSplit; ++p) {
+                    if (p < a.split) {
+                        const float w = exp2f(top_of[p] - b);
+                        x += w * v[p].x;
+                        y += w * v[p].y;
+                        l += w * sum_of[p];
+                    }
                 }
                 const bool none = l == 0.f || i >= len.rows;
                 const float inv = none ? 0.f : 1.f / l;
-                *reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col)) = none ? 0u : pack2<BF16>(x * inv, y * inv);
+                if (col < d) *reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col)) = none ? 0u : pack2<BF16>(x * inv, y * inv);
             }
             cluster.sync();  // no CTA leaves while another reads its part
             return;
@@ -443,7 +454,7 @@ template <int D, int WM, bool BF16> static int launch_shape(zq_ctx *ctx, AttnArg
     // 16.8 / 22.0 / 29.5 with the second kernel, heads of 64 at 1000 / 16000 (0.03 / 0.5 MB) 8.2 / 22.4 and 11.5 / 21.7.  Clusters of at most eight CTAs:
     // those of sixteen find room one after the other (17.5 us instead of 8.9 at 517 positions).
     const size_t items = (size_t)a.batch * a.c.heads * a.tiles, positions = (size_t)a.c.max_blocks << a.c.page_shift, units_most = (positions + S::kUnit - 1) / S::kUnit;
-    a.split = 8;
+    a.split = kMaxSplit;
     while (a.split > 1 && (items * a.split > (size_t)ctx->sm_count || (size_t)a.split >= 2 * units_most)) a.split /= 2;
     if (items * a.split <= (size_t)ctx->sm_count && positions * a.c.head_dim * 4 <= kClusterBytes * a.split) {
         cudaLaunchConfig_t cfg = {};
