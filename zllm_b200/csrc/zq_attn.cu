@@ -399,48 +399,51 @@ template <bool BF16> __global__ void __launch_bounds__(64 * kJoinRows) attention
     if (info.z == 0) return;
     __shared__ float4 s_sum[kJoinRows][32];
     const int seq = info.x, head = info.y / a.tiles, tile = info.y % a.tiles, pieces = info.z, d = a.c.head_dim;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, which = warp & 1, r = kJoinRows * blockIdx.y + (warp >> 1), row = tile * rows + r, i = row / a.group;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, which = warp & 1;
     const size_t floats = (size_t)rows * (d_pad + 2);
     auto part = [&](int p) { return a.parts + ((size_t)(blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * floats; };
-    float m = -INFINITY, l = 0.f;
-    if (i < a.rows)
-        for (int p = lane; p < pieces; p += 32) m = fmaxf(m, part(p)[rows * d_pad + r]);
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.f : m;
-    if (i < a.rows)
-        for (int p = lane; p < pieces; p += 32) l += exp2f(part(p)[rows * d_pad + r] - base) * part(p)[rows * d_pad + rows + r];
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    const bool none = l == 0.f || i >= info.w;
-    const float inv = none ? 0.f : 1.f / l;
-    for (int c0 = 0; c0 < d; c0 += 128) {
-        const int col = c0 + 4 * lane;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i < a.rows && col < d) {
+    for (int r = kJoinRows * blockIdx.y + (warp >> 1); r < rows; r += kJoinRows * gridDim.y) {
+        const int row = tile * rows + r, i = row / a.group;
+        float m = -INFINITY, l = 0.f;
+        if (i < a.rows)
+            for (int p = lane; p < pieces; p += 32) m = fmaxf(m, part(p)[rows * d_pad + r]);
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float base = m == -INFINITY ? 0.f : m;
+        if (i < a.rows)
+            for (int p = lane; p < pieces; p += 32) l += exp2f(part(p)[rows * d_pad + r] - base) * part(p)[rows * d_pad + rows + r];
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const bool none = l == 0.f || i >= info.w;
+        const float inv = none ? 0.f : 1.f / l;
+        for (int c0 = 0; c0 < d; c0 += 128) {
+            const int col = c0 + 4 * lane;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i < a.rows && col < d) {
 #pragma unroll 8
-            for (int p = which; p < pieces; p += 2) {
-                const float *f = part(p);
-                const float w = exp2f(f[rows * d_pad + r] - base);
-                const float4 v = *reinterpret_cast<const float4 *>(f + (size_t)r * d_pad + col);
-                sum.x += w * v.x;
-                sum.y += w * v.y;
-                sum.z += w * v.z;
-                sum.w += w * v.w;
+                for (int p = which; p < pieces; p += 2) {
+                    const float *f = part(p);
+                    const float w = exp2f(f[rows * d_pad + r] - base);
+                    const float4 v = *reinterpret_cast<const float4 *>(f + (size_t)r * d_pad + col);
+                    sum.x += w * v.x;
+                    sum.y += w * v.y;
+                    sum.z += w * v.z;
+                    sum.w += w * v.w;
+                }
             }
-        }
-        __syncthreads();
-        if (which) s_sum[warp >> 1][lane] = sum;
-        __syncthreads();
-        if (!which && i < a.rows && col < d) {
-            const float4 v = s_sum[warp >> 1][lane];
-            uint32_t *to = reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col));
-            to[0] = none ? 0u : pack2<BF16>((sum.x + v.x) * inv, (sum.y + v.y) * inv);
-            to[1] = none ? 0u : pack2<BF16>((sum.z + v.z) * inv, (sum.w + v.w) * inv);
+            __syncthreads();
+            if (which) s_sum[warp >> 1][lane] = sum;
+            __syncthreads();
+            if (!which && i < a.rows && col < d) {
+                const float4 v = s_sum[warp >> 1][lane];
+                uint32_t *to = reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col));
+                to[0] = none ? 0u : pack2<BF16>((sum.x + v.x) * inv, (sum.y + v.y) * inv);
+                to[1] = none ? 0u : pack2<BF16>((sum.z + v.z) * inv, (sum.w + v.w) * inv);
+            }
         }
     }
 }
 
 int launch_attention_join(zq_ctx *ctx, const AttnArgs &a, bool bf16, int ctas, int rows, int d_pad, zq_error *err) {
-    return launch_pdl(ctx, bf16 ? attention_join_kernel<true> : attention_join_kernel<false>, dim3((unsigned)ctas, (unsigned)(rows / kJoinRows)), dim3(64 * kJoinRows), 0, err, a, rows, d_pad);
+    return launch_pdl(ctx, bf16 ? attention_join_kernel<true> : attention_join_kernel<false>, dim3((unsigned)ctas, (unsigned)(rows / kJoinRows < 16 ? rows / kJoinRows : 16)), dim3(64 * kJoinRows), 0, err, a, rows, d_pad);
 }
 
 constexpr size_t kClusterBytes = size_t(512) << 10;

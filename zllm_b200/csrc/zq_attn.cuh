@@ -75,12 +75,6 @@ template <bool BF16> __device__ __forceinline__ bool drop_nonfinite(uint32_t &w)
     if (hi) w &= 0x0000ffffu;
     return lo || hi;
 }
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
 struct Share {
     int64_t first, last, total;  // units of this CTA; of all
     int ctas;                    // with a share

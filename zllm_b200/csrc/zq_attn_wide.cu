@@ -71,24 +71,6 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *m
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(head), "r"(row), "r"(page)
                  : "memory");
 }
-// Two f32 operations at once.
-__device__ __forceinline__ uint64_t pair64(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpair64(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t twice(float v) { return pair64(__float_as_uint(v), __float_as_uint(v)); }
 // 2^y of both halves on the FMA units, which have time where the exponential units have not: 2^n (n the nearest whole number) times a polynomial of degree 4
 // in the rest, fitted to the least relative error on [-1/2, 1/2] (2.7e-6, against 2^-12 of a weight's rounding).  y is at most about 8; below -126
 // it counts as -126.

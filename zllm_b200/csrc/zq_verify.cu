@@ -12,8 +12,10 @@
 // the same decision.  A row is read once for its largest logit and sum (f32); where the walk ends, once more (from L2) for f64 weights,
 // kept as one sum per segment of tokens.  The pick looks for its CTA, then its segment, then its token, and evaluates one segment again.
 //
-// What rejections of drawn children leave has a closed form: after k of them p is (p - m q)+ / Z with m = 1 at first and m + Z after each, Z the
-// sum of (p - m q)+.  So a rejection is one pass, in f32 for the test of the next child and, for those of the last row only, in f64.
+// What rejections of drawn children leave has a closed form: after k of them p is (p - m_k q)+ / Z_k with m_1 = 1 and m_(k+1) = m_k + Z_k, Z_k the
+// sum of (p - m_k q)+.  For the test of the next child Z_k is summed in f32.  Where the walk ends, one pass finds it in f64, for two rejections at a
+// time, although each m_k hangs on the Z before it: the pass sums at the m that f32 gave, along with the q of the tokens that count, which is
+// the sum's slope, and the sums are moved to the exact m afterwards (it lies 1e-7 away, so that what the line leaves out is 1e-14).
 #include <cooperative_groups.h>
 
 #include "zq_draft.cuh"
@@ -22,22 +24,23 @@ namespace zq {
 
 namespace cg = cooperative_groups;
 
-// 1024 threads of an SM in four CTAs: each pass waits for memory and for chains of dependent operations more than for issue slots (with 512 threads of
-// twice the tokens at a time 64 sequences of 128 003 tokens took 235 us, so 170).
-constexpr int kVerifyThreads = 256, kVerifyCtas = 4, kVerifyWarps = kVerifyThreads / 32, kMaxCluster = 16, kSegment = 256;  // tokens that a warp takes at a time and whose sum is kept
+// 1024 threads of an SM in four CTAs: each pass waits for memory and for chains of dependent operations more than for issue slots (64 sequences of 128 003
+// tokens take 150 us; with 768 threads 214, with 512 of twice the registers 179).
+constexpr int kVerifyThreads = 256, kVerifyCtas = 4, kVerifyWarps = kVerifyThreads / 32, kMaxCluster = 16, kAhead = 2, kSegment = 256;  // tokens that a warp takes at a time and whose sum is kept
 constexpr float kHeavy = -18.f;  // weights above 2^kHeavy of the largest are evaluated in f64
+constexpr int kSums = 6;         // sums of a pass over both rows: of p, of q; at two m: of what is left, its slope
 
 struct VerifyArgs {
     const uint8_t *logits, *draft;
     const int32_t *tokens, *parents, *lens;
     const float *accept_u, *sample_u, *temperature;
     int32_t *path, *accepted, *token;
-    int64_t vocab;
-    int rows, shared_parents, segments;  // segments of a CTA
+    int vocab, rows, shared_parents, segments;  // segments of a CTA
     uint32_t *status;
 };
 
-// A row's largest logit (NaN if the row holds one), its first place, and the sum of its weights relative to it.
+// A row's largest logit (NaN if the row holds one; where its place is not asked for, one that is not far below), its first place, and the sum of its weights
+// relative to it.
 struct RowPart {
     float top;
     int32_t at;
@@ -45,15 +48,19 @@ struct RowPart {
 };
 
 struct VerifyShared {
-    RowPart part[2][2][kMaxCluster];  // [exchanges in turn][target, draft]: what the CTAs of the cluster tell each other
+    // what the CTAs of the cluster tell each other, in two sets of places in turn
+    RowPart part[2][2][kMaxCluster];  // [..][target, draft]
+    double sums[2][kSums][kMaxCluster];
     RowPart warp_part[2][kVerifyWarps];
+    double warp_sums[kSums][kVerifyWarps];
+    double m[kMaxDraftRows];          // of the rejections at this row (drawn children)
     int32_t gone[kMaxDraftRows];      // rejected tokens at this row (chosen children)
     int32_t parent[kMaxDraftRows], token[kMaxDraftRows];
     float u[kMaxDraftRows];
-    float2 list[kVerifyWarps][kSegment];
+    alignas(16) float2 list[kVerifyWarps][kSegment];
 };
 
-template <class T> __device__ __forceinline__ float logit(const T *row, int64_t v) {
+template <class T> __device__ __forceinline__ float logit(const T *row, int v) {
     if constexpr (sizeof(T) == 4) return row[v];
     else if constexpr (std::is_same<T, __half>::value) return __half2float(row[v]);
     else return __bfloat162float(row[v]);
@@ -64,7 +71,7 @@ template <class T> __device__ __forceinline__ float logit(const T *row, int64_t 
 template <class T> struct Eight {
     static constexpr int kPer = 16 / sizeof(T);
     uint4 w[8 / kPer];
-    __device__ __forceinline__ void load(const T *row, int64_t v, int64_t vocab, bool wide) {
+    __device__ __forceinline__ void load(const T *row, int v, int vocab, bool wide) {
         if (wide && v >= 0 && v + 8 <= vocab) {
 #pragma unroll
             for (int j = 0; j < 8 / kPer; ++j) w[j] = *reinterpret_cast<const uint4 *>(row + v + j * kPer);
@@ -89,11 +96,6 @@ template <class T> struct Eight {
     }
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 __device__ __forceinline__ double warp_sum(double x) {
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
@@ -140,45 +142,65 @@ struct Weights {
     }
 };
 
-// The sum over a lane's tokens of `value` in f64 where a weight is heavy and of `light` elsewhere.  Few tokens are heavy: the warp lists them
-// and takes 32 at a time.
-template <class Heavy, class Value, class Light> __device__ __forceinline__ double lane_sum(float2 *list, const float (&l)[8], const float (&ql)[8], Heavy heavy, Value value, Light light) {
-    const int lane = threadIdx.x & 31;
-    unsigned heavies = 0;
-    float some = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float w = light(l[e], ql[e]);
-        const bool h = heavy(l[e], ql[e]);
-        if (h) heavies |= 1u << e;
-        some += h ? 0.f : w;
-    }
-    double t = (double)some;
-    const int mine = __popc(heavies);
+// Puts a lane's heavy tokens (bits of its eight) into the warp's list; returns how many there are.  Few are heavy, and the warp takes 32 of the list at a time.
+__device__ __forceinline__ int list_heavy(float2 *list, const float (&l)[8], const float (&ql)[8], unsigned heavies) {
+    const int lane = threadIdx.x & 31, mine = __popc(heavies);
     int incl = mine;
     for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += up;
     }
     const int total = __shfl_sync(0xffffffffu, incl, 31);
-    if (total == 0) return t;
-    int at = incl - mine;
+    if (total) {
+        int at = incl - mine;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (heavies >> e & 1) list[at++] = make_float2(l[e], ql[e]);
-    __syncwarp();
-    for (int i = lane; i - lane < total; i += 32) {
-        const float2 x = list[min(i, total - 1)];
-        const double v = value(x.x, x.y);
-        if (i < total) t += v;
+        for (int e = 0; e < 8; ++e)
+            if (heavies >> e & 1) list[at++] = make_float2(l[e], ql[e]);
+        __syncwarp();
     }
-    __syncwarp();
-    return t;
+    return total;
+}
+
+// Joins (largest, place, sum) of the lanes of a warp; a NaN stays.
+__device__ __noinline__ RowPart join_lanes(RowPart p, float scale32) {
+    RowPart m = p;
+    for (int o = 16; o > 0; o >>= 1) {
+        const float top = __shfl_xor_sync(0xffffffffu, m.top, o);
+        const int32_t at = __shfl_xor_sync(0xffffffffu, m.at, o);
+        if (isnan(top) || top > m.top || (top == m.top && at < m.at)) {
+            m.top = top;
+            m.at = at;
+        }
+    }
+    m.sum = warp_sum(p.top == -INFINITY ? 0.0 : p.sum * (double)exp2f((p.top - m.top) * scale32));
+    return m;
+}
+// Every CTA gets every CTA's part: the warps' parts are joined by a warp each, which stores the result into all CTAs.
+__device__ __noinline__ void exchange_rows(VerifyShared &s, int parity, bool both, float scale32) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __syncthreads();
+    if (warp < (both ? 2 : 1)) {
+        const RowPart p = join_lanes(lane < kVerifyWarps ? s.warp_part[warp][lane] : RowPart{-INFINITY, 0x7fffffff, 0.0}, scale32);
+        if (lane < (int)cluster.num_blocks()) cluster.map_shared_rank(&s, lane)->part[parity][warp][cluster.block_rank()] = p;
+    }
+    cluster.sync();
+}
+__device__ __noinline__ void exchange_sums(VerifyShared &s, int parity, int n) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    static_assert(kSums <= kVerifyWarps, "a warp each");
+    __syncthreads();
+    if (warp < n) {
+        const double sum = warp_sum(lane < kVerifyWarps ? s.warp_sums[warp][lane] : 0.0);
+        if (lane < (int)cluster.num_blocks()) cluster.map_shared_rank(&s, lane)->sums[parity][warp][cluster.block_rank()] = sum;
+    }
+    cluster.sync();
 }
 
 template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) verify_draft_kernel(const VerifyArgs a) {
     pdl_launch_dependents();
-    extern __shared__ double s_seg[];  // sums of this CTA's segments
+    extern __shared__ double s_seg[];  // sums of this CTA's segments, then their slopes
     __shared__ VerifyShared s;
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), seq = blockIdx.x / ctas;
@@ -197,127 +219,101 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
     const bool greedy = heat == 0.f, drawn = a.draft != nullptr && !greedy;
     const double scale = 1.4426950408889634074 / (greedy ? 1.0 : (double)heat);
     const float scale32 = (float)fmin(scale, 1e30);
-    const int64_t first = (int64_t)rank * a.segments, last = first + a.segments;
+    const int first = rank * a.segments, last = first + a.segments;
+    constexpr int kNowhere = 1 << 22;  // a segment behind every row's end
     int parity = 0, node = 0, count = 0, token = -1;
     bool bad = n > 0 && !(heat >= 0.f && heat < INFINITY);
 
     const T *row = nullptr, *qrow = nullptr;
-    int64_t shift = 0;
-    bool wide = false, q_wide = false;
+    int shift = 0;
+    bool q_wide = false;
     Weights pw, qw;
     double p_inv = 0, q_inv = 0;  // 1 / sum of weights
-    double m = 0, rest = 1;         // drawn children: p is (p - m q)+ / rest
     int n_gone = 0;
 
-    // Joins (largest, place, sum) of the lanes of a warp; a NaN stays.
-    auto join_lanes = [&](RowPart p) {
-        RowPart m = p;
-        for (int o = 16; o > 0; o >>= 1) {
-            const float top = __shfl_xor_sync(0xffffffffu, m.top, o);
-            const int32_t at = __shfl_xor_sync(0xffffffffu, m.at, o);
-            if (isnan(top) || top > m.top || (top == m.top && at < m.at)) {
-                m.top = top;
-                m.at = at;
-            }
-        }
-        m.sum = warp_sum(p.top == -INFINITY ? 0.0 : p.sum * (double)exp2f((p.top - m.top) * scale32));
-        return m;
-    };
-    // Every CTA gets every CTA's part: the warps' parts are joined by the first warp, which stores the result into all CTAs.
-    auto exchange = [&](bool both, bool sums_only) {
-        parity ^= 1;
-        __syncthreads();
-        if (warp < (both ? 2 : 1)) {
-            RowPart p = lane < kVerifyWarps ? s.warp_part[warp][lane] : RowPart{-INFINITY, 0x7fffffff, 0.0};
-            if (sums_only) p.sum = warp_sum(p.sum);
-            else p = join_lanes(p);
-            if (lane < ctas) cluster.map_shared_rank(&s, lane)->part[parity][warp][rank] = p;
-        }
-        cluster.sync();
-    };
     // Largest logit, its place and 1 / sum of a row from all CTAs' parts.
     auto joined = [&](int which, Weights &w, double &inv, int32_t &at) {
-        const RowPart p = join_lanes(lane < ctas ? s.part[parity][which][lane] : RowPart{-INFINITY, 0x7fffffff, 0.0});
+        const RowPart p = join_lanes(lane < ctas ? s.part[parity][which][lane] : RowPart{-INFINITY, 0x7fffffff, 0.0}, scale32);
         at = p.at;
         inv = 1.0 / p.sum;
         w.set(scale, p.top);
         return isfinite(p.top);
     };
-    auto total_of = [&](int which) { return warp_sum(lane < ctas ? s.part[parity][which][lane].sum : 0.0); };
-    auto place = [&](int64_t g) { return g * kSegment + lane * 8 - shift; };
-    auto load = [&](const T *r, bool w, int64_t g, float (&l)[8]) {
+    auto total_of = [&](int which) { return warp_sum(lane < ctas ? s.sums[parity][which][lane] : 0.0); };
+    auto place = [&](int g) { return g * kSegment + lane * 8 - shift; };
+    auto load = [&](const T *r, bool w, int g, float (&l)[8]) {
         Eight<T> x;
         x.load(r, place(g), a.vocab, w);
         x.get(l);
     };
-    // The largest logit and the sum of weights of this CTA's run of a row, in f32 inside a thread.  A NaN makes the sum one.
-    struct Run {
-        float top = -INFINITY, sum = 0.f;
-        int32_t at = 0x7fffffff;
-    };
-    auto take = [&](Run &run, const float (&l)[8], int64_t g) {
-        float most = l[0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) most = fmaxf(most, l[e]);
-        if (most > run.top) {
-            run.sum *= ex2((run.top - most) * scale32);
-            run.top = most;
-            int e0 = 7;
-#pragma unroll
-            for (int e = 7; e >= 0; --e)
-                if (l[e] == most) e0 = e;
-            run.at = (int32_t)(place(g) + e0);
-        }
-        const float base = run.top == -INFINITY ? 0.f : run.top;
-        float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sums[e & 3] += ex2((l[e] - base) * scale32);
-        run.sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    };
+    // A large logit, its place where it is asked for (greedy), and the sum of weights relative to it, of this CTA's run of the target's row and of the draft's, in f32 inside
+    // a thread.  They are relative to the largest logit of the warp's first segment; where that is none, or is so far from the others that the sum leaves f32's
+    // range, and where the place is asked for, the warp takes its run with a running maximum.  A NaN makes that sum one.
+    const uint64_t scale2 = twice(scale32);
     auto scan = [&](bool both) {
-        Run p, q;
-        for (int64_t g = first + warp; g < last; g += kVerifyWarps) {
-            Eight<T> x, y;
-            x.load(row, place(g), a.vocab, wide);
-            if (both) y.load(qrow, place(g), a.vocab, q_wide);
-            float l[8];
-            x.get(l);
-            take(p, l, g);
-            if (both) {
-                y.get(l);
-                take(q, l, g);
+#pragma unroll 1
+        for (int which = 0; which < (both ? 2 : 1); ++which) {
+            const T *r = which ? qrow : row;
+            const bool w = which ? q_wide : true;
+            float top = -INFINITY;
+            double sum = 0;
+            if (!greedy) {
+                float l[8];
+                load(r, w, first + warp < last ? first + warp : kNowhere, l);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, l[e]);
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                uint64_t sums[2] = {0, 0};
+                const uint64_t base2 = twice(-top);
+                for (int g = first + warp; g < last; g += kAhead * kVerifyWarps) {
+                    Eight<T> x[kAhead];
+#pragma unroll
+                    for (int k = 0; k < kAhead; ++k) x[k].load(r, place(g + k * kVerifyWarps < last ? g + k * kVerifyWarps : kNowhere), a.vocab, w);
+#pragma unroll
+                    for (int k = 0; k < kAhead; ++k) {
+                        x[k].get(l);
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            float lo, hi;
+                            unpair64(mul2(add2(pair64(__float_as_uint(l[e]), __float_as_uint(l[e + 1])), base2), scale2), lo, hi);
+                            sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair64(__float_as_uint(ex2(lo)), __float_as_uint(ex2(hi))));
+                        }
+                    }
+                }
+                float lo, hi;
+                unpair64(add2(sums[0], sums[1]), lo, hi);
+                sum = warp_sum((double)(lo + hi));
             }
+            RowPart p{top, 0x7fffffff, sum};
+            if (!(isfinite(top) && sum >= 0.5 && sum < 1e30)) {
+                float run = -INFINITY, some = 0.f;
+                int32_t at = 0x7fffffff;
+#pragma unroll 1
+                for (int g = first + warp; g < last; g += kVerifyWarps) {
+                    float l[8];
+                    load(r, w, g, l);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (l[e] > run) {
+                            some *= ex2((run - l[e]) * scale32);
+                            run = l[e];
+                            at = place(g) + e;
+                        }
+                        some += ex2((l[e] - (run == -INFINITY ? 0.f : run)) * scale32);
+                    }
+                }
+                p = join_lanes({isnan(some) ? NAN : run, at, (double)some}, scale32);
+            }
+            if (lane == 0) s.warp_part[which][warp] = p;
         }
-        const RowPart jp = join_lanes({isnan(p.sum) ? NAN : p.top, p.at, (double)p.sum});
-        if (lane == 0) s.warp_part[0][warp] = jp;
-        if (both) {
-            const RowPart jq = join_lanes({isnan(q.sum) ? NAN : q.top, q.at, (double)q.sum});
-            if (lane == 0) s.warp_part[1][warp] = jq;
-        }
-    };
-    // What is left of p at a token, times `rest`.  All lanes call it.
-    auto left = [&](float l, float ql, bool two) {
-        const double p = pw(l, root) * p_inv;
-        return two ? fmax(p - m * (qw(ql, root) * q_inv), 0.0) : p;
-    };
-    // Sum of a row's weights (its largest logit is known).
-    auto precise_sum = [&](const T *r, bool w, const Weights &weight, int which) {
-        double mine = 0;
-        for (int64_t g = first + warp; g < last; g += kVerifyWarps) {
-            float l[8];
-            load(r, w, g, l);
-            mine += lane_sum(s.list[warp], l, l, [&](float v, float) { return weight.heavy(v); }, [&](float v, float) { return weight(v, root); }, [&](float v, float) { return weight.light(v); });
-        }
-        mine = warp_sum(mine);
-        if (lane == 0) s.warp_part[which][warp] = {0.f, 0, mine};
     };
     // Takes the rejected tokens out of a lane's tokens of segment g.
-    auto drop_gone = [&](float (&l)[8], int64_t g) {
+    auto drop_gone = [&](float (&l)[8], int g) {
         for (int i0 = 0; i0 < n_gone; i0 += 32) {
-            const int64_t d = i0 + lane < n_gone ? s.gone[i0 + lane] - (g * kSegment - shift) : -1;
+            const int d = i0 + lane < n_gone ? s.gone[i0 + lane] - (g * kSegment - shift) : -1;
             unsigned hits = __ballot_sync(0xffffffffu, d >= 0 && d < kSegment);
             while (hits) {
-                const int at = __shfl_sync(0xffffffffu, (int)d, __ffs(hits) - 1);
+                const int at = __shfl_sync(0xffffffffu, d, __ffs(hits) - 1);
                 hits &= hits - 1;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -325,45 +321,119 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             }
         }
     };
-    // The sums of the segments of what is left, times `rest`; of all of them, over the cluster.
-    auto fill_segments = [&](bool two) {
+    // Sums of the segments of the target's weights, without rejected tokens.
+    auto row_segments = [&] {
         double mine = 0;
-        const float p32 = (float)p_inv, mq32 = (float)(m * q_inv);
-        for (int64_t g = first + warp; g < last; g += kVerifyWarps) {
-            float l[8];
-            double t;
-            load(row, wide, g, l);
-            if (two) {
-                float ql[8];
-                load(qrow, q_wide, g, ql);
-                t = lane_sum(s.list[warp], l, ql, [&](float v, float w) { return pw.heavy(v) || qw.heavy(w); }, [&](float v, float w) { return left(v, w, true); },
-                             [&](float v, float w) { return fmaxf(fmaf(-mq32, qw.light(w), p32 * pw.light(v)), 0.f); });
-            } else {
-                drop_gone(l, g);
-                t = lane_sum(s.list[warp], l, l, [&](float v, float) { return pw.heavy(v); }, [&](float v, float) { return left(v, v, false); }, [&](float v, float) { return p32 * pw.light(v); });
+#pragma unroll 1
+        for (int g = first + warp; g < last; g += kVerifyWarps) {
+            float l[8], some = 0.f;
+            load(row, true, g, l);
+            drop_gone(l, g);
+            unsigned heavies = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool h = pw.heavy(l[e]);
+                if (h) heavies |= 1u << e;
+                some += h ? 0.f : pw.light(l[e]);
+            }
+            const int total = list_heavy(s.list[warp], l, l, heavies);
+            double t = (double)some;
+            for (int i = lane; i - lane < total; i += 32) {
+                const double w = pw(s.list[warp][min(i, total - 1)].x, root);
+                if (i < total) t += w;
             }
             t = warp_sum(t);
-            if (lane == 0) s_seg[g - first] = t;
+            if (lane == 0) {
+                s_seg[g - first] = t;
+                s_seg[a.segments + g - first] = 0;
+            }
             mine += t;
         }
-        if (lane == 0) s.warp_part[0][warp] = {0.f, 0, mine};
-        exchange(false, true);
-        return total_of(0);
+        if (lane == 0) s.warp_sums[0][warp] = mine;
+        exchange_sums(s, parity ^= 1, 1);
     };
-    // The sum of what a rejection leaves, in f32 inside a thread.
-    auto light_rest = [&] {
-        float mine = 0.f;
-        const float p32 = (float)p_inv, mq32 = (float)(m * q_inv);
-        for (int64_t g = first + warp; g < last; g += kVerifyWarps) {
-            float l[8], ql[8];
-            load(row, wide, g, l);
+    // Sums over both rows: of p's weights and q's, and at factors c0 and c1 of (p - c q)+ and of the q in it, at c1 kept for every segment.
+    auto both_segments = [&](double c0, double c1) {
+        const float f0 = (float)c0, f1 = (float)c1;
+        double all[kSums] = {0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+        for (int g = first + warp; g < last; g += kVerifyWarps) {
+            float l[8], ql[8], some[kSums] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            load(row, true, g, l);
             load(qrow, q_wide, g, ql);
+            unsigned heavies = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mine += fmaxf(fmaf(-mq32, ex2((ql[e] - qw.top32) * scale32), p32 * ex2((l[e] - pw.top32) * scale32)), 0.f);
+            for (int e = 0; e < 8; ++e) {
+                const bool h = pw.heavy(l[e]) || qw.heavy(ql[e]);
+                if (h) heavies |= 1u << e;
+                const float p = h ? 0.f : pw.light(l[e]), q = h ? 0.f : qw.light(ql[e]), r0 = fmaf(-f0, q, p), r1 = fmaf(-f1, q, p);
+                some[0] += p;
+                some[1] += q;
+                some[2] += fmaxf(r0, 0.f);
+                some[3] += r0 > 0.f ? q : 0.f;
+                some[4] += fmaxf(r1, 0.f);
+                some[5] += r1 > 0.f ? q : 0.f;
+            }
+            const int total = list_heavy(s.list[warp], l, ql, heavies);
+            double left = (double)some[4], slope = (double)some[5];
+            all[0] += (double)some[0];
+            all[1] += (double)some[1];
+            all[2] += (double)some[2];
+            all[3] += (double)some[3];
+            for (int i = lane; i - lane < total; i += 32) {
+                const float2 x = s.list[warp][min(i, total - 1)];
+                const double p = pw(x.x, root), q = qw(x.y, root);
+                if (i < total) {
+                    const double r0 = p - c0 * q, r1 = p - c1 * q;
+                    all[0] += p;
+                    all[1] += q;
+                    all[2] += fmax(r0, 0.0);
+                    all[3] += r0 > 0 ? q : 0.0;
+                    left += fmax(r1, 0.0);
+                    slope += r1 > 0 ? q : 0.0;
+                }
+            }
+            all[4] += left;
+            all[5] += slope;
+            left = warp_sum(left);
+            slope = warp_sum(slope);
+            if (lane == 0) {
+                s_seg[g - first] = left;
+                s_seg[a.segments + g - first] = slope;
+            }
+            __syncwarp();
         }
-        const double t = warp_sum((double)mine);
-        if (lane == 0) s.warp_part[0][warp] = {0.f, 0, t};
-        exchange(false, true);
+#pragma unroll
+        for (int i = 0; i < kSums; ++i) {
+            all[i] = warp_sum(all[i]);
+            if (lane == 0) s.warp_sums[i][warp] = all[i];
+        }
+        exchange_sums(s, parity ^= 1, kSums);
+    };
+    // The sum of (p - m q)+, in f32 inside a thread.
+    auto light_rest = [&](double m) {
+        const float p32 = (float)p_inv, mq32 = (float)(m * q_inv);
+        float some[2] = {0.f, 0.f};
+        for (int g = first + warp; g < last; g += 2 * kVerifyWarps) {
+            Eight<T> x[2], y[2];
+            const int other = g + kVerifyWarps < last ? g + kVerifyWarps : kNowhere;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                x[k].load(row, place(k ? other : g), a.vocab, true);
+                y[k].load(qrow, place(k ? other : g), a.vocab, q_wide);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float l[8], ql[8];
+                x[k].get(l);
+                y[k].get(ql);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) some[e & 1] += fmaxf(fmaf(-mq32, ex2((ql[e] - qw.top32) * scale32), p32 * ex2((l[e] - pw.top32) * scale32)), 0.f);
+            }
+        }
+        const double t = warp_sum((double)(some[0] + some[1]));
+        if (lane == 0) s.warp_sums[0][warp] = t;
+        exchange_sums(s, parity ^= 1, 1);
         return total_of(0);
     };
 
@@ -372,11 +442,8 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
         if (rank == 0 && tid == 0) a.path[row0] = 0;
         while (true) {
             row = reinterpret_cast<const T *>(a.logits) + (row0 + node) * a.vocab;
-            shift = (int64_t)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-            wide = true;
+            shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
             n_gone = 0;
-            m = 0;
-            rest = 1;
             bool child = false;
             for (int j = node + 1; j < n && !child; ++j) child = s.parent[j] == node;
             const bool use_q = drawn && child;
@@ -385,15 +452,17 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
                 q_wide = ((reinterpret_cast<uintptr_t>(qrow) ^ reinterpret_cast<uintptr_t>(row)) & 15) == 0;
             }
             scan(use_q);
-            exchange(use_q, false);
+            exchange_rows(s, parity ^= 1, use_q, scale32);
             int32_t best, unused;
             bad = !joined(0, pw, p_inv, best);
             if (use_q) bad |= !joined(1, qw, q_inv, unused);
             if (bad) break;
 
+            // ---- its children
             int next = -1;
-            int rejected = 0;  // drawn children
-            double gone = 0;   // what the rejected chosen children had of p
+            int rejected = 0;         // drawn children that left something: p is (p - m q)+ / rest
+            double m = 0, rest = 1;
+            double gone = 0;          // what the rejected chosen children had of p
             for (int j = node + 1; j < n; ++j) {
                 if (s.parent[j] != node) continue;
                 const int t = s.token[j];
@@ -406,32 +475,33 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
                     if (next >= 0) break;
                     continue;
                 }
-                const double u = (double)s.u[j];
-                const float l = logit(row, t);
+                const double u = (double)s.u[j], p = pw(logit(row, t), root) * p_inv;
                 if (drawn) {
-                    const float ql = logit(qrow, t);
-                    if (u * qw(ql, root) * q_inv * rest < left(l, ql, true)) {
+                    const double q = qw(logit(qrow, t), root) * q_inv;
+                    if (u * q * rest < fmax(p - m * q, 0.0)) {
                         next = j;
                         break;
                     }
-                    const double before = m;
-                    m += rest;
-                    const double sum = light_rest();
-                    if (sum > 0) rest = sum;
-                    else m = before;  // nothing left: p stays as it was
-                    ++rejected;
+                    const double sum = light_rest(m + rest);
+                    if (sum > 0) {  // else nothing is left: p stays as it was
+                        m += rest;
+                        rest = sum;
+                        __syncthreads();
+                        if (tid == 0) s.m[rejected] = m;
+                        __syncthreads();
+                        ++rejected;
+                    }
                 } else {
                     bool again = false;
                     for (int i = 0; i < n_gone; ++i) again |= s.gone[i] == t;
-                    const double chance = again ? 0.0 : pw(l, root) * p_inv;
-                    if (u < chance / (1.0 - gone)) {
+                    if (!again && u < p / (1.0 - gone)) {
                         next = j;
                         break;
                     }
-                    if (!again && 1.0 - gone - chance > 0) {
+                    if (!again && 1.0 - gone - p > 0) {
                         __syncthreads();
                         if (tid == 0) s.gone[n_gone] = t;
-                        gone += chance;
+                        gone += p;
                         ++n_gone;
                         __syncthreads();
                     }
@@ -447,35 +517,41 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
                 token = best;
                 break;
             }
-            // ---- nobody kept: a token from what is left
-            bool filled = false;
-            if (rejected) {  // the rejections once more, in f64
-                precise_sum(row, wide, pw, 0);
-                precise_sum(qrow, q_wide, qw, 1);
-                exchange(true, true);
-                p_inv = 1.0 / total_of(0);
-                q_inv = 1.0 / total_of(1);
-                m = 0;
-                rest = 1;
-                for (int i = 0; i < rejected; ++i) {
-                    const double before = m;
+
+            // ---- nobody kept: a token from what is left, weights w_p - factor w_q where that is positive
+            double factor = 0, off = 0;  // off: the exact factor less the one that the segments are taken at
+            int sum_at = 0;              // place of the segments' sum among the pass's sums
+            for (int i = 0; i < rejected; i += 2) {
+                // factors for weights: m times (sum of w_p) / (sum of w_q), as f32 gave them; one rejection counts twice
+                const double by = q_inv / p_inv, c0 = s.m[i] * by, c1 = (i + 1 < rejected ? s.m[i + 1] : s.m[i]) * by;
+                both_segments(c0, c1);
+                const double sum_p = total_of(0), ratio = sum_p / total_of(1);
+                if (i == 0) m = 1;
+                factor = m * ratio;
+                off = factor - c0;
+                rest = (total_of(2) - off * total_of(3)) / sum_p;
+                if (i + 1 < rejected) {
                     m += rest;
-                    const double sum = fill_segments(true);
-                    filled = sum > 0;
-                    if (!filled) {  // and so it would be for the others
-                        m = before;
-                        break;
-                    }
-                    rest = sum;
+                    factor = m * ratio;
+                    off = factor - c1;
+                    rest = (total_of(4) - off * total_of(5)) / sum_p;
                 }
+                m += rest;  // of the next one
+                sum_at = 4;
             }
-            if (!filled) fill_segments(m > 0);
+            if (rejected && !(rest > 0)) rejected = 0;  // nothing left after all
+            if (!rejected) {
+                row_segments();
+                factor = off = 0;
+                sum_at = 0;
+            }
+            auto part_of = [&](int cta) { return sum_at ? fmax(s.sums[parity][4][cta] - off * s.sums[parity][5][cta], 0.0) : s.sums[parity][0][cta]; };
             double total = 0, before = 0, upto = 0;
             int owner = -1, some = 0;
-            for (int i = 0; i < ctas; ++i) total += s.part[parity][0][i].sum;
+            for (int i = 0; i < ctas; ++i) total += part_of(i);
             const double target = (double)a.sample_u[seq] * total;
             for (int i = 0; i < ctas; ++i) {
-                const double part = s.part[parity][0][i].sum;
+                const double part = part_of(i);
                 if (part > 0) some = i;
                 if (owner < 0 && upto + part > target) {
                     owner = i;
@@ -485,13 +561,14 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             }
             if (owner < 0) {  // the target is the total, to rounding
                 owner = some;
-                before = upto - s.part[parity][0][some].sum;
+                before = upto - part_of(some);
             }
             if (owner == rank && warp == 0) {
+                // the segment, 32 at a time
                 double at = before;
-                int64_t found = -1, likely = 0;
-                for (int64_t g0 = 0; g0 < a.segments && found < 0; g0 += 32) {
-                    const double x = g0 + lane < a.segments ? s_seg[g0 + lane] : 0.0;
+                int found = -1, likely = 0;
+                for (int g0 = 0; g0 < a.segments && found < 0; g0 += 32) {
+                    const double x = g0 + lane < a.segments ? fmax(s_seg[g0 + lane] - off * s_seg[a.segments + g0 + lane], 0.0) : 0.0;
                     double incl = x;
                     for (int o = 1; o < 32; o <<= 1) {
                         const double up = __shfl_up_sync(0xffffffffu, incl, o);
@@ -509,15 +586,21 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
                 }
                 const bool end = found < 0;
                 if (end) found = likely;
+                // its tokens, by way of the list: a lane's eight weights one after the other
                 float l[8], ql[8];
-                load(row, wide, first + found, l);
-                if (m > 0) load(qrow, q_wide, first + found, ql);
+                load(row, true, first + found, l);
                 drop_gone(l, first + found);
-                double x[8], t = 0;
+                if (factor > 0) load(qrow, q_wide, first + found, ql);
 #pragma unroll
+                for (int e = 0; e < 8; ++e) s.list[0][lane * 8 + e] = make_float2(l[e], factor > 0 ? ql[e] : 0.f);
+                double t = 0, *weight = reinterpret_cast<double *>(s.list[0]) + lane * 8;
+#pragma unroll 1
                 for (int e = 0; e < 8; ++e) {
-                    x[e] = left(l[e], ql[e], m > 0);
-                    t += x[e];
+                    const float2 v = s.list[0][lane * 8 + e];
+                    double x = pw(v.x, root);
+                    if (factor > 0) x = fmax(x - factor * qw(v.y, root), 0.0);
+                    weight[e] = x;
+                    t += x;
                 }
                 double incl = t;
                 for (int o = 1; o < 32; o <<= 1) {
@@ -526,14 +609,15 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
                 }
                 double run = at + incl - t;
                 int hit = -1, seen = -1;
-#pragma unroll
+#pragma unroll 1
                 for (int e = 0; e < 8; ++e) {
-                    run += x[e];
-                    if (x[e] > 0) seen = e;
-                    if (hit < 0 && !end && x[e] > 0 && run > target) hit = e;
+                    const double x = weight[e];
+                    run += x;
+                    if (x > 0) seen = e;
+                    if (hit < 0 && !end && x > 0 && run > target) hit = e;
                 }
                 const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, seen >= 0);
-                if (lane == (hits ? __ffs(hits) - 1 : any ? 31 - __clz(any) : 0)) a.token[seq] = (int32_t)(place(first + found) + (hits ? hit : seen));
+                if (lane == (hits ? __ffs(hits) - 1 : any ? 31 - __clz(any) : 0)) a.token[seq] = place(first + found) + (hits ? hit : seen);
             }
             token = -2;  // written by its owner
             break;
@@ -599,12 +683,12 @@ extern "C" int zq_verify_draft(zq_ctx *ctx, const void *dev_logits, const void *
     a.path = dev_path;
     a.accepted = dev_accepted;
     a.token = dev_token;
-    a.vocab = (int64_t)vocab;
+    a.vocab = (int)vocab;
     a.rows = (int)rows;
     a.shared_parents = parents_shared;
     a.status = ctx->status_dev;
     const size_t segments = (vocab + 7 + kSegment - 1) / kSegment;  // a row may begin up to seven values behind a boundary
     a.segments = (int)((segments + cluster - 1) / cluster);
-    const size_t smem = a.segments * sizeof(double);
+    const size_t smem = 2 * a.segments * sizeof(double);
     return dtype == ZQ_F32 ? launch_verify<float>(ctx, a, cluster, batch, smem, err) : dtype == ZQ_F16 ? launch_verify<__half>(ctx, a, cluster, batch, smem, err) : launch_verify<__nv_bfloat16>(ctx, a, cluster, batch, smem, err);
 }
