@@ -192,6 +192,32 @@ def test_attention_of_unequal_lengths(rows, group):
     run_attention(gen_of(rows), 6, rows, 2 * group, 2, 128, 32, [2000, 3, 0, 77, 511, 1024], torch.bfloat16, True, drafted=drafted)
 
 
+@pytest.mark.parametrize("rows,group,dim,page", [(5, 5, 64, 4), (9, 7, 128, 2), (3, 8, 96, 4), (40, 2, 80, 1), (17, 1, 40, 32), (9, 4, 48, 8)])
+def test_attention_of_pages_and_heads_that_the_fast_kernel_does_not_take(rows, group, dim, page):
+    run_attention(gen_of(dim), 2, rows, 2 * group, 2, dim, page, [33, 500], torch.bfloat16, True)
+    run_attention(gen_of(dim + 1), 3, rows, 2 * group, 2, dim, page, [0, 1200, 7], torch.float16, False, drafted=[rows, 2, 0])
+
+
+@pytest.mark.parametrize("rows,group", [(1024, 1), (700, 3), (129, 2)])
+def test_attention_of_many_rows(rows, group):
+    run_attention(gen_of(rows), 1, rows, group, 1, 64, 16, [70], torch.float16, rows != 700)
+
+
+def test_attention_of_queries_that_lie_apart():
+    g = gen_of(13)
+    k_pages, v_pages, table = make_cache(g, 2, 2, 64, 16, 8, torch.float16)
+    for extra in (0, 2, 3, 8):  # rows of a fused projection; with 3 more values their distance is odd
+        fused = torch.randn((2, 6, 8 * 64 + extra), generator=g).half().cuda()
+        q = fused[..., :8 * 64].unflatten(-1, (8, 64))
+        got = ctx().tree_attention(q, k_pages, v_pages, table, ints(100, 17))
+        want = ctx().tree_attention(q.contiguous(), k_pages, v_pages, table, ints(100, 17))
+        ctx().sync()
+        assert torch.equal(got, want)
+    got = ctx().tree_attention(q.transpose(0, 1).contiguous().transpose(0, 1), k_pages, v_pages, table, ints(100, 17))
+    ctx().sync()
+    assert torch.equal(got, want)
+
+
 def test_attention_over_a_long_context():
     run_attention(gen_of(1), 1, 2, 4, 1, 128, 64, [40000], torch.bfloat16, True)
 
@@ -469,3 +495,184 @@ def test_paths_that_lead_nowhere_are_skipped_and_reported():
     with pytest.raises(ffi.ZqFailure):
         ctx().sync()
     assert torch.equal(k, want)
+
+
+# ---- streams, graphs, and all of it together
+def step_inputs(g, batch, rows, kv, group, dim, vocab, dtype, contexts):
+    blocks = -(-(max(contexts) + rows) // 16)
+    k_pages, v_pages, table = make_cache(g, batch, kv, dim, 16, blocks, dtype)
+    return dict(k_pages=k_pages, v_pages=v_pages, table=table, context=ints(*contexts), parents=R.trees(g, batch, rows).cuda(), drafted=ints(*[rows - (b % 2) for b in range(batch)]),
+                q=torch.randn((batch, rows, kv * group, dim), generator=g).to(dtype).cuda(), k=torch.randn((batch, rows, kv, dim), generator=g).to(dtype).cuda(), v=torch.randn((batch, rows, kv, dim), generator=g).to(dtype).cuda(),
+                freq=(10000.0 ** (-torch.arange(dim // 2) / (dim // 2))).float().cuda(), logits=(torch.randn((batch, rows, vocab), generator=g) * 2).to(dtype).cuda(),
+                tokens=torch.randint(0, vocab, (batch, rows), generator=g, dtype=torch.int32).cuda(), accept_u=(torch.rand((batch, rows), generator=g) * 0.05).cuda(), sample_u=torch.rand(batch, generator=g).cuda(),
+                heat=torch.ones(batch).cuda())
+
+
+def step(c, s):
+    positions, mask = c.draft_tree(s["parents"], s["context"], s["drafted"])
+    q = c.rope_append(s["q"], s["k"], s["v"], s["k_pages"], s["v_pages"], s["table"], s["context"], positions.reshape(-1), s["freq"], draft_lens=s["drafted"])
+    y = c.tree_attention(q, s["k_pages"], s["v_pages"], s["table"], s["context"], mask=mask, draft_lens=s["drafted"])
+    path, accepted, token = c.verify_draft(s["logits"], s["tokens"], s["parents"], s["accept_u"], s["sample_u"], s["heat"], draft_lens=s["drafted"])
+    c.cache_keep_path(s["k_pages"], s["v_pages"], s["table"], s["context"], path, accepted)
+    return q, y, path, accepted, token, s["k_pages"], s["v_pages"]
+
+
+SHAPES = [(1, 5, 2, 1, 64, 900), (3, 12, 2, 4, 128, 5000), (2, 70, 1, 8, 64, 300)]
+
+
+def check_step(s, batch, rows, kv, group, dim, vocab, dtype):
+    """Each operator against its 64-bit form on what the one before it left on the device; the rows that each sequence keeps."""
+    before_k, before_v = s["k_pages"].clone(), s["v_pages"].clone()
+    q, y, path, accepted, token, k_pages, v_pages = step(ctx(), s)
+    ctx().sync()
+    context, drafted, table = s["context"].cpu(), s["drafted"].cpu(), s["table"].cpu()
+    positions, sees = R.tree(s["parents"].cpu(), context, drafted)
+    turned = R.rotate(s["k"].reshape(-1, kv, dim).cpu(), positions.reshape(-1), s["freq"].cpu(), 1.0, False, False).reshape(batch, rows, kv, dim)
+    for b in range(batch):
+        for i in range(int(drafted[b])):
+            at = R.cache_row(table[b], 16, int(context[b]) + i)
+            before_k[at], before_v[at] = turned[b, i].to(dtype).cuda(), s["v"][b, i]
+    want, bound = R.attention(q, before_k, before_v, s["table"], s["context"], sees, drafted, 1 / math.sqrt(dim))
+    # a key of the cache may be rounded the other way than the plain form's: one step of a key's value, in every product
+    moved = 2 * R.half_step(dtype) * float(before_k.abs().max()) * float(q.abs().max()) * math.sqrt(dim) * float(before_v.abs().max()) * 2.0 ** -4
+    assert ((y.double() - want).abs() <= bound + moved).all()
+    result = R.verify(s["logits"].cpu(), None, s["tokens"].cpu(), s["parents"].cpu(), s["accept_u"].cpu(), s["sample_u"].cpu(), s["heat"].cpu(), drafted)
+    check_verify((path, accepted, token), result, rows)
+    for b, (kept, n, _) in enumerate(result):
+        for i in range(n):
+            src, dst = R.cache_row(table[b], 16, int(context[b]) + kept[i]), R.cache_row(table[b], 16, int(context[b]) + i)
+            before_k[dst], before_v[dst] = before_k[src].clone(), before_v[src].clone()
+    assert torch.equal(v_pages, before_v)
+    assert ((k_pages.double() - before_k.double()).abs() <= 2 * R.half_step(dtype) * before_k.double().abs() + 1e-6).all()
+    return [kept for kept, _, _ in result]
+
+
+@pytest.mark.parametrize("batch,rows,kv,group,dim,vocab", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_step_of_all_operators(batch, rows, kv, group, dim, vocab, dtype):
+    s = step_inputs(gen_of(rows), batch, rows, kv, group, dim, vocab, dtype, [200 + 37 * b for b in range(batch)])
+    check_step(s, batch, rows, kv, group, dim, vocab, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_step_that_keeps_rows(dtype):
+    """The last child of every row drafts its row's likeliest token, and is kept at temperature 0."""
+    batch, rows, kv, group, dim, vocab = 3, 20, 2, 4, 128, 700
+    s = step_inputs(gen_of(77), batch, rows, kv, group, dim, vocab, dtype, [90, 31, 0])
+    parents = s["parents"].clone()
+    for b in range(batch):
+        for i in range(rows):
+            child = (parents[b] == i).nonzero().flatten().tolist()
+            if child:
+                s["tokens"][b, child[-1]] = int((s["logits"][b, i] == s["logits"][b, i].max()).nonzero()[0])
+    s["heat"].zero_()
+    kept = check_step(s, batch, rows, kv, group, dim, vocab, dtype)
+    assert max(len(k) for k in kept) > 2 and any(k != list(range(len(k))) for k in kept)
+
+
+def test_a_captured_step_replays_and_two_graphs_run_at_once():
+    """Graphs captured on two streams, replayed at once and in turns with eager calls: each has scratch of its own."""
+    from zllm_b200.backend import B200Context
+
+    c = B200Context(0)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    made = [[step_inputs(gen_of(40 + i), *shape[:6], torch.float16, [3000 + 700 * b for b in range(shape[0])]) for shape in SHAPES[1:]] for i in range(2)]
+    torch.cuda.synchronize()
+    keep = ("k_pages", "v_pages")
+    first = [[{n: s[n].clone() for n in keep} for s in m] for m in made]
+
+    def restore(i):
+        for s, f in zip(made[i], first[i]):
+            for n in keep:
+                s[n].copy_(f[n])
+
+    want = []
+    for i in range(2):
+        c.set_stream(torch.cuda.current_stream().cuda_stream)
+        want.append([[t.clone() for t in step(c, s)] for s in made[i]])
+        c.sync()
+        restore(i)
+    graphs, outs = [], []
+    for i in range(2):
+        c.set_stream(streams[i].cuda_stream)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[i]):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=streams[i]):
+                outs.append([step(c, s) for s in made[i]])
+            graphs.append(g)
+    for _ in range(20):
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                restore(i)
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            for got, w in zip(outs[i], want[i]):
+                assert all(torch.equal(x, y) for x, y in zip(got, w))
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    restore(0)
+    again = [step(c, s) for s in made[0]]
+    c.sync()
+    assert all(torch.equal(x, y) for got, w in zip(again, want[0]) for x, y in zip(got, w))
+    torch.cuda.synchronize()
+    del graphs, outs
+
+
+def test_calls_on_two_streams_at_once():
+    from zllm_b200.backend import B200Context
+
+    c = B200Context(0)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    made = [step_inputs(gen_of(60 + i), 4, 20, 2, 4, 64, 2000, torch.bfloat16, [2000, 3000, 10, 0]) for i in range(2)]
+    torch.cuda.synchronize()
+    want = []
+    for s in made:
+        q, mask = s["q"], c.draft_tree(s["parents"], s["context"], s["drafted"])[1]
+        want.append(c.tree_attention(q, s["k_pages"], s["v_pages"], s["table"], s["context"], mask=mask, draft_lens=s["drafted"]))
+        c.sync()
+    for _ in range(30):
+        got = []
+        for i, s in enumerate(made):
+            c.set_stream(streams[i].cuda_stream)
+            with torch.cuda.stream(streams[i]):
+                mask = c.draft_tree(s["parents"], s["context"], s["drafted"])[1]
+                got.append(c.tree_attention(s["q"], s["k_pages"], s["v_pages"], s["table"], s["context"], mask=mask, draft_lens=s["drafted"]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    c.sync()
+
+
+def test_operators_between_projections_of_the_framework():
+    """Two tokens of a small layer: q, k and v from packed weights, rotated into the cache, attended to, and through the output projection."""
+    import numpy as np
+
+    from tests import helpers as H
+    from zllm_b200.backend import rope_frequencies
+
+    hidden, kv, dim, heads = 256, 2, 64, 4
+    w = {n: ctx().prepare_weight(H.Q8_0, H.random_weight(H.Q8_0, rows, hidden, seed=i), rows, hidden) for i, (n, rows) in enumerate((("q", heads * dim), ("k", kv * dim), ("v", kv * dim), ("o", hidden)))}
+    deq = {n: ctx().dequantize(v).double() for n, v in w.items()}
+    x = torch.from_numpy(np.random.default_rng(3).standard_normal((2, hidden)).astype(np.float32)).cuda().half()
+    k_pages, v_pages = torch.zeros((4, 16, kv, dim), dtype=torch.float16, device="cuda"), torch.zeros((4, 16, kv, dim), dtype=torch.float16, device="cuda")
+    table, freq = ints(2, 0).reshape(1, 2), rope_frequencies(dim, 10000.0, device="cuda")[0]
+    for position in range(2):
+        q, k, v = ctx().triple_linear(x[position:position + 1], w["q"], w["k"], w["v"])
+        q = ctx().rope_append(q.view(1, 1, heads, dim), k.view(1, 1, kv, dim), v.view(1, 1, kv, dim), k_pages, v_pages, table, ints(position), ints(position), freq)
+        y = ctx().linear(ctx().tree_attention(q, k_pages, v_pages, table, ints(position)).reshape(1, heads * dim), w["o"])
+    ctx().sync()
+    rows = x.double()
+    q, k, v = (rows @ deq[n].T for n in ("q", "k", "v"))
+    angle = torch.arange(2, device="cuda").double().reshape(-1, 1, 1) * freq.double()
+
+    def turn(t):
+        a, b = t[..., :dim // 2], t[..., dim // 2:]
+        return torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()], -1)
+
+    q, k, v = turn(q.view(2, heads, dim)), turn(k.view(2, kv, dim)), v.view(2, kv, dim)
+    p = torch.softmax(torch.einsum("hd,khd->hk", q[1], k.repeat_interleave(heads // kv, 1)) / 8, 1)
+    want = torch.einsum("hk,khd->hd", p, v.repeat_interleave(heads // kv, 1)).reshape(1, -1) @ deq["o"].T
+    # f16 rows between five steps, each product within 3e-4 of its largest value by its integer activations and 2^-11 by rounding
+    assert (y.double() - want).abs().max() <= 5 * (3e-4 + 2.0 ** -11) * 4 * want.abs().max()

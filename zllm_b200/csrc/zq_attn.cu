@@ -511,6 +511,7 @@ extern "C" int zq_tree_attention(zq_ctx *ctx, const void *dev_q, size_t q_heads,
     if (q_stride < q_heads * cache->head_dim || q_stride % 2 || q_stride > (size_t)INT32_MAX) return set_error(err, ZQ_ERR_SHAPE, "zq_tree_attention: rows of q %zu values apart for %zu values", q_stride, q_heads * cache->head_dim);
     if (!(scale > 0) || scale > 1e30f) return set_error(err, ZQ_ERR_ARG, "zq_tree_attention: scale %g (positive)", (double)scale);
     if ((reinterpret_cast<uintptr_t>(dev_q) | reinterpret_cast<uintptr_t>(dev_out)) & 3) return set_error(err, ZQ_ERR_ARG, "zq_tree_attention: q or the output is not 4-byte aligned");
+    if (reinterpret_cast<uintptr_t>(dev_mask) & 7) return set_error(err, ZQ_ERR_ARG, "zq_tree_attention: the mask is not 8-byte aligned");
     if ((uint64_t)cache->max_blocks * cache->page_size > (uint64_t)INT32_MAX - 4096) return set_error(err, ZQ_ERR_SHAPE, "zq_tree_attention: %zu blocks of %zu positions", cache->max_blocks, cache->page_size);
     if ((rc = use_device(ctx, err))) return rc;
     a.q = static_cast<const uint8_t *>(dev_q);

@@ -627,7 +627,12 @@ PyObject *py_tree_attention(PyObject *, PyObject *const *a, Py_ssize_t) {
     return guarded([&]() -> PyObject * {
         zq_ctx *ctx = ctx_of(a[0]);
         const int device = device_of(a[1]);
-        const Rows q = rows_3d(a[2], device, "query");
+        Rows q = rows_3d(a[2], device, "query");
+        if (q.stride % 8 || (reinterpret_cast<uintptr_t>(q.t.data_ptr()) & 15)) {  // the kernels read whole words, the fast one 16 bytes
+            NoGil g;
+            q.t = q.t.clone(at::MemoryFormat::Contiguous);
+            q.stride = q.heads * q.dim;
+        }
         const Cache cache = cache_of(a[3], a[4], a[5], a[6], device, false);
         const int64_t batch = (int64_t)cache.c.batch, rows = q.rows / batch;
         if (q.rows % batch || q.dim != (int64_t)cache.c.head_dim) fail(1, "tree_attention: query of shape " + sizes_of(q.t) + " for " + std::to_string(batch) + " sequences of a cache of " + sizes_of(cache.k));
