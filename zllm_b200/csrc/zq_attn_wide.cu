@@ -71,25 +71,6 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *m
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(head), "r"(row), "r"(page)
                  : "memory");
 }
-// 2^y of both halves on the FMA units, which have time where the exponential units have not: 2^n (n the nearest whole number) times a polynomial of degree 4
-// in the rest, fitted to the least relative error on [-1/2, 1/2] (2.7e-6, against 2^-12 of a weight's rounding).  y is at most about 8; below -126
-// it counts as -126.
-__device__ __forceinline__ void ex2_fma(uint64_t y, float &lo, float &hi) {
-    unpair64(y, lo, hi);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-126.f));
-    y = pair64(__float_as_uint(lo), __float_as_uint(hi));
-    const uint64_t t = add2(y, twice(12582912.f)), f = fma2(add2(t, twice(-12582912.f)), twice(-1.f), y);
-    uint64_t v = fma2(f, twice(0.0095701022f), twice(0.055917859f));
-    v = fma2(f, v, twice(0.24024744f));
-    v = fma2(f, v, twice(0.69312179f));
-    v = fma2(f, v, twice(0.99999928f));
-    float n_lo, n_hi;
-    unpair64(t, n_lo, n_hi);
-    unpair64(v, lo, hi);
-    lo = __uint_as_float(__float_as_uint(lo) + (__float_as_uint(n_lo) << 23));
-    hi = __uint_as_float(__float_as_uint(hi) + (__float_as_uint(n_hi) << 23));
-}
 // A tile of 128-byte swizzled rows, eight rows (1024 bytes) from one group to the next.  K-major (Q, K: a row is 64 values of the reduced
 // dimension): the leading offset is not used.  The other way round (V: a row is a key, the reduced dimension): the leading offset leads to the next 64 values.
 // sw128_low is the half that holds the address; one lane's value for the warp, so that the MMAs' operands are uniform registers.
@@ -394,13 +375,9 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                         for (int e = 0; e < 32; e += 2) {
                             const uint64_t y = fma2(pair64(z[e], z[e + 1]), scale2, off2);
                             float lo, hi;
-                            if ((e & 6) == 6) {
-                                ex2_fma(y, lo, hi);
-                            } else {
-                                unpair64(y, lo, hi);
-                                lo = ex2(lo);
-                                hi = ex2(hi);
-                            }
+                            unpair64(y, lo, hi);
+                            lo = ex2(lo);
+                            hi = ex2(hi);
                             sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair64(__float_as_uint(lo), __float_as_uint(hi)));
                             p[16 * c + (e >> 1)] = pack2<BF16>(lo, hi);
                         }
