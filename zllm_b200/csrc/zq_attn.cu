@@ -317,33 +317,45 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
         const bool whole = !a.split && ua == 0 && ub == units;
         float *part = a.split ? reinterpret_cast<float *>(smem + S::kPartAt) : a.parts + ((size_t)blockIdx.x * 2 + (ua == 0 ? 1 : 0)) * S::kPartFloats;  // in a cluster its own memory
         const int n_out = min(S::kRows, a.rows * a.group - tile * S::kRows) * (D / 2);  // pairs of columns of the tile's rows
-        for (int idx = tid; idx < n_out; idx += S::kThreads) {
-            const int r = idx / (D / 2), col = 2 * (idx % (D / 2)), row = tile * S::kRows + r, i = row / a.group;
-            float m = -INFINITY;
+        // a row's factors of the groups' sums, once, in place of their largest scores
+        for (int r = tid; r < S::kRows; r += S::kThreads) {
+            float m = -INFINITY, l = 0.f, f[S::kGroups];
 #pragma unroll
             for (int g = 0; g < S::kGroups; ++g) m = fmaxf(m, m_top[g * S::kRows + r]);
             const float b = m == -INFINITY ? 0.f : m;
-            float x = 0.f, y = 0.f, l = 0.f;
 #pragma unroll
             for (int g = 0; g < S::kGroups; ++g) {
-                const float w = exp2f(m_top[g * S::kRows + r] - b);
+                f[g] = exp2f(m_top[g * S::kRows + r] - b);
+                l += f[g] * m_sum[g * S::kRows + r];
+            }
+            const bool none = whole && (l == 0.f || (tile * S::kRows + r) / a.group >= len.rows);
+            const float by = !whole ? 1.f : none ? 0.f : 1.f / l;
+#pragma unroll
+            for (int g = 0; g < S::kGroups; ++g) m_top[g * S::kRows + r] = none ? -1.f : f[g] * by;
+            if (!whole && (tile * S::kRows + r) < a.rows * a.group) {
+                part[S::kRows * D + r] = m;
+                part[S::kRows * D + S::kRows + r] = l;
+            }
+        }
+        __syncthreads();
+#pragma unroll 2
+        for (int idx = tid; idx < n_out; idx += S::kThreads) {
+            const int r = idx / (D / 2), col = 2 * (idx % (D / 2));
+            float x = 0.f, y = 0.f;
+            bool none = false;
+#pragma unroll
+            for (int g = 0; g < S::kGroups; ++g) {
+                const float w = m_top[g * S::kRows + r];
                 const float2 v = *reinterpret_cast<const float2 *>(m_o + (g * S::kRows + r) * D + col);
+                none = w < 0.f;
                 x += w * v.x;
                 y += w * v.y;
-                l += w * m_sum[g * S::kRows + r];
             }
-            if (whole) {
-                if (i < a.rows && col < d) {
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    const bool none = l == 0.f || i >= len.rows;
-                    *reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col)) = none ? 0u : pack2<BF16>(x * inv, y * inv);
-                }
-            } else {
+            if (!whole) {
                 *reinterpret_cast<float2 *>(part + r * D + col) = make_float2(x, y);
-                if (col == 0) {
-                    part[S::kRows * D + r] = m;
-                    part[S::kRows * D + S::kRows + r] = l;
-                }
+            } else if (col < d) {
+                const int row = tile * S::kRows + r, i = row / a.group;
+                *reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row - i * a.group) * d + col)) = none ? 0u : pack2<BF16>(x, y);
             }
         }
         if (a.split) {
