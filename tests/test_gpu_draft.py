@@ -134,6 +134,43 @@ def test_rope_append_writes_the_cache_and_nothing_else(dtype, batch, rows, heads
     assert torch.equal(got_q, turned_q) and torch.equal(k_pages, want_k) and torch.equal(v_pages, want_v)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("interleaved,suffix", [(False, False), (True, True)])
+@pytest.mark.parametrize("heads,kv,dim,rotary", [(4, 1, 64, 64), (6, 3, 96, 32), (3, 1, 128, 128), (40, 8, 128, 128), (1, 1, 8, 8)])
+def test_many_rows_turn_as_few_do(dtype, interleaved, suffix, heads, kv, dim, rotary):
+    """Rows by the thousand get fewer threads each than rows by the hundred; same values, same sines, same order of operations."""
+    g = gen_of(heads + dim)
+    rows = 5000
+    q, k = torch.randn((rows, heads, dim), generator=g).to(dtype).cuda(), torch.randn((rows, kv, dim), generator=g).to(dtype).cuda()
+    positions = torch.randint(-1, 1 << 17, (rows,), generator=g, dtype=torch.int32).cuda()
+    freq = (10000.0 ** (-torch.arange(rotary // 2) / (rotary // 2))).float().cuda()
+    got_q, got_k = ctx().rope_rows(q, k, positions, freq, interleaved=interleaved, suffix=suffix, factor=1.1)
+    parts = [ctx().rope_rows(q[i:i + 500], k[i:i + 500], positions[i:i + 500], freq, interleaved=interleaved, suffix=suffix, factor=1.1) for i in range(0, rows, 500)]
+    ctx().sync()
+    assert torch.equal(got_q, torch.cat([p[0] for p in parts])) and torch.equal(got_k, torch.cat([p[1] for p in parts]))
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (5, 5, 40)])
+def test_many_rows_are_appended_as_few_are(heads, kv, dim):
+    g = gen_of(dim)
+    batch, rows, page = 13, 150, 16
+    k_pages, v_pages, table = make_cache(g, batch, kv, dim, page, 14, torch.bfloat16)
+    table[3, 2] = 10 ** 6  # a page that is none
+    q, k, v = (torch.randn((batch, rows, h, dim), generator=g).bfloat16().cuda() for h in (heads, kv, kv))
+    context = torch.randint(0, 70, (batch,), generator=g, dtype=torch.int32).cuda()
+    drafted = torch.randint(0, rows + 1, (batch,), generator=g, dtype=torch.int32).cuda()
+    positions = torch.randint(-1, 9000, (batch * rows,), generator=g, dtype=torch.int32).cuda()
+    freq = (10000.0 ** (-torch.arange(dim // 2) / (dim // 2))).float().cuda()
+    want_k, want_v = k_pages.clone(), v_pages.clone()
+    got_q = ctx().rope_append(q, k, v, k_pages, v_pages, table, context, positions, freq, draft_lens=drafted)
+    want_q = [ctx().rope_append(q[b:b + 1], k[b:b + 1], v[b:b + 1], want_k, want_v, table[b:b + 1], context[b:b + 1], positions[b * rows:(b + 1) * rows], freq, draft_lens=drafted[b:b + 1]) for b in range(batch)]
+    from zllm_b200 import ffi
+
+    with pytest.raises(ffi.ZqFailure):
+        ctx().sync()
+    assert torch.equal(got_q, torch.cat(want_q)) and torch.equal(k_pages, want_k) and torch.equal(v_pages, want_v)
+
+
 def test_rope_append_skips_rows_without_a_page():
     from zllm_b200 import ffi
 

@@ -110,12 +110,7 @@ template <class T, int VEC> __global__ void __launch_bounds__(256, 4) rope_rows_
     }
     __syncthreads();
     if (!here) return;
-    float2 sines[VEC];
     const bool turns = pair >= 0 && position >= 0;
-    if (turns) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sines[j] = turn[j * pairs + c];
-    }
     T *q_out = reinterpret_cast<T *>(a.q_out) + row * a.q_heads * a.head_dim, *k_out = a.cache.k ? reinterpret_cast<T *>(a.cache.k) + keep : reinterpret_cast<T *>(a.k_out) + row * a.k_heads * a.head_dim,
       *v_out = reinterpret_cast<T *>(a.cache.v) + keep;
     auto finish = [&](int h, V x, V y) {
@@ -128,7 +123,7 @@ template <class T, int VEC> __global__ void __launch_bounds__(256, 4) rope_rows_
                 memcpy(yw, &y, sizeof(y));
 #pragma unroll
                 for (int j = 0; j < VEC; j += 2) {
-                    const float2 a0 = sines[j], a1 = sines[j + 1];
+                    const float2 a0 = turn[j * pairs + c], a1 = turn[(j + 1) * pairs + c];
                     if (a.interleaved) {  // words 0..VEC/2 are x's pairs, the others y's
                         uint32_t &w0 = j < VEC / 2 ? xw[j] : yw[j - VEC / 2], &w1 = j < VEC / 2 ? xw[j + 1] : yw[j + 1 - VEC / 2];
                         const float2 s = two_f32<T>(w0), t = two_f32<T>(w1);
@@ -148,8 +143,8 @@ template <class T, int VEC> __global__ void __launch_bounds__(256, 4) rope_rows_
                     const bool beside = a.interleaved && VEC > 1;
                     T &r = beside ? (2 * j < VEC ? x : y).v[2 * j % VEC] : x.v[j], &i = beside ? (2 * j < VEC ? x : y).v[(2 * j + 1) % VEC] : y.v[j];
                     const float re = to_f32(r), im = to_f32(i);
-                    r = from_f32<T>(re * sines[j].x - im * sines[j].y);
-                    i = from_f32<T>(im * sines[j].x + re * sines[j].y);
+                    r = from_f32<T>(re * turn[j * pairs + c].x - im * turn[j * pairs + c].y);
+                    i = from_f32<T>(im * turn[j * pairs + c].x + re * turn[j * pairs + c].y);
                 }
             }
         }
