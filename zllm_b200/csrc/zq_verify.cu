@@ -258,17 +258,19 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             float top = -INFINITY;
             double sum = 0;
             if (!greedy) {
-                float l[8];
-                load(r, w, first + warp < last ? first + warp : kNowhere, l);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, l[e]);
-                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                uint64_t sums[2] = {0, 0};
-                const uint64_t base2 = twice(-top);
+                uint64_t sums[2] = {0, 0}, base2 = 0;
                 for (int g = first + warp; g < last; g += kAhead * kVerifyWarps) {
                     Eight<T> x[kAhead];
+                    float l[8];
 #pragma unroll
                     for (int k = 0; k < kAhead; ++k) x[k].load(r, place(g + k * kVerifyWarps < last ? g + k * kVerifyWarps : kNowhere), a.vocab, w);
+                    if (g == first + warp) {
+                        x[0].get(l);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, l[e]);
+                        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        base2 = twice(-top);
+                    }
 #pragma unroll
                     for (int k = 0; k < kAhead; ++k) {
                         x[k].get(l);
@@ -348,6 +350,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
                 s_seg[a.segments + g - first] = 0;
             }
             mine += t;
+            __syncwarp();
         }
         if (lane == 0) s.warp_sums[0][warp] = mine;
         exchange_sums(s, parity ^= 1, 1);
