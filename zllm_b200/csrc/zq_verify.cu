@@ -109,14 +109,16 @@ __device__ __forceinline__ double warp_sum(double x) {
 struct Weights {
     double c, top;
     float low, c_hi, c_lo, top32, least;
-    __device__ void set(double scale, float largest) {
+    __device__ void scale_by(double scale) {
         c = scale;
-        top = (double)largest;
-        low = fmaxf((float)(top - 900.0 / c), -3.4028235e38f);
-        top32 = largest;
         c_hi = (float)fmin(scale, 1e30);
         c_lo = (float)(fmin(scale, 1e30) - (double)c_hi);
         least = fmaxf(-200.f / c_hi, -3.4028235e38f);
+    }
+    __device__ void relative_to(float largest, double gap) {  // gap: 900 / c
+        top = (double)largest;
+        low = fmaxf((float)(top - gap), -3.4028235e38f);
+        top32 = largest;
     }
     __device__ __forceinline__ bool heavy(float l) const { return (l - top32) * c_hi > kHeavy; }
     __device__ __forceinline__ float light(float l) const {
@@ -161,10 +163,10 @@ __device__ __forceinline__ int list_heavy(float2 *list, const float (&l)[8], con
     return total;
 }
 
-// Joins (largest, place, sum) of the lanes of a warp; a NaN stays.
-__device__ __noinline__ RowPart join_lanes(RowPart p, float scale32) {
+// Joins (largest, place, sum) of the lanes of each half of a warp; a NaN stays.
+__device__ __noinline__ RowPart join_halves(RowPart p, float scale32) {
     RowPart m = p;
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = 8; o > 0; o >>= 1) {
         const float top = __shfl_xor_sync(0xffffffffu, m.top, o);
         const int32_t at = __shfl_xor_sync(0xffffffffu, m.at, o);
         if (isnan(top) || top > m.top || (top == m.top && at < m.at)) {
@@ -172,17 +174,19 @@ __device__ __noinline__ RowPart join_lanes(RowPart p, float scale32) {
             m.at = at;
         }
     }
-    m.sum = warp_sum(p.top == -INFINITY ? 0.0 : p.sum * (double)exp2f((p.top - m.top) * scale32));
+    m.sum = p.top == -INFINITY ? 0.0 : p.sum * (double)exp2f((p.top - m.top) * scale32);
+    for (int o = 8; o > 0; o >>= 1) m.sum += __shfl_xor_sync(0xffffffffu, m.sum, o);
     return m;
 }
-// Every CTA gets every CTA's part: the warps' parts are joined by a warp each, which stores the result into all CTAs.
+// Every CTA gets every CTA's part of both rows: half a warp joins the warps' parts of a row and stores the result into all CTAs.
 __device__ __noinline__ void exchange_rows(VerifyShared &s, int parity, bool both, float scale32) {
     cg::cluster_group cluster = cg::this_cluster();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int which = threadIdx.x >> 4, i = threadIdx.x & 15;
+    static_assert(kVerifyWarps <= 16 && kMaxCluster <= 16, "half a warp");
     __syncthreads();
-    if (warp < (both ? 2 : 1)) {
-        const RowPart p = join_lanes(lane < kVerifyWarps ? s.warp_part[warp][lane] : RowPart{-INFINITY, 0x7fffffff, 0.0}, scale32);
-        if (lane < (int)cluster.num_blocks()) cluster.map_shared_rank(&s, lane)->part[parity][warp][cluster.block_rank()] = p;
+    if (threadIdx.x < 32) {
+        const RowPart p = join_halves(i < kVerifyWarps && (both || !which) ? s.warp_part[which][i] : RowPart{-INFINITY, 0x7fffffff, 0.0}, scale32);
+        if (i < (int)cluster.num_blocks()) cluster.map_shared_rank(&s, i)->part[parity][which][cluster.block_rank()] = p;
     }
     cluster.sync();
 }
@@ -228,16 +232,32 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
     int shift = 0;
     bool q_wide = false;
     Weights pw, qw;
+    const double gap = 900.0 / scale;
+    pw.scale_by(scale);
+    qw.scale_by(scale);
     double p_inv = 0, q_inv = 0;  // 1 / sum of weights
     int n_gone = 0;
 
-    // Largest logit, its place and 1 / sum of a row from all CTAs' parts.
-    auto joined = [&](int which, Weights &w, double &inv, int32_t &at) {
-        const RowPart p = join_lanes(lane < ctas ? s.part[parity][which][lane] : RowPart{-INFINITY, 0x7fffffff, 0.0}, scale32);
-        at = p.at;
-        inv = 1.0 / p.sum;
-        w.set(scale, p.top);
-        return isfinite(p.top);
+    // Largest logit, its place and 1 / sum of the rows from all CTAs' parts; false where one is no distribution.
+    auto joined = [&](bool both, int32_t &at) {
+        const int i = lane & 15;
+        const RowPart p = join_halves(i < ctas ? s.part[parity][lane >> 4][i] : RowPart{-INFINITY, 0x7fffffff, 0.0}, scale32);
+        const double inv = 1.0 / p.sum;
+        const float p_top = __shfl_sync(0xffffffffu, p.top, 0), q_top = __shfl_sync(0xffffffffu, p.top, 16);
+        at = __shfl_sync(0xffffffffu, p.at, 0);
+        p_inv = __shfl_sync(0xffffffffu, inv, 0);
+        q_inv = __shfl_sync(0xffffffffu, inv, 16);
+        pw.relative_to(p_top, gap);
+        if (both) qw.relative_to(q_top, gap);
+        return isfinite(p_top) && (!both || isfinite(q_top));
+    };
+    // The next row from `from` on that hangs below the walk's row, -1 where there is none.
+    auto child_from = [&](int from) {
+        for (int j0 = from; j0 < n; j0 += 32) {
+            const unsigned hits = __ballot_sync(0xffffffffu, j0 + lane < n && s.parent[j0 + lane] == node);
+            if (hits) return j0 + __ffs(hits) - 1;
+        }
+        return -1;
     };
     auto total_of = [&](int which) { return warp_sum(lane < ctas ? s.sums[parity][which][lane] : 0.0); };
     auto place = [&](int g) { return g * kSegment + lane * 8 - shift; };
@@ -250,50 +270,70 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
     // a thread.  They are relative to the largest logit of the warp's first segment; where that is none, or is so far from the others that the sum leaves f32's
     // range, and where the place is asked for, the warp takes its run with a running maximum.  A NaN makes that sum one.
     const uint64_t scale2 = twice(scale32);
+    auto weigh = [&](const Eight<T> &x, uint64_t base2, uint64_t (&sums)[2]) {
+        float l[8];
+        x.get(l);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            float lo, hi;
+            unpair64(mul2(add2(pair64(__float_as_uint(l[e]), __float_as_uint(l[e + 1])), base2), scale2), lo, hi);
+            sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair64(__float_as_uint(ex2(lo)), __float_as_uint(ex2(hi))));
+        }
+    };
+    auto most_of = [&](const Eight<T> &x) {
+        float l[8], m;
+        x.get(l);
+        m = l[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) m = fmaxf(m, l[e]);
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        return m;
+    };
     auto scan = [&](bool both) {
-#pragma unroll 1
-        for (int which = 0; which < (both ? 2 : 1); ++which) {
-            const T *r = which ? qrow : row;
-            const bool w = which ? q_wide : true;
-            float top = -INFINITY;
-            double sum = 0;
-            if (!greedy) {
-                uint64_t sums[2] = {0, 0}, base2 = 0;
-                for (int g = first + warp; g < last; g += kAhead * kVerifyWarps) {
-                    Eight<T> x[kAhead];
-                    float l[8];
+        float top[2] = {-INFINITY, -INFINITY};
+        double sum[2] = {0, 0};
+        if (!greedy) {
+            uint64_t ps[2] = {0, 0}, qs[2] = {0, 0}, p_base = 0, q_base = 0;
+            for (int g = first + warp; g < last; g += kAhead * kVerifyWarps) {
+                Eight<T> x[kAhead], y[kAhead];
 #pragma unroll
-                    for (int k = 0; k < kAhead; ++k) x[k].load(r, place(g + k * kVerifyWarps < last ? g + k * kVerifyWarps : kNowhere), a.vocab, w);
-                    if (g == first + warp) {
-                        x[0].get(l);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) top = fmaxf(top, l[e]);
-                        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        base2 = twice(-top);
-                    }
-#pragma unroll
-                    for (int k = 0; k < kAhead; ++k) {
-                        x[k].get(l);
-#pragma unroll
-                        for (int e = 0; e < 8; e += 2) {
-                            float lo, hi;
-                            unpair64(mul2(add2(pair64(__float_as_uint(l[e]), __float_as_uint(l[e + 1])), base2), scale2), lo, hi);
-                            sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair64(__float_as_uint(ex2(lo)), __float_as_uint(ex2(hi))));
-                        }
+                for (int k = 0; k < kAhead; ++k) {
+                    const int v = place(g + k * kVerifyWarps < last ? g + k * kVerifyWarps : kNowhere);
+                    x[k].load(row, v, a.vocab, true);
+                    if (both) y[k].load(qrow, v, a.vocab, q_wide);
+                }
+                if (g == first + warp) {
+                    top[0] = most_of(x[0]);
+                    p_base = twice(-top[0]);
+                    if (both) {
+                        top[1] = most_of(y[0]);
+                        q_base = twice(-top[1]);
                     }
                 }
-                float lo, hi;
-                unpair64(add2(sums[0], sums[1]), lo, hi);
-                sum = warp_sum((double)(lo + hi));
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    weigh(x[k], p_base, ps);
+                    if (both) weigh(y[k], q_base, qs);
+                }
             }
-            RowPart p{top, 0x7fffffff, sum};
-            if (!(isfinite(top) && sum >= 0.5 && sum < 1e30)) {
+            float lo, hi;
+            unpair64(add2(ps[0], ps[1]), lo, hi);
+            sum[0] = warp_sum((double)(lo + hi));
+            unpair64(add2(qs[0], qs[1]), lo, hi);
+            if (both) sum[1] = warp_sum((double)(lo + hi));
+        }
+#pragma unroll 1
+        for (int which = 0; which < (both ? 2 : 1); ++which) {
+            const float t = which ? top[1] : top[0];
+            const double all = which ? sum[1] : sum[0];
+            RowPart p{t, 0x7fffffff, all};  // of a warp without tokens: no logit, no sum
+            if (!(isfinite(t) && all >= 0.5 && all < 1e30) && (first + warp) * kSegment - shift < a.vocab) {
                 float run = -INFINITY, some = 0.f;
                 int32_t at = 0x7fffffff;
 #pragma unroll 1
                 for (int g = first + warp; g < last; g += kVerifyWarps) {
                     float l[8];
-                    load(r, w, g, l);
+                    load(which ? qrow : row, which ? q_wide : true, g, l);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         if (l[e] > run) {
@@ -304,7 +344,15 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
                         some += ex2((l[e] - (run == -INFINITY ? 0.f : run)) * scale32);
                     }
                 }
-                p = join_lanes({isnan(some) ? NAN : run, at, (double)some}, scale32);
+                p = join_halves({isnan(some) ? NAN : run, at, (double)some}, scale32);
+                // the two halves
+                const float other = __shfl_xor_sync(0xffffffffu, p.top, 16);
+                const int32_t other_at = __shfl_xor_sync(0xffffffffu, p.at, 16);
+                const double other_sum = __shfl_xor_sync(0xffffffffu, p.sum, 16);
+                const float larger = isnan(p.top) || isnan(other) ? NAN : fmaxf(p.top, other);
+                p.sum = (p.top == -INFINITY ? 0.0 : p.sum * (double)exp2f((p.top - larger) * scale32)) + (other == -INFINITY ? 0.0 : other_sum * (double)exp2f((other - larger) * scale32));
+                if (other > p.top || (other == p.top && other_at < p.at)) p.at = other_at;
+                p.top = larger;
             }
             if (lane == 0) s.warp_part[which][warp] = p;
         }
@@ -340,9 +388,10 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             }
             const int total = list_heavy(s.list[warp], l, l, heavies);
             double t = (double)some;
+#pragma unroll 4
             for (int i = lane; i - lane < total; i += 32) {
                 const double w = pw(s.list[warp][min(i, total - 1)].x, root);
-                if (i < total) t += w;
+                t += i < total ? w : 0.0;
             }
             t = warp_sum(t);
             if (lane == 0) {
@@ -383,18 +432,17 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             all[1] += (double)some[1];
             all[2] += (double)some[2];
             all[3] += (double)some[3];
+#pragma unroll 2
             for (int i = lane; i - lane < total; i += 32) {
                 const float2 x = s.list[warp][min(i, total - 1)];
-                const double p = pw(x.x, root), q = qw(x.y, root);
-                if (i < total) {
-                    const double r0 = p - c0 * q, r1 = p - c1 * q;
-                    all[0] += p;
-                    all[1] += q;
-                    all[2] += fmax(r0, 0.0);
-                    all[3] += r0 > 0 ? q : 0.0;
-                    left += fmax(r1, 0.0);
-                    slope += r1 > 0 ? q : 0.0;
-                }
+                const bool in = i < total;
+                const double p = pw(x.x, root), q = qw(x.y, root), wp = in ? p : 0.0, wq = in ? q : 0.0, r0 = wp - c0 * wq, r1 = wp - c1 * wq;
+                all[0] += wp;
+                all[1] += wq;
+                all[2] += fmax(r0, 0.0);
+                all[3] += r0 > 0 ? wq : 0.0;
+                left += fmax(r1, 0.0);
+                slope += r1 > 0 ? wq : 0.0;
             }
             all[4] += left;
             all[5] += slope;
@@ -447,18 +495,23 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             row = reinterpret_cast<const T *>(a.logits) + (row0 + node) * a.vocab;
             shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
             n_gone = 0;
-            bool child = false;
-            for (int j = node + 1; j < n && !child; ++j) child = s.parent[j] == node;
-            const bool use_q = drawn && child;
+            const int child = child_from(node + 1);
+            const bool use_q = drawn && child >= 0;
             if (use_q) {
                 qrow = reinterpret_cast<const T *>(a.draft) + (row0 + node) * a.vocab;
                 q_wide = ((reinterpret_cast<uintptr_t>(qrow) ^ reinterpret_cast<uintptr_t>(row)) & 15) == 0;
             }
+            if (child >= 0 && !greedy) {  // the first child's logits come while the rows are summed
+                const int t = s.token[child];
+                if (t >= 0 && t < a.vocab) {
+                    asm volatile("prefetch.global.L1 [%0];" ::"l"(row + t));
+                    if (use_q) asm volatile("prefetch.global.L1 [%0];" ::"l"(qrow + t));
+                }
+            }
             scan(use_q);
             exchange_rows(s, parity ^= 1, use_q, scale32);
-            int32_t best, unused;
-            bad = !joined(0, pw, p_inv, best);
-            if (use_q) bad |= !joined(1, qw, q_inv, unused);
+            int32_t best;
+            bad = !joined(use_q, best);
             if (bad) break;
 
             // ---- its children
@@ -466,8 +519,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             int rejected = 0;         // drawn children that left something: p is (p - m q)+ / rest
             double m = 0, rest = 1;
             double gone = 0;          // what the rejected chosen children had of p
-            for (int j = node + 1; j < n; ++j) {
-                if (s.parent[j] != node) continue;
+            for (int j = child; j >= 0; j = child_from(j + 1)) {
                 const int t = s.token[j];
                 if (t < 0 || t >= a.vocab) {
                     if (tid == 0 && rank == 0) atomicMax(a.status, (uint32_t)kStatusBadIndex);
@@ -497,7 +549,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
                 } else {
                     bool again = false;
                     for (int i = 0; i < n_gone; ++i) again |= s.gone[i] == t;
-                    if (!again && u < p / (1.0 - gone)) {
+                    if (!again && u * (1.0 - gone) < p) {
                         next = j;
                         break;
                     }
@@ -548,24 +600,19 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
                 factor = off = 0;
                 sum_at = 0;
             }
-            auto part_of = [&](int cta) { return sum_at ? fmax(s.sums[parity][4][cta] - off * s.sums[parity][5][cta], 0.0) : s.sums[parity][0][cta]; };
-            double total = 0, before = 0, upto = 0;
-            int owner = -1, some = 0;
-            for (int i = 0; i < ctas; ++i) total += part_of(i);
-            const double target = (double)a.sample_u[seq] * total;
-            for (int i = 0; i < ctas; ++i) {
-                const double part = part_of(i);
-                if (part > 0) some = i;
-                if (owner < 0 && upto + part > target) {
-                    owner = i;
-                    before = upto;
-                }
-                upto += part;
+            // a lane has a CTA's part; before: of the CTAs in front
+            double part = 0;
+            if (lane < ctas) part = sum_at ? fmax(s.sums[parity][4][lane] - off * s.sums[parity][5][lane], 0.0) : s.sums[parity][0][lane];
+            double upto = part;
+            for (int o = 1; o < 16; o <<= 1) {
+                const double up = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += up;
             }
-            if (owner < 0) {  // the target is the total, to rounding
-                owner = some;
-                before = upto - part_of(some);
-            }
+            const double target = (double)a.sample_u[seq] * __shfl_sync(0xffffffffu, upto, ctas - 1);
+            const unsigned over_here = __ballot_sync(0xffffffffu, lane < ctas && part > 0 && upto > target), some = __ballot_sync(0xffffffffu, part > 0);
+            // where none is over, the target is the total, to rounding
+            const int owner = over_here ? __ffs(over_here) - 1 : some ? 31 - __clz(some) : 0;
+            const double before = __shfl_sync(0xffffffffu, upto - part, owner);
             if (owner == rank && warp == 0) {
                 // the segment, 32 at a time
                 double at = before;
@@ -597,7 +644,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s.list[0][lane * 8 + e] = make_float2(l[e], factor > 0 ? ql[e] : 0.f);
                 double t = 0, *weight = reinterpret_cast<double *>(s.list[0]) + lane * 8;
-#pragma unroll 1
+#pragma unroll 4
                 for (int e = 0; e < 8; ++e) {
                     const float2 v = s.list[0][lane * 8 + e];
                     double x = pw(v.x, root);
