@@ -3,11 +3,11 @@
 //     out_i = sum_j w_ij v_j / sum_j w_ij,   w_ij = exp(scale q_i k_j - top_i)
 //
 // One pass over the keys with a running maximum and sum per row (the sums so far are multiplied down when the maximum rises).  The rows of
-// all query heads that share a head of the cache go through the matrix instructions together (m16n8k16), so that the cache is read once for them: bytes
-// bound while rows * group stays below about 100.
+// all query heads that share a head of the cache go through the matrix instructions together (m16n8k16), so that the cache is read once for them. For up to
+// 32 rows per cache head; above, zq_attn_wide.cu takes over where its layout allows. One row each of 64 sequences at 16384 positions streams the cache at 6.6 TB/s.
 //
-// Work: an item is a (sequence, cache head, tile of rows); its keys are cut into units.  The units of all items, in one line, are
-// dealt to the CTAs (one per SM) in equal shares, so that one long sequence or many unequal ones keep all SMs at work; an item cut by a border is
+// Work: an item is a (sequence, cache head, tile of rows); its keys are cut into units.  The units of all items, in one line, with a few
+// places behind each item for what its end costs, are dealt to the CTAs (one per SM) in equal shares, so that one long sequence or many unequal ones keep all SMs at work; an item cut by a border is
 // left in parts (largest score, sum of weights and weighted sums per row, f32) which a second, small kernel joins in ascending order:
 // results do not depend on timing.  The lengths are on the device, so each CTA finds its share from them itself.
 //
@@ -44,6 +44,9 @@ template <bool BF16> __device__ __forceinline__ void mma16(float (&d)[4], const 
         mma_16816(d, a[0], a[1], a[2], a[3], b0, b1);
 }
 constexpr int kMaxSplit = 8;  // CTAs of an item in a cluster
+// What the end of an item costs, in units.  A decode step of 8 rows per cache head of 128, 4 cache heads, takes 26.0 / 42.2 / 74.8 / 68.4 us for 64 unequal sequences of up to
+// 200 and 1000, 150 of 900 and 40 of 5000 positions without it, 25.8 / 39.1 / 69.8 / 65.4 with 1, 22.8 / 36.3 / 62.4 / 62.4 with 3, 22.8 / 37.7 / 65.3 / 64.2 with 6.
+constexpr int kItemEnd = 3;
 
 // Shape of the kernel for a head of up to D values and WM warps of 16 rows.
 template <int D, int WM> struct AttnShape {
@@ -79,9 +82,10 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
         share.first = item * n + rank * n / a.split;
         share.last = item * n + (rank + 1) * n / a.split;
         share.total = 0;
+        share.extra = 0;
         share.ctas = 0;
     } else {
-        share = find_share<S::kThreads>(a, S::kUnit, smem + S::kSmem - 1024);
+        share = find_share<S::kThreads>(a, S::kUnit, kItemEnd, smem + S::kSmem - 1024);
         if (tid == 0) a.info[blockIdx.x] = make_int4(0, 0, 0, 0);
         if (share.first >= share.last) return;
     }
@@ -94,15 +98,19 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
     int units = units_of(len, S::kUnit);
 
     for (int64_t u = share.first; u < share.last || a.split;) {  // in a cluster once, with no units too
-        while (!a.split && u >= seq_first + (int64_t)units * a.c.heads * a.tiles) {
-            seq_first += (int64_t)units * a.c.heads * a.tiles;
+        while (!a.split && u >= seq_first + (int64_t)(units + share.extra) * a.c.heads * a.tiles) {
+            seq_first += (int64_t)(units + share.extra) * a.c.heads * a.tiles;
             len = seq_len(a, ++seq);
             units = units_of(len, S::kUnit);
         }
-        const int item = a.split ? (int)(blockIdx.x / a.split) % (a.c.heads * a.tiles) : (int)((u - seq_first) / units);
-        const int64_t item_first = seq_first + (int64_t)item * units;
+        const int item = a.split ? (int)(blockIdx.x / a.split) % (a.c.heads * a.tiles) : (int)((u - seq_first) / (units + share.extra));
+        const int64_t item_first = seq_first + (int64_t)item * (units + share.extra);
         const int head = item / a.tiles, tile = item % a.tiles;
         const int ua = (int)(u - item_first), ub = (int)min((int64_t)units, share.last - item_first);
+        if (!a.split && ua >= units) {  // behind its units
+            u = item_first + units + share.extra;
+            continue;
+        }
         const int steps = ub - ua, keys = len.rows ? len.context + len.rows : 0;
         const int row0 = tile * S::kRows + wm * 16, n_rows = len.rows * a.group;
 
@@ -397,7 +405,7 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
             a.info[blockIdx.x] = make_int4(seq, item, last - (int)blockIdx.x + 1, len.rows);
         }
         __syncthreads();
-        u = item_first + ub;
+        u = item_first + units + share.extra;
     }
 }
 

@@ -76,18 +76,20 @@ template <bool BF16> __device__ __forceinline__ bool drop_nonfinite(uint32_t &w)
     return lo || hi;
 }
 struct Share {
-    int64_t first, last, total;  // units of this CTA; of all
+    int64_t first, last, total;  // places of this CTA; of all
+    int extra;                   // places of an item behind its units'
     int ctas;                    // with a share
-    int seq;                     // of the first unit
-    int64_t seq_first;           // first unit of that sequence
+    int seq;                     // of the first place
+    int64_t seq_first;           // first place of that sequence
 };
 
 __device__ __forceinline__ int units_of(const SeqLen &s, int unit) {
     return s.rows ? (s.context + s.rows + unit - 1) / unit : 1;  // a sequence without rows has its output set to zero by its one unit
 }
 
-// The CTA's share of the units.  Every thread adds up some sequences, the thread whose sequences hold the first unit looks for it.
-template <int kThreads> __device__ Share find_share(const AttnArgs &a, int unit, uint8_t *scratch) {
+// The CTA's share of the places in line: those of an item's units, and `extra` behind them for what the end of an item costs (a CTA that walks
+// from one item into the next has that much less to read).  Every thread adds up some sequences, the thread whose sequences hold the first place looks for it.
+template <int kThreads> __device__ Share find_share(const AttnArgs &a, int unit, int extra, uint8_t *scratch) {
     int64_t *s_sum = reinterpret_cast<int64_t *>(scratch);  // [kThreads / 32 + 3]
     const int tid = threadIdx.x, lane = tid & 31, per = (a.batch + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
@@ -106,9 +108,13 @@ template <int kThreads> __device__ Share find_share(const AttnArgs &a, int unit,
         if (w < tid / 32) before += s_sum[w];
         total += s_sum[w];
     }
-    int64_t at = before + incl - mine;
+    if (total <= (int64_t)gridDim.x) extra = 0;  // a unit each: nobody walks on
+    total += a.batch * items * extra;
+    mine += (b1 - b0) * items * extra;
+    int64_t at = before + incl + b1 * items * extra - mine;
     Share s;
     s.total = total;
+    s.extra = extra;
     s.ctas = (int)min((int64_t)gridDim.x, total);
     const int64_t c = blockIdx.x;
     s.first = c < s.ctas ? c * total / s.ctas : total;
@@ -116,7 +122,7 @@ template <int kThreads> __device__ Share find_share(const AttnArgs &a, int unit,
     int64_t *s_found = s_sum + kThreads / 32;
     if (s.first >= at && s.first < at + mine) {
         for (int b = b0; b < b1; ++b) {
-            const int64_t n = units_of(seq_len(a, b), unit) * items;
+            const int64_t n = (units_of(seq_len(a, b), unit) + extra) * items;
             if (s.first < at + n) {
                 s_found[0] = b;
                 s_found[1] = at;

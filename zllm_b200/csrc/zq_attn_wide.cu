@@ -25,6 +25,10 @@
 namespace zq {
 
 constexpr int kWideThreads = 320, kWideTile = 128;
+// What the end of an item and the start of the next cost, in tiles of keys: 15 000 cycles, in which the ring stands still (the sums out of tensor memory, the rows
+// of Q, the first scores with nothing beside them).  40 rows per cache head of 128, 4 cache heads: 64 unequal sequences of up to 200 and 1000, 150 of 900 and 16 of 8000
+// positions take 42.7 / 63.9 / 114 / 53.5 us without it, 36.3 / 53.8 / 94 / 51.8 with 3, 32.2 / 48.4 / 85 / 49.0 with 7, 32.1 / 49.0 / 85 / 49.7 with 12.
+constexpr int kWideEnd = 7;
 
 __device__ __forceinline__ bool wide_elect() {
     uint32_t r;
@@ -135,7 +139,7 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
         if (base & 1023) atomicMax(a.status, (uint32_t)kStatusTmaTimeout);  // swizzled tiles begin at multiples of 1024 bytes
     }
     if (base & 1023) return;
-    const Share share = find_share<kWideThreads>(a, kWideTile, smem);
+    const Share share = find_share<kWideThreads>(a, kWideTile, kWideEnd, smem);
     if (share.first >= share.last) return;
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)), "r"(512) : "memory");
@@ -167,20 +171,22 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
     int units = units_of(len, kWideTile), head = 0, tile = 0, ua = 0, ub = 0, item = 0, keys = 0;
     int64_t item_first = 0;
     auto next_item = [&]() {
-        if (u >= share.last) return false;
-        while (u >= seq_first + (int64_t)units * a.c.heads * a.tiles) {
-            seq_first += (int64_t)units * a.c.heads * a.tiles;
-            len = seq_len(a, ++seq);
-            units = units_of(len, kWideTile);
-        }
-        item = (int)((u - seq_first) / units);
-        item_first = seq_first + (int64_t)item * units;
+        do {
+            if (u >= share.last) return false;
+            while (u >= seq_first + (int64_t)(units + share.extra) * a.c.heads * a.tiles) {
+                seq_first += (int64_t)(units + share.extra) * a.c.heads * a.tiles;
+                len = seq_len(a, ++seq);
+                units = units_of(len, kWideTile);
+            }
+            item = (int)((u - seq_first) / (units + share.extra));
+            item_first = seq_first + (int64_t)item * (units + share.extra);
+            ua = (int)(u - item_first);
+            u = item_first + units + share.extra;
+        } while (ua >= units);  // a share that begins behind an item's units
         head = item / a.tiles;
         tile = item % a.tiles;
-        ua = (int)(u - item_first);
         ub = (int)min((int64_t)units, share.last - item_first);
         keys = len.rows ? len.context + len.rows : 0;
-        u = item_first + ub;
         return true;
     };
 
@@ -642,8 +648,9 @@ template <int D, bool BF16, bool PAIR> static int launch_wide(zq_ctx *ctx, AttnA
     return launch_attention_join(ctx, a, BF16, (int)ctas, kRows, D, err);
 }
 
-// From 33 rows on.  With 20 rows of heads of 128 the kernel of zq_attn.cu takes 13.4 / 25.3 / 49.0 us for one sequence at 200, eight at 4000 and sixteen at 8000
-// positions of four cache heads, this one 16.3 / 29.4 / 48.9; with 40 rows 19.4 / 38.7 / 71.0 and 17.3 / 31.1 / 50.9.
+// From 33 rows on.  With 24 rows of heads of 128 the kernel of zq_attn.cu takes 14.1 / 26.3 / 46.4 us for one sequence at 200, eight at 4000 and sixteen at 8000
+// positions of four cache heads, this one 17.9 / 25.6 / 48.7; with 40 rows 19.5 / 38.4 / 68.6 and 18.6 / 26.6 / 50.3 (pages of 64; of 8, where a copy is a
+// short box: 19.5 / 40.5 / 83.4 and 18.6 / 32.9 / 78.2 for 40 rows).
 int launch_attention_wide(zq_ctx *ctx, AttnArgs &a, const zq_kv_cache *cache, bool &taken, zq_error *err) {
     const int rows = a.rows * a.group, d = a.c.head_dim;
     taken = rows > 32 && d >= 64 && d <= 128 && cache->page_size >= 8 && ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 && a.q_stride % 8 == 0;
