@@ -30,6 +30,10 @@ constexpr int kWideThreads = 320, kWideTile = 128;
 // positions take 42.7 / 63.9 / 114 / 53.5 us without it, 36.3 / 53.8 / 94 / 51.8 with 3, 32.2 / 48.4 / 85 / 49.0 with 7, 32.1 / 49.0 / 85 / 49.7 with 12.
 constexpr int kWideEnd = 7;
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool there) {
+    const int n = there ? 16 : 0;  // 0: sixteen zero bytes, nothing is read
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
 __device__ __forceinline__ bool wide_elect() {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
@@ -86,18 +90,19 @@ template <int D> struct WideShape {
     static constexpr int kBlock = kWideTile * 128;      // bytes of 64 values of 128 rows
     static constexpr int kTileBytes = kBlocks * kBlock;
     static constexpr int kRing = D == 128 ? 5 : 10;     // K and V tiles
-    static constexpr int kQ = 0, kRingAt = 2 * kTileBytes, kBars = kRingAt + kRing * kTileBytes;
+    static constexpr int kQ = 0, kPlace = 2 * kWideTile * 128, kRingAt = 2 * kPlace, kBars = kRingAt + kRing * kTileBytes;
+    static_assert(kTileBytes <= kPlace, "a place of Q: a tile, later 32 columns of both slots' sums");
     static constexpr int kSmem = kBars + 3072;          // barriers, maxima and sums of the slots' rows
     static_assert(kSmem <= 227 << 10, "shared memory");
 };
 
 struct WideBars {
-    uint64_t full[10], empty[10], scores[2], weights[2], sums[2], q[2], end;  // 8 bytes each, at kFull and so on
+    uint64_t full[10], empty[10], scores[2], weights[2], sums[2], q[2], left[2], start, end;  // 8 bytes each, at kFull and so on
     uint32_t tmem, dead, poison[2][4];     // rows of a tile of V that were cleared of infinities and NaN, per slot
     float top[2][kWideTile], sum[2][kWideTile];  // of the slots' rows, when the slots share rows
 };
-constexpr uint32_t kFull = 0, kEmpty = 80, kScores = 160, kWeights = 176, kSums = 192, kQ = 208, kEnd = 224;
-static_assert(sizeof(WideBars) <= 3072 && offsetof(WideBars, q) == kQ && offsetof(WideBars, end) == kEnd, "barriers");
+constexpr uint32_t kFull = 0, kEmpty = 80, kScores = 160, kWeights = 176, kSums = 192, kQ = 208, kLeft = 224, kStart = 240, kEnd = 248;
+static_assert(sizeof(WideBars) <= 3072 && offsetof(WideBars, q) == kQ && offsetof(WideBars, left) == kLeft && offsetof(WideBars, start) == kStart && offsetof(WideBars, end) == kEnd, "barriers");
 
 __device__ __forceinline__ bool poll(uint32_t at, uint32_t parity) {
     uint32_t ok;
@@ -130,8 +135,10 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
             mbar_init(&bar.scores[i], 1);
             mbar_init(&bar.weights[i], kWideTile);
             mbar_init(&bar.sums[i], 1);
-            mbar_init(&bar.q[i], kWideTile);
+            mbar_init(&bar.q[i], PAIR ? kWideTile : 32);
+            mbar_init(&bar.left[i], 2 * kWideTile);
         }
+        mbar_init(&bar.start, kWideThreads);
         mbar_init(&bar.end, 1);
         bar.dead = 0;
         fence_mbar_init();
@@ -190,11 +197,33 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
         return true;
     };
 
+    // The rows of Q of an item into one of two tiles, in turn (slots that have rows of their own load them themselves: their tiles have no second place).  The first
+    // item's by all threads, those of the next ones by the copying warp while the item before is worked on.
+    int nth = 0;  // item of this CTA
+    auto load_q = [&](int who, int of) {
+        const uint8_t *from = a.q + 2 * ((int64_t)seq * a.rows * a.q_stride + (int64_t)head * a.group * d);
+        const uint32_t to = base + S::kQ + (nth & 1) * S::kPlace;
+#pragma unroll 2
+        for (int idx = who; idx < kWideTile * (D / 8); idx += of) {
+            const int r = idx / (D / 8), c = idx % (D / 8), q_row = tile * kRows + r, qi = (int)((unsigned)q_row / (unsigned)a.group);
+            const bool there = qi < len.rows && 8 * c < d;
+            cp_async16(to + (c >> 3) * S::kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), there ? from + 2 * (qi * a.q_stride + (int64_t)(q_row - qi * a.group) * d + 8 * c) : a.q, there);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto have_q = [&](uint64_t *barrier) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        fence_proxy_async();
+        mbar_arrive(barrier);
+    };
+    bool more = next_item();
+    if (!PAIR && more) load_q(tid, kWideThreads);
+
     if (warp == 8) {
         // ---- copies
         const int box_shift = min(a.c.page_shift, 7), boxes = kWideTile >> box_shift, box_rows = 1 << box_shift;
         uint32_t at = 0, phase = 0;  // ring place; how often round
-        while (next_item()) {
+        for (; more; more = next_item(), ++nth) {
             auto page_of = [&](int t) {
                 const int key = t * kWideTile + lane * box_rows;
                 if (lane >= boxes || t >= ub || key >= keys) return a.c.pages;  // no page: zeros
@@ -222,6 +251,13 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                         ++phase;
                     }
                 }
+                if (!PAIR && t == ua) {
+                    if (nth) {
+                        if (nth > 1) wait(kLeft + 8 * (nth & 1), ((nth >> 1) - 1) & 1, kStatusMmaTimeout);
+                        load_q(lane, 32);
+                    }
+                    have_q(nth ? &bar.q[nth & 1] : &bar.start);
+                }
             }
         }
         // where waits ran out, nobody has waited for the last copies
@@ -248,17 +284,19 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
             }
         } k_at{0, 0}, v_at{1, 0};
         const uint32_t ring_k = sw128_low(base + S::kRingAt, 16), ring_v = sw128_low(base + S::kRingAt, S::kBlock);
-        const uint32_t q_low[2] = {sw128_low(base + S::kQ, 16), sw128_low(base + S::kQ + (PAIR ? S::kTileBytes : 0), 16)};
+        const uint32_t q_at[2] = {sw128_low(base + S::kQ, 16), sw128_low(base + S::kQ + S::kPlace, 16)};  // of the slots, or of this item and the next
+        if (!PAIR && more) have_q(&bar.start);
         // products of slot s: scores with the K tile at k_at, sums with the V tile at v_at
         auto scores = [&](int s) {
             if (!PAIR || s == 0) wait(kFull + 8 * k_at.slot, k_at.parity, kStatusTmaTimeout);
             tc_after();
+            const uint32_t q_low = q_at[PAIR ? s : nth & 1];
             const uint32_t kd = __shfl_sync(0xffffffffu, ring_k + k_at.slot * (S::kTileBytes / 16), 0), release = bars + kEmpty + 8 * k_at.slot;
             if (wide_elect()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint32_t off = (k >> 2) * (S::kBlock / 16) + (k & 3) * 2;
-                    mma_ss(tmem + s * 256, sw128_desc(q_low[s] + off), sw128_desc(kd + off), idesc_s, k > 0);
+                    mma_ss(tmem + s * 256, sw128_desc(q_low + off), sw128_desc(kd + off), idesc_s, k > 0);
                 }
                 tc_commit(bars + kScores + 8 * s);
                 if (!PAIR || s == 1) tc_commit(release);
@@ -281,11 +319,17 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
             __syncwarp();
             if (!PAIR || s == 1) v_at.step();
         };
-        while (next_item()) {
+        for (; more; more = next_item(), ++nth) {
             const int n = ub - ua, jobs = PAIR ? 2 * n : n;
-            wait(kQ, q_phase, kStatusMmaTimeout);
-            if (PAIR) wait(kQ + 8, q_phase, kStatusMmaTimeout);
-            q_phase ^= 1;
+            if (PAIR) {
+                wait(kQ, q_phase, kStatusMmaTimeout);
+                wait(kQ + 8, q_phase, kStatusMmaTimeout);
+                q_phase ^= 1;
+            } else if (nth) {
+                wait(kQ + 8 * (nth & 1), (nth - 1) >> 1 & 1, kStatusMmaTimeout);
+            } else {
+                wait(kStart, 0, kStatusMmaTimeout);
+            }
             scores(0);
             if (jobs > 1) scores(1);
 #pragma unroll 1
@@ -309,11 +353,12 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
         uint32_t n_sums = 0;   // products that this slot has been through
         uint32_t first = 0;
         const int chunks = d / 8;
-        while (next_item()) {
+        if (!PAIR && more) have_q(&bar.start);
+        for (; more; more = next_item(), ++nth) {
             const int n = ub - ua, mine = PAIR ? n : (n + 1 - s) / 2;
             // ---- this slot's rows of Q
-            if (PAIR || s == 0) {
-                uint8_t *q_tile = smem + S::kQ + s * S::kTileBytes;
+            if (PAIR) {
+                uint8_t *q_tile = smem + S::kQ + s * S::kPlace;
                 const int r0 = tile * kRows + s * kWideTile, n_rows = len.rows * a.group;
                 uint4 v[D / 8];
 #pragma unroll
@@ -336,7 +381,7 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) tm_st32(t_o + 32 * c, zero);
             tm_st_wait();
-            if (PAIR || s == 0) mbar_arrive(&bar.q[s]);
+            if (PAIR) mbar_arrive(&bar.q[s]);
             const int q_row = tile * kRows + (PAIR ? s * kWideTile : 0) + row, i = q_row / a.group;
             float top = -INFINITY, sum = 0.f;  // top: what the weights are relative to, in scores as they come
 
@@ -533,7 +578,7 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
             const int64_t to = i >= a.rows ? -1 : whole ? (((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + q_row % a.group) * d : (int64_t)part_row * D;
             // The sums leave by way of the place of Q, which is through ([128][D / 2] f32, chunks of 16 bytes swizzled), whole lines at a time: 32 columns of the
             // warp's 32 rows.  Loops, not straight code: it runs once per item, at the pace of instruction fetches.
-            auto chunk_at = [&](uint8_t *region, int r, int c) { return region + r * (2 * D) + ((c ^ (r & 7)) << 4); };
+            auto chunk_at = [&](uint8_t *region, int r, int c) { return region + r * (PAIR ? 2 * D : 128) + ((c ^ (r & 7)) << 4); };
             auto put = [&](uint8_t *region, int c0, int col) {
                 __syncwarp();
 #pragma unroll 2
@@ -548,7 +593,7 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                 __syncwarp();
             };
             float log_top = top == -INFINITY ? -INFINITY : top * a.scale;
-            uint8_t *stage = smem + S::kQ + s * S::kTileBytes;
+            uint8_t *stage = smem + S::kQ + (PAIR ? s * S::kPlace : (nth & 1) * S::kPlace + s * (S::kPlace / 2));
             uint32_t x[32];
             if (PAIR) {
                 const bool none = whole && (sum == 0.f || i >= len.rows);
@@ -569,27 +614,24 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                 bar.sum[s][row] = sum;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 const float other = bar.top[1 - s][row], both = fmaxf(log_top, other), scale = log_top == -INFINITY ? 0.f : ex2(log_top - both);
+                sum = (scale == 0.f ? 0.f : sum * scale) + (other == -INFINITY ? 0.f : bar.sum[1 - s][row] * ex2(other - both));
+                log_top = both;
+                const bool none = whole && (sum == 0.f || i >= len.rows);
+                const float inv = !whole ? 1.f : none ? 0.f : 1.f / sum;
+                uint8_t *from = smem + S::kQ + (nth & 1) * S::kPlace + (1 - s) * (S::kPlace / 2);
 #pragma unroll 1
                 for (int c = 0; c < D / 64; ++c) {
                     tm_ld32(t_o + (1 - s) * (D / 2) + 32 * c, x);
                     tm_ld_wait(x);
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4 *>(chunk_at(stage, row, 8 * c + e / 4)) = scale == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(__uint_as_float(x[e]) * scale, __uint_as_float(x[e + 1]) * scale, __uint_as_float(x[e + 2]) * scale, __uint_as_float(x[e + 3]) * scale);
-                }
-                sum = (scale == 0.f ? 0.f : sum * scale) + (other == -INFINITY ? 0.f : bar.sum[1 - s][row] * ex2(other - both));
-                log_top = both;
-                const bool none = whole && (sum == 0.f || i >= len.rows);
-                const float inv = !whole ? 1.f : none ? 0.f : 1.f / sum;
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                uint8_t *from = smem + S::kQ + (1 - s) * S::kTileBytes;
-#pragma unroll 1
-                for (int c = 0; c < D / 64; ++c) {
+                        *reinterpret_cast<float4 *>(chunk_at(stage, row, e / 4)) = scale == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(__uint_as_float(x[e]) * scale, __uint_as_float(x[e + 1]) * scale, __uint_as_float(x[e + 2]) * scale, __uint_as_float(x[e + 3]) * scale);
                     tm_ld32(t_o + s * (D / 2) + 32 * c, x);
                     tm_ld_wait(x);
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
-                        float4 *at = reinterpret_cast<float4 *>(chunk_at(from, row, 8 * c + e / 4));
+                        float4 *at = reinterpret_cast<float4 *>(chunk_at(from, row, e / 4));
                         float4 v = *at;
                         if (scale != 0.f) {
                             v.x += __uint_as_float(x[e]) * scale;
@@ -599,14 +641,16 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                         }
                         *at = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
                     }
-                    put(from, 8 * c, s * (D / 2) + 32 * c);
+                    put(from, 0, s * (D / 2) + 32 * c);
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
                 }
+                mbar_arrive(&bar.left[nth & 1]);
             }
             if (!whole && (PAIR || s == 0)) {
                 part[kRows * D + part_row] = log_top;
                 part[kRows * D + kRows + part_row] = sum;
             }
-            asm volatile("bar.sync %0, %1;" ::"r"(PAIR ? 2 + s : 1), "n"(PAIR ? kWideTile : 2 * kWideTile) : "memory");  // the next item's rows of Q and maxima go where these sums were
+            if (PAIR) asm volatile("bar.sync %0, %1;" ::"r"(2 + s), "n"(kWideTile) : "memory");  // the next item's rows of Q go where these sums were
             if (tid == 0 && ua == 0 && ub < units) {
                 const int64_t end = item_first + units;
                 a.info[blockIdx.x] = make_int4(seq, item, (int)((end * share.ctas - 1) / share.total) - (int)blockIdx.x + 1, len.rows);
