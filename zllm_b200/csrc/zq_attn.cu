@@ -44,8 +44,8 @@ template <bool BF16> __device__ __forceinline__ void mma16(float (&d)[4], const 
         mma_16816(d, a[0], a[1], a[2], a[3], b0, b1);
 }
 constexpr int kMaxSplit = 8;  // CTAs of an item in a cluster
-// What the end of an item costs, in units.  A decode step of 8 rows per cache head of 128, 4 cache heads, takes 26.0 / 42.2 / 74.8 / 68.4 us for 64 unequal sequences of up to
-// 200 and 1000, 150 of 900 and 40 of 5000 positions without it, 25.8 / 39.1 / 69.8 / 65.4 with 1, 22.8 / 36.3 / 62.4 / 62.4 with 3, 22.8 / 37.7 / 65.3 / 64.2 with 6.
+// What the end of an item costs, in units.  A decode step of 8 rows per cache head of 128, 4 cache heads, takes 24.8 / 40.2 / 73.1 / 66.6 us for 64 unequal sequences of up to
+// 200 and 1000, 150 of 900 and 40 of 5000 positions without it, 21.6 / 35.1 / 60.7 / 61.1 with 3, 21.8 / 36.6 / 63.7 / 63.4 with 6.
 constexpr int kItemEnd = 3;
 
 // Shape of the kernel for a head of up to D values and WM warps of 16 rows.
@@ -409,61 +409,68 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
     }
 }
 
-// Joins the parts of the item that starts in CTA blockIdx.x's share, in the order of its keys: four rows per CTA, two warps a row, which take the parts in
-// turn; a lane has four columns.
-constexpr int kJoinRows = 4;
-template <bool BF16> __global__ void __launch_bounds__(64 * kJoinRows) attention_join_kernel(const AttnArgs a, int rows, int d_pad) {
+// Joins the parts of the item that starts in CTA blockIdx.x's share, in the order of its keys: a warp per row, a lane has four columns.  It waits for memory and little
+// else, so a row's first parts, and the maxima and sums of the first 32, are on their way before any is used; weights come from the lanes that have them.
+// (40 sequences of up to 5000 positions with 240 rows per cache head of 128, 30 MB of parts: 15 us; 33 with two warps a row that took four rows in turn and
+// the weights from memory; 20 with four parts ahead, 34 with eight, as the code is met cold.)
+constexpr int kJoinRows = 8, kJoinAhead = 2;
+template <bool BF16> __global__ void __launch_bounds__(32 * kJoinRows) attention_join_kernel(const AttnArgs a, int rows, int d_pad) {
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int4 info = a.info[blockIdx.x];
-    if (info.z == 0) return;
-    __shared__ float4 s_sum[kJoinRows][32];
     const int seq = info.x, head = info.y / a.tiles, tile = info.y % a.tiles, pieces = info.z, d = a.c.head_dim;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, which = warp & 1;
+    const int lane = threadIdx.x & 31, r = kJoinRows * blockIdx.y + (threadIdx.x >> 5), row = tile * rows + r, i = row / a.group;
+    if (pieces == 0 || r >= rows || i >= a.rows) return;
     const size_t floats = (size_t)rows * (d_pad + 2);
     auto part = [&](int p) { return a.parts + ((size_t)(blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * floats; };
-    for (int r = kJoinRows * blockIdx.y + (warp >> 1); r < rows; r += kJoinRows * gridDim.y) {
-        const int row = tile * rows + r, i = row / a.group;
-        float m = -INFINITY, l = 0.f;
-        if (i < a.rows)
-            for (int p = lane; p < pieces; p += 32) m = fmaxf(m, part(p)[rows * d_pad + r]);
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float base = m == -INFINITY ? 0.f : m;
-        if (i < a.rows)
-            for (int p = lane; p < pieces; p += 32) l += exp2f(part(p)[rows * d_pad + r] - base) * part(p)[rows * d_pad + rows + r];
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        const bool none = l == 0.f || i >= info.w;
-        const float inv = none ? 0.f : 1.f / l;
-        for (int c0 = 0; c0 < d; c0 += 128) {
-            const int col = c0 + 4 * lane;
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (i < a.rows && col < d) {
-#pragma unroll 8
-                for (int p = which; p < pieces; p += 2) {
-                    const float *f = part(p);
-                    const float w = exp2f(f[rows * d_pad + r] - base);
-                    const float4 v = *reinterpret_cast<const float4 *>(f + (size_t)r * d_pad + col);
-                    sum.x += w * v.x;
-                    sum.y += w * v.y;
-                    sum.z += w * v.z;
-                    sum.w += w * v.w;
-                }
+    auto values = [&](int p, int col) { return p < pieces && col < d ? *reinterpret_cast<const float4 *>(part(p) + (size_t)r * d_pad + col) : make_float4(0.f, 0.f, 0.f, 0.f); };
+    float4 v[kJoinAhead];
+#pragma unroll
+    for (int p = 0; p < kJoinAhead; ++p) v[p] = values(p, 4 * lane);
+    const float first_top = lane < pieces ? part(lane)[rows * d_pad + r] : -INFINITY, first_sum = lane < pieces ? part(lane)[rows * d_pad + rows + r] : 0.f;
+    float m = first_top;
+    for (int p = lane + 32; p < pieces; p += 32) m = fmaxf(m, part(p)[rows * d_pad + r]);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float base = m == -INFINITY ? 0.f : m, first_w = exp2f(first_top - base);
+    float l = first_w * first_sum;
+    for (int p = lane + 32; p < pieces; p += 32) l += exp2f(part(p)[rows * d_pad + r] - base) * part(p)[rows * d_pad + rows + r];
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const bool none = l == 0.f || i >= info.w;
+    const float inv = none ? 0.f : 1.f / l;
+    for (int c0 = 0; c0 < d; c0 += 128) {
+        const int col = c0 + 4 * lane;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float w_lane = first_w;
+        auto add = [&](float w, const float4 &x) {
+            sum.x += w * x.x;
+            sum.y += w * x.y;
+            sum.z += w * x.z;
+            sum.w += w * x.w;
+        };
+        for (int p0 = 0; p0 < pieces; p0 += kJoinAhead) {
+            float4 next[kJoinAhead];  // those behind, or the next columns' first
+            const bool over = p0 + kJoinAhead >= pieces;
+#pragma unroll
+            for (int k = 0; k < kJoinAhead; ++k) next[k] = values(over ? k : p0 + kJoinAhead + k, over ? col + 128 : col);
+            if (p0 && p0 % 32 == 0) w_lane = p0 + lane < pieces ? exp2f(part(p0 + lane)[rows * d_pad + r] - base) : 0.f;
+#pragma unroll
+            for (int k = 0; k < kJoinAhead; ++k) {
+                const float w = __shfl_sync(0xffffffffu, w_lane, (p0 + k) & 31);
+                if (p0 + k < pieces) add(w, v[k]);
+                v[k] = next[k];
             }
-            __syncthreads();
-            if (which) s_sum[warp >> 1][lane] = sum;
-            __syncthreads();
-            if (!which && i < a.rows && col < d) {
-                const float4 v = s_sum[warp >> 1][lane];
-                uint32_t *to = reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col));
-                to[0] = none ? 0u : pack2<BF16>((sum.x + v.x) * inv, (sum.y + v.y) * inv);
-                to[1] = none ? 0u : pack2<BF16>((sum.z + v.z) * inv, (sum.w + v.w) * inv);
-            }
+        }
+        if (col < d) {
+            uint32_t *to = reinterpret_cast<uint32_t *>(a.out + 2 * ((((int64_t)seq * a.rows + i) * a.c.heads * a.group + head * a.group + row % a.group) * d + col));
+            to[0] = none ? 0u : pack2<BF16>(sum.x * inv, sum.y * inv);
+            to[1] = none ? 0u : pack2<BF16>(sum.z * inv, sum.w * inv);
         }
     }
 }
 
 int launch_attention_join(zq_ctx *ctx, const AttnArgs &a, bool bf16, int ctas, int rows, int d_pad, zq_error *err) {
-    return launch_pdl(ctx, bf16 ? attention_join_kernel<true> : attention_join_kernel<false>, dim3((unsigned)ctas, (unsigned)(rows / kJoinRows < 16 ? rows / kJoinRows : 16)), dim3(64 * kJoinRows), 0, err, a, rows, d_pad);
+    const int used = a.rows * a.group < rows ? a.rows * a.group : rows;
+    return launch_pdl(ctx, bf16 ? attention_join_kernel<true> : attention_join_kernel<false>, dim3((unsigned)ctas, (unsigned)((used + kJoinRows - 1) / kJoinRows)), dim3(32 * kJoinRows), 0, err, a, rows, d_pad);
 }
 
 constexpr size_t kClusterBytes = size_t(512) << 10;

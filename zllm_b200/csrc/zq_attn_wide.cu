@@ -25,9 +25,9 @@
 namespace zq {
 
 constexpr int kWideThreads = 320, kWideTile = 128;
-// What the end of an item and the start of the next cost, in tiles of keys: 15 000 cycles, in which the ring stands still (the sums out of tensor memory, the rows
-// of Q, the first scores with nothing beside them).  40 rows per cache head of 128, 4 cache heads: 64 unequal sequences of up to 200 and 1000, 150 of 900 and 16 of 8000
-// positions take 42.7 / 63.9 / 114 / 53.5 us without it, 36.3 / 53.8 / 94 / 51.8 with 3, 32.2 / 48.4 / 85 / 49.0 with 7, 32.1 / 49.0 / 85 / 49.7 with 12.
+// What the end of an item and the start of the next cost, in tiles of keys: some 10 000 cycles in which the ring stands still (the sums out of tensor memory, the first
+// weights with no product beside them).  40 rows per cache head of 128, 4 cache heads: 64 unequal sequences of up to 200 and 1000, 150 of 900 and 16 of 8000
+// positions take 34.7 / 50.5 / 93 / 48.4 us without it, 28.0 / 41.6 / 74 / 45.4 with 7, 27.9 / 42.5 / 74 / 45.6 with 11.
 constexpr int kWideEnd = 7;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool there) {
@@ -692,9 +692,9 @@ template <int D, bool BF16, bool PAIR> static int launch_wide(zq_ctx *ctx, AttnA
     return launch_attention_join(ctx, a, BF16, (int)ctas, kRows, D, err);
 }
 
-// From 33 rows on.  With 24 rows of heads of 128 the kernel of zq_attn.cu takes 14.1 / 26.3 / 46.4 us for one sequence at 200, eight at 4000 and sixteen at 8000
-// positions of four cache heads, this one 17.9 / 25.6 / 48.7; with 40 rows 19.5 / 38.4 / 68.6 and 18.6 / 26.6 / 50.3 (pages of 64; of 8, where a copy is a
-// short box: 19.5 / 40.5 / 83.4 and 18.6 / 32.9 / 78.2 for 40 rows).
+// From 33 rows on.  With 24 rows of heads of 128 the kernel of zq_attn.cu takes 14.2 / 26.4 / 45.5 us for one sequence at 200, eight at 4000 and sixteen at 8000
+// positions of four cache heads, this one 15.5 / 22.0 / 44.4; with 40 rows 19.5 / 38.6 / 65.2 and 15.7 / 23.1 / 45.2 (pages of 64; of 8, where a copy is a
+// short box: 14.1 / 28.4 / 50.4 and 17.1 / 32.2 / 74.3 for 24 rows, 19.5 / 40.3 / 80.3 and 17.3 / 31.0 / 74.8 for 40).
 int launch_attention_wide(zq_ctx *ctx, AttnArgs &a, const zq_kv_cache *cache, bool &taken, zq_error *err) {
     const int rows = a.rows * a.group, d = a.c.head_dim;
     taken = rows > 32 && d >= 64 && d <= 128 && cache->page_size >= 8 && ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 && a.q_stride % 8 == 0;
