@@ -270,6 +270,23 @@ def test_attention_of_many_sequences():
     run_attention(g, 700, 1, 2, 1, 64, 16, contexts, torch.float16, False)
 
 
+# more units than CTAs: shares that end and begin inside items, between them, and over many short ones
+@pytest.mark.parametrize("rows,group,dim", [(1, 1, 128), (1, 8, 64), (3, 8, 128), (6, 8, 128), (9, 5, 64), (20, 8, 128), (70, 4, 64)])
+@pytest.mark.parametrize("longest", [60, 400, 1500])
+def test_attention_of_shares_that_cross_items(rows, group, dim, longest):
+    g = gen_of(90 + rows + longest)
+    contexts = torch.randint(0, longest + 1, (93,), generator=g).tolist()
+    drafted = torch.randint(0, rows + 1, (93,), generator=g).tolist()
+    run_attention(g, 93, rows, 2 * group, 2, dim, 16, contexts, torch.bfloat16, tree=True, drafted=drafted)
+
+
+# few long items over all CTAs, many parts each
+@pytest.mark.parametrize("rows,group,context", [(1, 4, 30011), (2, 24, 9001), (66, 2, 20000), (1, 1, 148 * 128 - 1)])
+@pytest.mark.parametrize("dim", [64, 128, 192])
+def test_attention_of_items_in_many_parts(rows, group, context, dim):
+    run_attention(gen_of(300 + rows), 1, rows, group, 1, dim, 64, [context], torch.float16, tree=True)
+
+
 @pytest.mark.parametrize("rows,group", [(6, 1), (6, 5), (12, 8)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf])
