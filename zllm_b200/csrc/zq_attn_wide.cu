@@ -24,7 +24,7 @@
 
 namespace zq {
 
-constexpr int kWideThreads = 320, kWideTile = 128;
+constexpr int kWideThreads = 320, kWideTile = 128, kBarBytes = 3 << 10;
 // What the end of an item and the start of the next cost, in tiles of keys: some 10 000 cycles in which the ring stands still (the sums out of tensor memory, the first
 // weights with no product beside them).  40 rows per cache head of 128, 4 cache heads: 64 unequal sequences of up to 200 and 1000, 150 of 900 and 16 of 8000
 // positions take 34.7 / 50.5 / 93 / 48.4 us without it, 28.0 / 41.6 / 74 / 45.4 with 7, 27.9 / 42.5 / 74 / 45.6 with 11.
@@ -92,7 +92,7 @@ template <int D> struct WideShape {
     static constexpr int kRing = D == 128 ? 5 : 10;     // K and V tiles
     static constexpr int kQ = 0, kPlace = 2 * kWideTile * 128, kRingAt = 2 * kPlace, kBars = kRingAt + kRing * kTileBytes;
     static_assert(kTileBytes <= kPlace, "a place of Q: a tile, later 32 columns of both slots' sums");
-    static constexpr int kSmem = kBars + 3072;          // barriers, maxima and sums of the slots' rows
+    static constexpr int kSmem = kBars + kBarBytes;     // barriers, maxima and sums of the slots' rows
     static_assert(kSmem <= 227 << 10, "shared memory");
 };
 
@@ -102,7 +102,7 @@ struct WideBars {
     float top[2][kWideTile], sum[2][kWideTile];  // of the slots' rows, when the slots share rows
 };
 constexpr uint32_t kFull = 0, kEmpty = 80, kScores = 160, kWeights = 176, kSums = 192, kQ = 208, kLeft = 224, kStart = 240, kEnd = 248;
-static_assert(sizeof(WideBars) <= 3072 && offsetof(WideBars, q) == kQ && offsetof(WideBars, left) == kLeft && offsetof(WideBars, start) == kStart && offsetof(WideBars, end) == kEnd, "barriers");
+static_assert(sizeof(WideBars) <= kBarBytes && offsetof(WideBars, q) == kQ && offsetof(WideBars, left) == kLeft && offsetof(WideBars, start) == kStart && offsetof(WideBars, end) == kEnd, "barriers");
 
 __device__ __forceinline__ bool poll(uint32_t at, uint32_t parity) {
     uint32_t ok;
