@@ -1,0 +1,24 @@
+"""Rules of the kernels on drafted tokens that no run shows, read from the sources: what breaks them shows up as a wrong value or a fault once in a long while, if at all."""
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "zllm_b200", "csrc")
+
+
+def _source(name):
+    with open(os.path.join(CSRC, name)) as f:
+        return re.sub(r"//[^\n]*", "", f.read())
+
+
+def test_verification_stores_into_ctas_that_run():
+    """Shared memory of another CTA may be touched once that CTA has started, which a barrier of the cluster alone tells: every thread arrives at one as the kernel
+    begins and waits for it, outside of any condition, before the first exchange and before it can leave."""
+    text = _source("zq_verify.cu")
+    kernel = text[text.index("verify_draft_kernel(const VerifyArgs a) {"):]
+    kernel = kernel[:kernel.index("template <class T> static int launch_verify")]
+    arrive, wait = kernel.index("cluster.barrier_arrive();"), kernel.index("cluster.barrier_wait();")
+    assert kernel.count("barrier_arrive") == kernel.count("barrier_wait") == 1
+    first = min(kernel.index(word) for word in ("exchange_rows(", "exchange_sums(", "map_shared_rank", "cluster.sync()") if word in kernel)
+    assert arrive < wait < first
+    assert kernel[:arrive].count("{") - kernel[:arrive].count("}") == 1 and kernel[:wait].count("{") - kernel[:wait].count("}") == 1  # in the body itself
+    assert "return" not in kernel[:wait]

@@ -207,6 +207,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
     extern __shared__ double s_seg[];  // sums of this CTA's segments, then their slopes
     __shared__ VerifyShared s;
     cg::cluster_group cluster = cg::this_cluster();
+    cluster.barrier_arrive();  // this CTA runs: peers wait for it before they store into this CTA
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), seq = blockIdx.x / ctas;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const double root = exp2(lane / 32.0);
@@ -220,6 +221,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
         s.u[i] = a.accept_u[row0 + i];
     }
     __syncthreads();
+    cluster.barrier_wait();  // all CTAs run, and have done so since before the tables were read
     const bool greedy = heat == 0.f, drawn = a.draft != nullptr && !greedy;
     const double scale = 1.4426950408889634074 / (greedy ? 1.0 : (double)heat);
     const float scale32 = (float)fmin(scale, 1e30);
