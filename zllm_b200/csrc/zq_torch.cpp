@@ -467,14 +467,15 @@ Rows rows_3d(PyObject *o, int device, const char *what) {
     for (int64_t i = 0; i < n - 2; ++i) r.rows *= r.t.size(i);
     if (r.rows == 0 || r.heads == 0 || r.dim == 0) fail(1, std::string(what) + " of shape " + sizes_of(r.t) + " is empty");
     bool one = (r.dim == 1 || r.t.stride(n - 1) == 1) && (r.heads == 1 || r.t.stride(n - 2) == r.dim);
-    int64_t step = 0, inner = 1;  // the leading dimensions as one
+    int64_t step = r.heads * r.dim, inner = 1;  // the leading dimensions as one; a single row needs no distance
+    bool seen = false;                          // a dimension of more than one row, whose stride may be 0 (expanded)
     for (int64_t i = n - 3; i >= 0 && one; --i) {
         if (r.t.size(i) == 1) continue;
-        if (!step) step = r.t.stride(i);
+        if (!seen) step = r.t.stride(i);
         else one = r.t.stride(i) == step * inner;
+        seen = true;
         inner *= r.t.size(i);
     }
-    if (!step) step = r.heads * r.dim;
     if (!one || step < r.heads * r.dim) {
         r.t = contiguous(r.t);
         step = r.heads * r.dim;
