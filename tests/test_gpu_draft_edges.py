@@ -53,3 +53,62 @@ def test_expanded_queries_attend_as_dense_ones_do(small, shape, heads):
     want = ctx().tree_attention(q.contiguous(), k_pages, v_pages, table, context)
     ctx().sync()
     assert torch.equal(got, want)
+
+
+# ---- verification
+def test_verification_of_the_largest_vocabulary_by_many_sequences():
+    """Many sequences have few CTAs each, and these have the sums of a long run of the vocabulary in shared memory."""
+    batch, vocab = 300, 1 << 22
+    logits = torch.zeros((1, 1, vocab), dtype=torch.float16, device="cuda").repeat(batch, 1, 1)
+    g = gen_of(6)
+    at = torch.randint(0, vocab, (batch,), generator=g)
+    at[:4] = torch.tensor([0, vocab - 1, vocab // 2, vocab // 2 - 1])
+    logits[torch.arange(batch), 0, at.cuda()] = 40.0  # e^40 times as likely as each other one, 5.6e10 times as all of them
+    u, heat, parents = torch.rand(batch, generator=g), torch.ones(batch), torch.full((1,), -1, dtype=torch.int32)
+    u[:] = 0.25 + 0.5 * u
+    heat[::3] = 0.0
+    for device_heat in (heat, torch.ones(batch) * 1e30):
+        path, accepted, token = ctx().verify_draft(logits, torch.zeros((batch, 1), dtype=torch.int32).cuda(), parents.cuda(), torch.zeros((batch, 1)).cuda(), u.cuda(), device_heat.cuda())
+        ctx().sync()
+        assert (path == 0).all() and (accepted == 1).all()
+        if device_heat is heat:
+            assert torch.equal(token.cpu().long(), at)
+        else:  # all tokens as likely to 1e-28: the first whose number of tokens up to it exceeds u vocab, but where the two are within the sums' 1e-9 of each other
+            want = torch.floor(u.double() * vocab)
+            clear = (u.double() * vocab - want - 0.5).abs() < 0.49
+            assert clear.sum() > batch // 2 and torch.equal(token.cpu().double()[clear], want[clear])
+
+
+def test_two_threads_verify_vocabularies_of_unlike_sizes():
+    """Contexts of two threads, on streams of their own: what one launch asks for must not be taken from the other's."""
+    import threading
+
+    from zllm_b200.backend import B200Context
+
+    batch = 300
+    done, made = {}, {}
+    for name, vocab in (("small", 1000), ("large", 1 << 17)):
+        logits = torch.zeros((batch, 1, vocab), dtype=torch.bfloat16, device="cuda")
+        logits[:, 0, vocab - 2] = 60.0
+        made[name] = (logits, torch.zeros((batch, 1), dtype=torch.int32).cuda(), ints(-1), torch.zeros((batch, 1)).cuda(), torch.full((batch,), 0.5).cuda(), torch.ones(batch).cuda())
+    torch.cuda.synchronize()
+
+    def work(name):
+        try:
+            stream = torch.cuda.Stream()
+            c = B200Context(0)
+            c.set_stream(stream.cuda_stream)
+            with torch.cuda.stream(stream):
+                got = [c.verify_draft(*made[name])[2] for _ in range(200)]
+            c.sync()
+            done[name] = all((t == made[name][0].shape[2] - 2).all().item() for t in got)
+            c.close()
+        except Exception as e:  # reported by the assertion below
+            done[name] = repr(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in made]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert done == {"small": True, "large": True}

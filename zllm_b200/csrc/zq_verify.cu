@@ -59,6 +59,7 @@ struct VerifyShared {
     float u[kMaxDraftRows];
     alignas(16) float2 list[kVerifyWarps][kSegment];
 };
+constexpr size_t kSegmentBytes = (227 << 10) - (sizeof(VerifyShared) + 1023) / 1024 * 1024;  // room for the sums of a CTA's segments
 
 template <class T> __device__ __forceinline__ float logit(const T *row, int v) {
     if constexpr (sizeof(T) == 4) return row[v];
@@ -688,7 +689,8 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
 
 template <class T> static int launch_verify(zq_ctx *ctx, VerifyArgs &a, int cluster, size_t batch, size_t smem, zq_error *err) {
     ZQ_CUDA_CHECK(cudaFuncSetAttribute(verify_draft_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), err);
-    ZQ_CUDA_CHECK(cudaFuncSetAttribute(verify_draft_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), err);
+    // the same value every time: calls of other threads set it too
+    ZQ_CUDA_CHECK(cudaFuncSetAttribute(verify_draft_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSegmentBytes), err);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(batch * cluster));
     cfg.blockDim = dim3(kVerifyThreads);
@@ -740,7 +742,10 @@ extern "C" int zq_verify_draft(zq_ctx *ctx, const void *dev_logits, const void *
     a.shared_parents = parents_shared;
     a.status = ctx->status_dev;
     const size_t segments = (vocab + 7 + kSegment - 1) / kSegment;  // a row may begin up to seven values behind a boundary
+    auto bytes = [&](int ctas) { return 2 * ((segments + ctas - 1) / ctas) * sizeof(double); };
+    while (bytes(cluster) > kSegmentBytes) cluster *= 2;  // some 3 million tokens a CTA
+    static_assert(2 * ((((size_t(1) << 22) + 7) / kSegment + 1) / 2 + 1) * sizeof(double) <= kSegmentBytes, "two CTAs hold the largest vocabulary");
     a.segments = (int)((segments + cluster - 1) / cluster);
-    const size_t smem = 2 * a.segments * sizeof(double);
+    const size_t smem = bytes(cluster);
     return dtype == ZQ_F32 ? launch_verify<float>(ctx, a, cluster, batch, smem, err) : dtype == ZQ_F16 ? launch_verify<__half>(ctx, a, cluster, batch, smem, err) : launch_verify<__nv_bfloat16>(ctx, a, cluster, batch, smem, err);
 }
