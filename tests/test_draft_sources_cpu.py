@@ -15,7 +15,7 @@ def test_verification_stores_into_ctas_that_run():
     begins and waits for it, outside of any condition, before the first exchange and before it can leave."""
     text = _source("zq_verify.cu")
     kernel = text[text.index("verify_draft_kernel(const VerifyArgs a) {"):]
-    kernel = kernel[:kernel.index("template <class T> static int launch_verify")]
+    kernel = kernel[:kernel.index("static int launch_verify")]
     arrive, wait = kernel.index("cluster.barrier_arrive();"), kernel.index("cluster.barrier_wait();")
     assert kernel.count("barrier_arrive") == kernel.count("barrier_wait") == 1
     first = min(kernel.index(word) for word in ("exchange_rows(", "exchange_sums(", "map_shared_rank", "cluster.sync()") if word in kernel)

@@ -1,9 +1,12 @@
 """Operators on drafted tokens at calls that are allowed and rare: expanded and padded tensors, the largest shapes, random numbers next to a border, values next to the types' ends."""
+import math
+
 import pytest
 import torch
 
+from tests import draft_ref as R
 from tests.gpu_util import ctx
-from tests.test_gpu_draft import gen_of, ints, make_cache
+from tests.test_gpu_draft import check_verify, gen_of, ints, make_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +115,94 @@ def test_two_threads_verify_vocabularies_of_unlike_sizes():
     for t in threads:
         t.join()
     assert done == {"small": True, "large": True}
+
+
+def verified(logits, draft, tokens, parents, accept_u, sample_u, heat):
+    """Of one sequence for each row of `tokens`, against the definition; the paths and tokens."""
+    batch, rows = tokens.shape
+    got = ctx().verify_draft(logits.cuda(), tokens.cuda(), parents.cuda(), accept_u.cuda(), sample_u.cuda(), heat.cuda(), draft_logits=draft.cuda() if draft is not None else None)
+    ctx().sync()
+    want = R.verify(logits, draft, tokens, parents.expand(batch, -1), accept_u, sample_u, heat, [rows] * batch)
+    check_verify(got, want, rows)
+    return want
+
+
+LAST = 1 - 2.0 ** -24  # the largest random number
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("spread", [0.1, 1.0, 4.0, 12.0])
+@pytest.mark.parametrize("vocab", [2, 7, 33, 4099])
+def test_children_that_hold_all_that_is_likely(dtype, spread, vocab):
+    """The children of the root are all tokens of finite logit: with the largest random numbers every child but the last is rejected, and the last one has all of p."""
+    g = gen_of(vocab)
+    batch, rows = 40, 8
+    few = min(rows - 1, vocab)
+    logits = torch.full((batch, rows, vocab), -math.inf, dtype=dtype)
+    tokens = torch.zeros((batch, rows), dtype=torch.int32)
+    for b in range(batch):
+        some = torch.randperm(vocab, generator=g)[:few]
+        logits[b, :, some] = (torch.randn((rows, few), generator=g) * spread).to(dtype)
+        tokens[b, 1:1 + few] = some[torch.randperm(few, generator=g)].to(torch.int32)
+        tokens[b, 1 + few:] = some[0]
+    parents = torch.tensor([-1] + [0] * (rows - 1), dtype=torch.int32)
+    accept_u, sample_u, heat = torch.full((batch, rows), LAST), torch.rand(batch, generator=g), torch.ones(batch)
+    sample_u[::2] = LAST
+    want = verified(logits, None, tokens, parents, accept_u, sample_u, heat)
+    assert all(n == 2 for _, n, _ in want)
+    # as many children but one: what is left is the token that is no child's
+    if few > 1:
+        tokens[:, few:] = tokens[:, 1:2]
+        want = verified(logits, None, tokens, parents, accept_u, sample_u, heat)
+        assert spread > 4 or any(n == 1 for _, n, _ in want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_random_numbers_next_to_a_childs_border(dtype):
+    """The f32 number in front of p(t) / (1 - what is gone), and the one behind it: one child is kept, the other is not."""
+    g = gen_of(17)
+    batch, vocab = 64, 3001
+    logits = (torch.randn((batch, 1, vocab), generator=g) * 2).to(dtype).expand(batch, 4, vocab).contiguous()
+    tokens = torch.zeros((batch, 4), dtype=torch.int32)
+    accept_u = torch.full((batch, 4), 0.999)
+    for b in range(batch):
+        p = torch.softmax(logits[b, 0].double(), 0)
+        top = p.topk(3).indices
+        tokens[b, 1:] = top.to(torch.int32)
+        border = float(p[top[1]] / (1 - p[top[0]]))
+        at = torch.tensor(border, dtype=torch.float32)
+        lower, upper = (at, torch.nextafter(at, torch.tensor(2.0))) if float(at) < border else (torch.nextafter(at, torch.tensor(-1.0)), at)
+        accept_u[b, 2] = lower if b % 2 else upper
+    parents = torch.tensor([-1, 0, 0, 0], dtype=torch.int32)
+    want = verified(logits, None, tokens, parents, accept_u, torch.rand(batch, generator=g), torch.ones(batch))
+    assert [w[0][1] if w[1] > 1 else 0 for w in want] == [2 if b % 2 else 0 for b in range(batch)]
+
+
+@pytest.mark.parametrize("near", [1e-2, 1e-4, 1e-6])
+@pytest.mark.parametrize("vocab", [50, 1003, 40000])
+def test_drafts_near_the_target(near, vocab):
+    """Draft and target differ by so little that a rejection leaves less than f32 sums tell apart; several children are rejected."""
+    g = gen_of(vocab + 1)
+    batch, rows = 24, 7
+    logits = torch.randn((batch, rows, vocab), generator=g) * 2
+    draft = logits + torch.randn((batch, rows, vocab), generator=g) * near
+    tokens = torch.stack([torch.multinomial(torch.softmax(draft[b, 0], 0), rows, replacement=True, generator=g) for b in range(batch)]).to(torch.int32)
+    parents = torch.tensor([-1] + [0] * (rows - 1), dtype=torch.int32)
+    accept_u = torch.full((batch, rows), LAST)
+    accept_u[::3] = 1 - 2.0 ** -10 * torch.rand((len(accept_u[::3]), rows), generator=g)
+    want = verified(logits, draft, tokens, parents, accept_u, torch.rand(batch, generator=g), torch.ones(batch))
+    assert any(n == 1 for _, n, _ in want) and any(n > 1 for _, n, _ in want)
+
+
+def test_drafts_that_are_the_target():
+    """Every drawn child is kept; with random numbers that are none (1 and above) all are rejected, nothing is left, and p stays as it was."""
+    g = gen_of(23)
+    batch, rows, vocab = 6, 5, 5003
+    logits = torch.randn((batch, rows, vocab), generator=g).half()
+    tokens = torch.randint(0, vocab, (batch, rows), generator=g, dtype=torch.int32)
+    parents = torch.tensor([-1, 0, 1, 2, 3], dtype=torch.int32)
+    accept_u, sample_u, heat = torch.full((batch, rows), LAST), torch.rand(batch, generator=g), torch.ones(batch)
+    want = verified(logits, logits.clone(), tokens, parents, accept_u, sample_u, heat)
+    assert all(n == rows for _, n, _ in want)
+    want = verified(logits, logits.clone(), tokens, parents, torch.full((batch, rows), 1.5), sample_u, heat)
+    assert all(n == 1 and t is not None for _, n, t in want)

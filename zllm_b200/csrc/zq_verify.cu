@@ -5,7 +5,8 @@
 //
 // The token drawn at the end is a whole number that a random number picks among a vocabulary's running sums, most of which lie closer
 // together than f32 tells apart (two f32 sums of 128 000 weights disagree about one pick in a hundred): the weights of that pick and their sums
-// are f64, exact to 2e-12 (of the lightest tokens: in f32, see Weights).  A child's test has one border only; while none was rejected at a row, its sums are f32 inside a thread.
+// are f64, exact to 2e-12 (of the lightest tokens: in f32, see Weights).  A child's test has one border only: its sums are f32 inside a thread, and a test that lies
+// within their error of its border, some one in ten thousand, is decided by the f64 pass, as is whether a rejection left anything.
 //
 // Only rows on the walk are read, so the work is latency more than bytes: a cluster of CTAs per sequence shares a row (each CTA a
 // run of the vocabulary) and walks in step: all CTAs exchange their sums through distributed shared memory, one barrier each time, and come to
@@ -36,8 +37,14 @@ struct VerifyArgs {
     const float *accept_u, *sample_u, *temperature;
     int32_t *path, *accepted, *token;
     int vocab, rows, shared_parents, segments;  // segments of a CTA
+    float border;  // how far f32's sums may be off, relative to themselves (first_error)
     uint32_t *status;
 };
+
+// What the f32 sums of a row, and of what a rejection leaves, are off by, at most: ex2.approx by 2^-22, its argument, of up to 100, by three roundings, 100 x 3 x
+// 2^-24 ln 2 = 2^-16.3, and a thread adds four weights of a segment to each of two sums, half a step each. With p, q, the factors m and the sums Z
+// off by that much (m and Z of the k-th rejection by 2 (k + 1) as much: m + Z moves by no more than m does), both sides of a child's test differ from the exact ones by less than this times (2 k + 2) q + p.
+static float first_error(int segments) { return 1.f / (1 << 15) + (float)segments / (1 << 25); }
 
 // A row's largest logit (NaN if the row holds one; where its place is not asked for, one that is not far below), its first place, and the sum of its weights
 // relative to it.
@@ -57,6 +64,7 @@ struct VerifyShared {
     int32_t gone[kMaxDraftRows];      // rejected tokens at this row (chosen children)
     int32_t parent[kMaxDraftRows], token[kMaxDraftRows];
     float u[kMaxDraftRows];
+    double roots[32];
     alignas(16) float2 list[kVerifyWarps][kSegment];
 };
 constexpr size_t kSegmentBytes = (227 << 10) - (sizeof(VerifyShared) + 1023) / 1024 * 1024;  // room for the sums of a CTA's segments
@@ -102,8 +110,8 @@ __device__ __forceinline__ double warp_sum(double x) {
     return x;
 }
 
-// 2^((l - top) c) to 2e-12 of itself: 2^(n + j / 32 + r), |r| <= 1 / 64, with 2^(j / 32) from lane j of the warp and a Taylor sum of degree 4 for
-// 2^r; 11 f64 operations.  Below `low` (2^-900 of the largest) it is 0.  All lanes of the warp call it.
+// 2^((l - top) c) to 2e-12 of itself: 2^(n + j / 32 + r), |r| <= 1 / 64, with 2^(j / 32) from a table and a Taylor sum of degree 4 for
+// 2^r; 11 f64 operations.  Below `low` (2^-900 of the largest) it is 0.
 //
 // light(): the same in f32, the argument to twice f32's bits, off by 2^-21 of the weight.  Of weights below 2^-18 of the largest that is
 // 2^-39 each, and of either sign: 128 000 of them move a running sum by less than 1e-9 of a border's usual distance.
@@ -121,14 +129,14 @@ struct Weights {
         low = fmaxf((float)(top - gap), -3.4028235e38f);
         top32 = largest;
     }
-    __device__ __forceinline__ bool heavy(float l) const { return (l - top32) * c_hi > kHeavy; }
+    __device__ __forceinline__ bool heavy(float l, float from) const { return (l - top32) * c_hi > from; }
     __device__ __forceinline__ float light(float l) const {
         const float d = fmaxf(l - top32, least), y = d * c_hi;
         float w = ex2(y);
         w = fmaf(w * 0.69314718f, fmaf(d, c_lo, fmaf(d, c_hi, -y)), w);
         return l == -INFINITY ? 0.f : w;
     }
-    __device__ __forceinline__ double operator()(float l, double root) const {
+    __device__ __forceinline__ double operator()(float l, const double *roots) const {
         constexpr double kMagic = 6755399441055744.0 / 32;  // 1.5 * 2^52 / 32: adding it leaves the number of 32nds in the low bits
         const bool none = !(l >= low);
         const double y = none ? 0.0 : ((double)l - top) * c;
@@ -139,7 +147,7 @@ struct Weights {
         s = fma(r, s, 2.402265069591007e-1);
         s = fma(r, s, 6.931471805599453e-1);
         s = fma(r, s, 1.0);
-        s *= __shfl_sync(0xffffffffu, root, k & 31);
+        s *= roots[k & 31];
         s = __hiloint2double(__double2hiint(s) + ((k >> 5) << 20), __double2loint(s));
         return none ? 0.0 : s;
     }
@@ -203,7 +211,9 @@ __device__ __noinline__ void exchange_sums(VerifyShared &s, int parity, int n) {
     cluster.sync();
 }
 
-template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) verify_draft_kernel(const VerifyArgs a) {
+// DRAWN: children were drawn from the draft's distributions. (A constant: with a condition in its place, nvcc 12.9 took the way behind the children's loop for a sequence of
+// chosen ones, whatever the condition.)
+template <class T, bool DRAWN> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) verify_draft_kernel(const VerifyArgs a) {
     pdl_launch_dependents();
     extern __shared__ double s_seg[];  // sums of this CTA's segments, then their slopes
     __shared__ VerifyShared s;
@@ -211,7 +221,8 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
     cluster.barrier_arrive();  // this CTA runs: peers wait for it before they store into this CTA
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), seq = blockIdx.x / ctas;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const double root = exp2(lane / 32.0);
+    if (tid < 32) s.roots[tid] = exp2(tid / 32.0);
+    const double *root = s.roots;
     pdl_wait_prior_grid();
     const int n = draft_len(a.lens, seq, a.rows, a.status);
     const size_t row0 = (size_t)seq * a.rows;
@@ -223,7 +234,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
     }
     __syncthreads();
     cluster.barrier_wait();  // all CTAs run, and have done so since before the tables were read
-    const bool greedy = heat == 0.f, drawn = a.draft != nullptr && !greedy;
+    const bool greedy = heat == 0.f;
     const double scale = 1.4426950408889634074 / (greedy ? 1.0 : (double)heat);
     const float scale32 = (float)fmin(scale, 1e30);
     const int first = rank * a.segments, last = first + a.segments;
@@ -375,7 +386,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
         }
     };
     // Sums of the segments of the target's weights, without rejected tokens.
-    auto row_segments = [&] {
+    auto row_segments = [&](float from) {
         double mine = 0;
 #pragma unroll 1
         for (int g = first + warp; g < last; g += kVerifyWarps) {
@@ -385,7 +396,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             unsigned heavies = 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const bool h = pw.heavy(l[e]);
+                const bool h = pw.heavy(l[e], from);
                 if (h) heavies |= 1u << e;
                 some += h ? 0.f : pw.light(l[e]);
             }
@@ -408,7 +419,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
         exchange_sums(s, parity ^= 1, 1);
     };
     // Sums over both rows: of p's weights and q's, and at factors c0 and c1 of (p - c q)+ and of the q in it, at c1 kept for every segment.
-    auto both_segments = [&](double c0, double c1) {
+    auto both_segments = [&](double c0, double c1, float from) {
         const float f0 = (float)c0, f1 = (float)c1;
         double all[kSums] = {0, 0, 0, 0, 0, 0};
 #pragma unroll 1
@@ -419,7 +430,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             unsigned heavies = 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const bool h = pw.heavy(l[e]) || qw.heavy(ql[e]);
+                const bool h = pw.heavy(l[e], from) || qw.heavy(ql[e], from);
                 if (h) heavies |= 1u << e;
                 const float p = h ? 0.f : pw.light(l[e]), q = h ? 0.f : qw.light(ql[e]), r0 = fmaf(-f0, q, p), r1 = fmaf(-f1, q, p);
                 some[0] += p;
@@ -491,6 +502,12 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
         return total_of(0);
     };
 
+    auto note = [&](auto &list, int at, auto value) {
+        __syncthreads();
+        if (tid == 0) list[at] = value;
+        __syncthreads();
+    };
+
     if (n > 0 && !bad) {
         count = 1;
         if (rank == 0 && tid == 0) a.path[row0] = 0;
@@ -499,7 +516,7 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
             n_gone = 0;
             const int child = child_from(node + 1);
-            const bool use_q = drawn && child >= 0;
+            const bool use_q = DRAWN && !greedy && child >= 0;
             if (use_q) {
                 qrow = reinterpret_cast<const T *>(a.draft) + (row0 + node) * a.vocab;
                 q_wide = ((reinterpret_cast<uintptr_t>(qrow) ^ reinterpret_cast<uintptr_t>(row)) & 15) == 0;
@@ -516,53 +533,134 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             int32_t best;
             bad = !joined(use_q, best);
             if (bad) break;
+            int sum_at = 0;              // place of the segments' sum among the last pass's sums
 
-            // ---- its children
+            // ---- its children, in f32's sums until one is kept, none is left, or one lies within these sums' error of a border; then in 64 bits
             int next = -1;
             int rejected = 0;         // drawn children that left something: p is (p - m q)+ / rest
             double m = 0, rest = 1;
             double gone = 0;          // what the rejected chosen children had of p
-            for (int j = child; j >= 0; j = child_from(j + 1)) {
-                const int t = s.token[j];
-                if (t < 0 || t >= a.vocab) {
-                    if (tid == 0 && rank == 0) atomicMax(a.status, (uint32_t)kStatusBadIndex);
-                    continue;
-                }
-                if (greedy) {
-                    if (t == best) next = j;
-                    if (next >= 0) break;
-                    continue;
-                }
-                const double u = (double)s.u[j], p = pw(logit(row, t), root) * p_inv;
-                if (drawn) {
-                    const double q = qw(logit(qrow, t), root) * q_inv;
-                    if (u * q * rest < fmax(p - m * q, 0.0)) {
-                        next = j;
-                        break;
+            double factor = 0, off = 0;  // what is left: w_p - factor w_q; off: the exact factor less the one that the segments are taken at
+            bool seen = false;        // child j has failed its test in 64 bits
+            for (int j = child;;) {
+                enum { kToken, kChild, kRest } ask = kToken;  // what the sums in 64 bits are for
+                for (; j >= 0; j = child_from(j + 1)) {
+                    const int t = s.token[j];
+                    if (t < 0 || t >= a.vocab) {
+                        if (tid == 0 && rank == 0) atomicMax(a.status, (uint32_t)kStatusBadIndex);
+                        continue;
                     }
-                    const double sum = light_rest(m + rest);
-                    if (sum > 0) {  // else nothing is left: p stays as it was
+                    if (greedy) {
+                        if (t == best) next = j;
+                        if (next >= 0) break;
+                        continue;
+                    }
+                    const double u = (double)s.u[j], p = pw(logit(row, t), root) * p_inv;
+                    if constexpr (DRAWN) {
+                        if (!seen) {
+                            const double q = qw(logit(qrow, t), root) * q_inv, bound = u * q * rest, of = p - m * q;
+                            if (p > 0 && fabs(bound - of) <= (double)a.border * ((2 * rejected + 2) * q + p)) {
+                                ask = kChild;
+                                break;
+                            }
+                            if (bound < fmax(of, 0.0)) {
+                                next = j;
+                                break;
+                            }
+                        }
+                        seen = false;
                         m += rest;
-                        rest = sum;
-                        __syncthreads();
-                        if (tid == 0) s.m[rejected] = m;
-                        __syncthreads();
-                        ++rejected;
+                        rest = light_rest(m);
+                        note(s.m, rejected++, m);
+                        if (!(rest > (double)a.border * (rejected + 1))) {
+                            ask = kRest;
+                            break;
+                        }
+                    } else {
+                        bool again = false;
+                        for (int i = 0; i < n_gone; ++i) again |= s.gone[i] == t;
+                        if (again) continue;  // nothing of it is left
+                        const double bound = u * (1.0 - gone), near = (double)a.border * (p + gone);
+                        const bool close = p > 0 && (fabs(bound - p) <= near || (!(bound < p) && 1.0 - gone - p <= near));
+                        if (!close && bound < p) {
+                            next = j;
+                            break;
+                        }
+                        note(s.gone, n_gone++, t);
+                        if (close) {
+                            ask = kChild;
+                            break;
+                        }
+                        gone += p;
+                    }
+                }
+                if (next >= 0 || greedy) break;
+
+                // ---- the sums in 64 bits; where little is left, of the lightest tokens too
+                const float from = ask == kRest || (DRAWN ? rest : 1.0 - gone) < 1.0 / 64 ? -INFINITY : kHeavy;
+                const bool both = DRAWN && (rejected || ask != kToken);
+                double m_before = 0, rest_before = 1;  // the last rejection
+                factor = off = 0;
+                if (both) {
+                    // where little is left, p and q are near each other and many terms change sign on a step of m: once more from the m of the first time
+                    for (int times = from < kHeavy && rejected ? 2 : 1; times > 0; --times) {
+                        m = 0;
+                        rest = 1;
+                        double sum_p = 0, ratio = 0;
+                        for (int i = 0; i == 0 || i < rejected; i += 2) {
+                            // factors for weights: m times (sum of w_p) / (sum of w_q), as f32 gave them; one rejection counts twice
+                            const double by = q_inv / p_inv, c0 = i < rejected ? s.m[i] * by : 0.0, c1 = i + 1 < rejected ? s.m[i + 1] * by : c0;
+                            both_segments(c0, c1, from);
+                            sum_p = total_of(0);
+                            ratio = sum_p / total_of(1);
+#pragma unroll 1
+                            for (int k = 0; k < 2 && i + k < rejected; ++k) {
+                                m_before = m;
+                                rest_before = rest;
+                                m += rest;
+                                factor = m * ratio;
+                                off = factor - (k ? c1 : c0);
+                                rest = (total_of(2 + 2 * k) - off * total_of(3 + 2 * k)) / sum_p;
+                                note(s.m, i + k, m);
+                            }
+                        }
+                        p_inv = 1.0 / sum_p;
+                        q_inv = ratio * p_inv;
                     }
                 } else {
-                    bool again = false;
-                    for (int i = 0; i < n_gone; ++i) again |= s.gone[i] == t;
-                    if (!again && u * (1.0 - gone) < p) {
-                        next = j;
-                        break;
+                    row_segments(from);
+                }
+                if (ask == kToken) {
+                    sum_at = both ? 4 : 0;
+                    break;
+                }
+                if (ask == kRest) {
+                    if (!(rest > 0)) {  // nothing: p stays as it was
+                        --rejected;
+                        m = m_before;
+                        rest = rest_before;
                     }
-                    if (!again && 1.0 - gone - p > 0) {
-                        __syncthreads();
-                        if (tid == 0) s.gone[n_gone] = t;
-                        gone += p;
-                        ++n_gone;
-                        __syncthreads();
+                    j = child_from(j + 1);
+                    continue;
+                }
+                const double u = (double)s.u[j], w = pw(logit(row, s.token[j]), root);
+                bool yes;
+                if constexpr (DRAWN) {
+                    const double p = w * p_inv, q = qw(logit(qrow, s.token[j]), root) * q_inv;
+                    yes = u * q * rest < fmax(p - m * q, 0.0);
+                    seen = !yes;
+                } else {
+                    const double others = total_of(0);  // u (w + others) < w, also where w is all there is
+                    yes = u * others < (1.0 - u) * w;
+                    if (!yes) {
+                        if (others > 0) gone += w * p_inv;
+                        else --n_gone;  // nothing left: p stays as it was
+                        j = child_from(j + 1);
                     }
+                }
+                if (yes) {
+                    next = j;
+                    break;
                 }
             }
             if (next >= 0) {
@@ -577,32 +675,6 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
             }
 
             // ---- nobody kept: a token from what is left, weights w_p - factor w_q where that is positive
-            double factor = 0, off = 0;  // off: the exact factor less the one that the segments are taken at
-            int sum_at = 0;              // place of the segments' sum among the pass's sums
-            for (int i = 0; i < rejected; i += 2) {
-                // factors for weights: m times (sum of w_p) / (sum of w_q), as f32 gave them; one rejection counts twice
-                const double by = q_inv / p_inv, c0 = s.m[i] * by, c1 = (i + 1 < rejected ? s.m[i + 1] : s.m[i]) * by;
-                both_segments(c0, c1);
-                const double sum_p = total_of(0), ratio = sum_p / total_of(1);
-                if (i == 0) m = 1;
-                factor = m * ratio;
-                off = factor - c0;
-                rest = (total_of(2) - off * total_of(3)) / sum_p;
-                if (i + 1 < rejected) {
-                    m += rest;
-                    factor = m * ratio;
-                    off = factor - c1;
-                    rest = (total_of(4) - off * total_of(5)) / sum_p;
-                }
-                m += rest;  // of the next one
-                sum_at = 4;
-            }
-            if (rejected && !(rest > 0)) rejected = 0;  // nothing left after all
-            if (!rejected) {
-                row_segments();
-                factor = off = 0;
-                sum_at = 0;
-            }
             // a lane has a CTA's part; before: of the CTAs in front
             double part = 0;
             if (lane < ctas) part = sum_at ? fmax(s.sums[parity][4][lane] - off * s.sums[parity][5][lane], 0.0) : s.sums[parity][0][lane];
@@ -661,16 +733,34 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
                     if (lane >= o) incl += up;
                 }
                 double run = at + incl - t;
-                int hit = -1, seen = -1;
+                int hit = -1, last_one = -1;
 #pragma unroll 1
                 for (int e = 0; e < 8; ++e) {
                     const double x = weight[e];
                     run += x;
-                    if (x > 0) seen = e;
+                    if (x > 0) last_one = e;
                     if (hit < 0 && !end && x > 0 && run > target) hit = e;
                 }
-                const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, seen >= 0);
-                if (lane == (hits ? __ffs(hits) - 1 : any ? 31 - __clz(any) : 0)) a.token[seq] = place(first + found) + (hits ? hit : seen);
+                const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, last_one >= 0);
+                if (hits | any) {
+                    if (lane == (hits ? __ffs(hits) - 1 : 31 - __clz(any))) a.token[seq] = place(first + found) + (hits ? hit : last_one);
+                } else {  // the segment's sum was rounding, and so is the choice: its likeliest token
+                    load(row, true, first + found, l);
+                    drop_gone(l, first + found);
+                    RowPart p{-INFINITY, 0x7fffffff, 0.0};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (l[e] > p.top) p.top = l[e], p.at = place(first + found) + e;
+                    for (int o = 16; o > 0; o >>= 1) {
+                        const float top = __shfl_xor_sync(0xffffffffu, p.top, o);
+                        const int32_t at = __shfl_xor_sync(0xffffffffu, p.at, o);
+                        if (top > p.top || (top == p.top && at < p.at)) p.top = top, p.at = at;
+                    }
+                    if (lane == 0) {
+                        if (p.top == -INFINITY) atomicMax(a.status, (uint32_t)kStatusBadIndex);
+                        a.token[seq] = p.top == -INFINITY ? -1 : p.at;
+                    }
+                }
             }
             token = -2;  // written by its owner
             break;
@@ -687,10 +777,10 @@ template <class T> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas
     cluster.sync();  // no CTA leaves while another may still write into its shared memory
 }
 
-template <class T> static int launch_verify(zq_ctx *ctx, VerifyArgs &a, int cluster, size_t batch, size_t smem, zq_error *err) {
-    ZQ_CUDA_CHECK(cudaFuncSetAttribute(verify_draft_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), err);
+template <class T, bool DRAWN> static int launch_verify(zq_ctx *ctx, VerifyArgs &a, int cluster, size_t batch, size_t smem, zq_error *err) {
+    ZQ_CUDA_CHECK(cudaFuncSetAttribute(verify_draft_kernel<T, DRAWN>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), err);
     // the same value every time: calls of other threads set it too
-    ZQ_CUDA_CHECK(cudaFuncSetAttribute(verify_draft_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSegmentBytes), err);
+    ZQ_CUDA_CHECK(cudaFuncSetAttribute(verify_draft_kernel<T, DRAWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSegmentBytes), err);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(batch * cluster));
     cfg.blockDim = dim3(kVerifyThreads);
@@ -704,7 +794,7 @@ template <class T> static int launch_verify(zq_ctx *ctx, VerifyArgs &a, int clus
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->disable_pdl ? 1 : 2;
-    ZQ_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_draft_kernel<T>, a), err);
+    ZQ_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_draft_kernel<T, DRAWN>, a), err);
     ctx->launches++;
     return ZQ_OK;
 }
@@ -746,6 +836,8 @@ extern "C" int zq_verify_draft(zq_ctx *ctx, const void *dev_logits, const void *
     while (bytes(cluster) > kSegmentBytes) cluster *= 2;  // some 3 million tokens a CTA
     static_assert(2 * ((((size_t(1) << 22) + 7) / kSegment + 1) / 2 + 1) * sizeof(double) <= kSegmentBytes, "two CTAs hold the largest vocabulary");
     a.segments = (int)((segments + cluster - 1) / cluster);
+    a.border = first_error(a.segments);
     const size_t smem = bytes(cluster);
-    return dtype == ZQ_F32 ? launch_verify<float>(ctx, a, cluster, batch, smem, err) : dtype == ZQ_F16 ? launch_verify<__half>(ctx, a, cluster, batch, smem, err) : launch_verify<__nv_bfloat16>(ctx, a, cluster, batch, smem, err);
+    if (a.draft) return dtype == ZQ_F32 ? launch_verify<float, true>(ctx, a, cluster, batch, smem, err) : dtype == ZQ_F16 ? launch_verify<__half, true>(ctx, a, cluster, batch, smem, err) : launch_verify<__nv_bfloat16, true>(ctx, a, cluster, batch, smem, err);
+    return dtype == ZQ_F32 ? launch_verify<float, false>(ctx, a, cluster, batch, smem, err) : dtype == ZQ_F16 ? launch_verify<__half, false>(ctx, a, cluster, batch, smem, err) : launch_verify<__nv_bfloat16, false>(ctx, a, cluster, batch, smem, err);
 }
