@@ -206,3 +206,27 @@ def test_drafts_that_are_the_target():
     assert all(n == rows for _, n, _ in want)
     want = verified(logits, logits.clone(), tokens, parents, torch.full((batch, rows), 1.5), sample_u, heat)
     assert all(n == 1 and t is not None for _, n, t in want)
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("row,parent", [(0, 0), (1, -2), (3, 3), (3, 7), (2, 2 ** 31 - 1), (4, -2 ** 31)])
+def test_parents_out_of_range_are_reported_by_verification(drawn, row, parent):
+    from zllm_b200 import ffi
+
+    g = gen_of(29)
+    logits, draft = torch.randn((3, 6, 700), generator=g), torch.randn((3, 6, 700), generator=g)
+    parents = R.trees(g, 3, 6)
+    tokens, accept_u, sample_u = torch.randint(0, 700, (3, 6), generator=g, dtype=torch.int32), torch.rand((3, 6), generator=g) * 0.01, torch.rand(3, generator=g)
+
+    def run(lens):
+        return ctx().verify_draft(logits.cuda(), tokens.cuda(), parents.cuda(), accept_u.cuda(), sample_u.cuda(), torch.ones(3).cuda(), draft_logits=draft.cuda() if drawn else None, draft_lens=ints(*lens))
+
+    parents[1, row] = parent
+    got = run([6, 6, 6])
+    with pytest.raises(ffi.ZqFailure) as e:
+        ctx().sync()
+    assert e.value.code == 5
+    check_verify(got, R.verify(logits, draft if drawn else None, tokens, parents, accept_u, sample_u, torch.ones(3), [6, 6, 6]), 6)
+    got = run([6, row, 6])  # a row of padding is not looked at
+    ctx().sync()
+    check_verify(got, R.verify(logits, draft if drawn else None, tokens, parents, accept_u, sample_u, torch.ones(3), [6, row, 6]), 6)

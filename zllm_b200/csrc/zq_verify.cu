@@ -228,7 +228,9 @@ template <class T, bool DRAWN> __global__ void __launch_bounds__(kVerifyThreads,
     const size_t row0 = (size_t)seq * a.rows;
     const float heat = a.temperature[seq];
     for (int i = tid; i < n; i += kVerifyThreads) {
-        s.parent[i] = a.parents[(a.shared_parents ? 0 : row0) + i];
+        const int up = a.parents[(a.shared_parents ? 0 : row0) + i];
+        if (rank == 0 && (up < -1 || up >= i)) atomicMax(a.status, (uint32_t)kStatusBadIndex);  // such a row hangs below none: it is never tried
+        s.parent[i] = up;
         s.token[i] = a.tokens[row0 + i];
         s.u[i] = a.accept_u[row0 + i];
     }
