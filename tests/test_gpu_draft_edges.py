@@ -230,3 +230,39 @@ def test_parents_out_of_range_are_reported_by_verification(drawn, row, parent):
     got = run([6, row, 6])  # a row of padding is not looked at
     ctx().sync()
     check_verify(got, R.verify(logits, draft if drawn else None, tokens, parents, accept_u, sample_u, torch.ones(3), [6, row, 6]), 6)
+
+
+# ---- caches
+def odd_strides(t, dims):
+    """The same values, with another stride in each of `dims`, which are of size 1."""
+    return t.as_strided(t.shape, [999 if i in dims else s for i, s in enumerate(t.stride())])
+
+
+@pytest.mark.parametrize("pages,page,kv,layers", [(1, 8, 2, 1), (3, 1, 2, 1), (3, 8, 1, 1), (1, 1, 1, 1), (1, 8, 1, 3), (4, 8, 2, 1)])
+def test_strides_of_dimensions_of_one_mean_nothing(pages, page, kv, layers):
+    g = gen_of(31)
+    k, v = (torch.randn((layers, pages, page, kv, 16), generator=g).half().cuda() for _ in range(2))
+    ones = [i for i in range(5) if k.shape[i] == 1]
+    table, context = torch.arange(pages, dtype=torch.int32).reshape(1, pages).cuda(), ints(0)
+    q = torch.randn((1, 1, 2 * kv, 16), generator=g).half().cuda()
+    odd, inner = odd_strides(v, ones), [i - 1 for i in ones if i > 0]
+    got = ctx().tree_attention(q, k[0], odd_strides(v[0], inner), table, context)
+    want = ctx().tree_attention(q, k[0], v[0], table, context)
+    ctx().sync()
+    assert torch.equal(got, want)
+    if pages * page > 2:
+        want_k, want_v = k.clone(), v.clone()
+        want_k.view(layers, -1, kv, 16)[:, 1], want_v.view(layers, -1, kv, 16)[:, 1] = k.view(layers, -1, kv, 16)[:, 2], v.view(layers, -1, kv, 16)[:, 2]
+        ctx().cache_keep_path(k, odd, table, context, ints(0, 2, -1).reshape(1, 3), ints(2))
+        ctx().sync()
+        assert torch.equal(k, want_k) and torch.equal(v, want_v)
+
+
+def test_caches_of_unlike_strides_are_refused():
+    from zllm_b200 import ffi
+
+    k = torch.zeros((4, 8, 2, 16), dtype=torch.float16, device="cuda")
+    v = torch.zeros((8, 8, 2, 16), dtype=torch.float16, device="cuda")[::2]
+    with pytest.raises(ffi.ZqFailure) as e:
+        ctx().tree_attention(torch.zeros((1, 1, 2, 16), dtype=torch.float16, device="cuda"), k, v, ints(0).reshape(1, 1), ints(0))
+    assert e.value.code == 1

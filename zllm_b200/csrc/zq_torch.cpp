@@ -494,7 +494,9 @@ Cache cache_of(PyObject *k, PyObject *v, PyObject *blocks, PyObject *lens, int d
     const int64_t n = s.k.dim();
     if (n != 4 && !(layers && n == 5)) fail(1, "k_pages of shape " + sizes_of(s.k) + ": [pages, page_size, heads, head_dim] is needed" + (layers ? ", or that behind a dimension of layers" : ""));
     if (s.k.scalar_type() != s.v.scalar_type()) type_error("k_pages is " + dtype_name(s.k.scalar_type()) + " and v_pages " + dtype_name(s.v.scalar_type()));
-    if (s.k.sizes() != s.v.sizes() || s.k.strides() != s.v.strides()) fail(1, "k_pages and v_pages differ in shape or strides: " + sizes_of(s.k) + ", " + sizes_of(s.v));
+    bool alike = s.k.sizes() == s.v.sizes();
+    for (int64_t i = 0; alike && i < n; ++i) alike = s.k.size(i) == 1 || s.k.stride(i) == s.v.stride(i);  // a dimension of one has any stride
+    if (!alike) fail(1, "k_pages and v_pages differ in shape or strides: " + sizes_of(s.k) + ", " + sizes_of(s.v));
     if (s.k.numel() == 0) fail(1, "k_pages of shape " + sizes_of(s.k) + " is empty");
     const int64_t heads = s.k.size(n - 2), dim = s.k.size(n - 1), size = s.k.size(n - 3);
     if ((dim > 1 && s.k.stride(n - 1) != 1) || (heads > 1 && s.k.stride(n - 2) != dim) || (size > 1 && s.k.stride(n - 3) != heads * dim)) fail(1, "a page of the cache is not dense");
