@@ -22,3 +22,16 @@ def test_verification_stores_into_ctas_that_run():
     assert arrive < wait < first
     assert kernel[:arrive].count("{") - kernel[:arrive].count("}") == 1 and kernel[:wait].count("{") - kernel[:wait].count("}") == 1  # in the body itself
     assert "return" not in kernel[:wait]
+
+
+def test_sums_in_tensor_memory_are_stored_before_they_are_loaded_again():
+    """tcgen05.st and a later tcgen05.ld of the same columns: only tcgen05.wait::st between them orders the two.  Each row of V with an infinity adds to the same sums."""
+    text = _source("zq_attn_wide.cu")
+    loop = text[text.index("for (int r = 0; r < kWideTile; ++r) {"):]
+    depth, end = 0, 0
+    for end, c in enumerate(loop):
+        depth += (c == "{") - (c == "}")
+        if c == "}" and depth == 0:
+            break
+    body = loop[:end]
+    assert body.index("tm_ld32(t_o") < body.index("tm_st32(t_o") < body.index("tm_st_wait();")

@@ -6,7 +6,7 @@ import torch
 
 from tests import draft_ref as R
 from tests.gpu_util import ctx
-from tests.test_gpu_draft import check_verify, gen_of, ints, make_cache
+from tests.test_gpu_draft import check_verify, gen_of, ints, make_cache, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -266,3 +266,31 @@ def test_caches_of_unlike_strides_are_refused():
     with pytest.raises(ffi.ZqFailure) as e:
         ctx().tree_attention(torch.zeros((1, 1, 2, 16), dtype=torch.float16, device="cuda"), k, v, ints(0).reshape(1, 1), ints(0))
     assert e.value.code == 1
+
+
+# ---- attention
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,group,dim", [(12, 4, 64), (20, 2, 128), (40, 4, 64), (70, 4, 128), (66, 4, 72)])
+def test_several_visible_infinities_of_a_tile(dtype, rows, group, dim):
+    """A chain whose drafted keys hold an infinity each, in a column of their own: a row has those of all rows up to itself, in 16-row, 128-row and 256-row tiles."""
+    g = gen_of(37)
+    k_pages, v_pages, table = make_cache(g, 1, 2, dim, 16, 8, dtype)
+    q = torch.randn((1, rows, 2 * group, dim), generator=g).to(dtype).cuda()
+    context, bad = 19, {2: (7, math.inf), 3: (30, -math.inf), 4: (7, math.inf), 5: (31, math.inf), 9: (0, -math.inf), 10: (dim - 1, math.inf)}
+    for i, (column, value) in bad.items():
+        b, o = R.cache_row(table[0].cpu(), 16, context + i)
+        v_pages[b, o, :, column] = value
+    got = ctx().tree_attention(q, k_pages, v_pages, table, ints(context))
+    ctx().sync()
+    want = torch.zeros((rows, dim))
+    for i, (column, value) in bad.items():
+        want[i:, column] = value
+    want = want.cuda().reshape(1, rows, 1, dim).expand_as(got)
+    assert torch.equal(torch.where(torch.isfinite(got), 0.0, got.float()), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [72, 88, 104, 112, 120])
+@pytest.mark.parametrize("rows,group", [(9, 4), (40, 2), (70, 4)])
+def test_attention_of_heads_between_the_tiles_sizes(dtype, dim, rows, group):
+    run_attention(gen_of(dim + rows), 2, rows, 2 * group, 2, dim, 16, [37, 300], dtype, tree=True, drafted=[rows, rows - 3])

@@ -557,8 +557,8 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                                 }
                                 tm_st32(t_o + 32 * c, x);
                             }
+                            tm_st_wait();  // the next such row of V loads what this one has stored
                         }
-                        tm_st_wait();
                     }
                     asm volatile("bar.sync %0, %1;" ::"r"(PAIR ? 1 : 2 + s), "n"(PAIR ? 2 * kWideTile : kWideTile) : "memory");
                 }
