@@ -289,8 +289,58 @@ def test_several_visible_infinities_of_a_tile(dtype, rows, group, dim):
     assert torch.equal(torch.where(torch.isfinite(got), 0.0, got.float()), want)
 
 
+@pytest.mark.parametrize("rows,group,dim,page", [(66, 4, 64, 16), (66, 4, 128, 16), (70, 8, 72, 32), (40, 2, 104, 8), (6, 1, 72, 16), (20, 4, 128, 128)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf])
+def test_what_rows_of_large_tiles_do_not_see_does_not_reach_them(dtype, rows, group, dim, page, poison):
+    """Masked drafted rows, rows of padding, the ends of pages and pages of nobody hold infinities and NaN; three rows see one each, of which two are neighbours in a tile."""
+    g = gen_of(41)
+    kv, context = 2, 101
+    k_pages, v_pages, table = make_cache(g, 1, kv, dim, page, -(-(context + rows) // page) + 1, dtype)
+    q = torch.randn((1, rows, group * kv, dim), generator=g).to(dtype).cuda()
+    parents, n = torch.tensor([[-1] + [0] * (rows - 1)], dtype=torch.int32), rows - 1
+    _, sees = R.tree(parents, [context], [n])
+    mask = R.words(sees).cuda()
+    clean = ctx().tree_attention(q, k_pages, v_pages, table, ints(context), mask=mask, draft_lens=ints(n))
+    hit = sorted({2, 3, n - 1})
+    for pages in (k_pages, v_pages):
+        flat = pages.view(-1, kv, dim)
+        used = torch.zeros(flat.shape[0], dtype=torch.bool)
+        for p in range(context + n):
+            b, o = R.cache_row(table[0].cpu(), page, p)
+            used[b * page + o] = True
+        flat[~used.cuda()] = poison
+        for i in hit:
+            b, o = R.cache_row(table[0].cpu(), page, context + i)
+            pages[b, o] = poison
+    got = ctx().tree_attention(q, k_pages, v_pages, table, ints(context), mask=mask, draft_lens=ints(n))
+    ctx().sync()
+    others = [i for i in range(rows) if i not in hit]
+    assert torch.equal(got[:, others], clean[:, others]) and torch.isfinite(got[:, others]).all()
+    assert not torch.isfinite(got[:, hit]).any()
+    assert (got[:, n:] == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("dim", [72, 88, 104, 112, 120])
 @pytest.mark.parametrize("rows,group", [(9, 4), (40, 2), (70, 4)])
 def test_attention_of_heads_between_the_tiles_sizes(dtype, dim, rows, group):
     run_attention(gen_of(dim + rows), 2, rows, 2 * group, 2, dim, 16, [37, 300], dtype, tree=True, drafted=[rows, rows - 3])
+
+
+@pytest.mark.parametrize("rows,group,dim", [(3, 2, 64), (12, 4, 128), (40, 2, 64), (70, 4, 128), (9, 8, 192)])
+@pytest.mark.parametrize("context", [0, 127, 128, 300])
+def test_a_row_whose_only_visible_score_is_none(rows, group, dim, context):
+    """The last row sees itself alone among the drafted rows, in a share of the keys of which it sees no other, and that score is a NaN: so is the row."""
+    g = gen_of(43)
+    k_pages, v_pages, table = make_cache(g, 1, 1, dim, 16, -(-(context + rows) // 16), torch.bfloat16)
+    q = torch.randn((1, rows, group, dim), generator=g).bfloat16().cuda()
+    mask = torch.zeros((1, rows, -(-rows // 64)), dtype=torch.int64)
+    for i in range(rows):
+        mask[0, i, i // 64] = (1 << (i % 64)) - ((1 << 64) if i % 64 == 63 else 0)
+    clean = ctx().tree_attention(q, k_pages, v_pages, table, ints(context), mask=mask.cuda())
+    b, o = R.cache_row(table[0].cpu(), 16, context + rows - 1)
+    k_pages[b, o, 0, 5] = math.nan
+    got = ctx().tree_attention(q, k_pages, v_pages, table, ints(context), mask=mask.cuda())
+    ctx().sync()
+    assert torch.isnan(got[0, -1]).all() and torch.equal(got[0, :-1], clean[0, :-1])

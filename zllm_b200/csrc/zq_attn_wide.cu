@@ -592,7 +592,8 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                 }
                 __syncwarp();
             };
-            float log_top = top == -INFINITY ? -INFINITY : top * a.scale;
+            // A slot that saw no score but NaN has no largest one and a sum of NaN: it must not be taken for a slot that saw nothing.
+            float log_top = top == -INFINITY ? (PAIR || sum == 0.f ? -INFINITY : NAN) : top * a.scale;
             uint8_t *stage = smem + S::kQ + (PAIR ? s * S::kPlace : (nth & 1) * S::kPlace + s * (S::kPlace / 2));
             uint32_t x[32];
             if (PAIR) {
