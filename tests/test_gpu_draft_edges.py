@@ -344,3 +344,30 @@ def test_a_row_whose_only_visible_score_is_none(rows, group, dim, context):
     got = ctx().tree_attention(q, k_pages, v_pages, table, ints(context), mask=mask.cuda())
     ctx().sync()
     assert torch.isnan(got[0, -1]).all() and torch.equal(got[0, :-1], clean[0, :-1])
+
+
+# few sequences: a row's keys are cut into parts, each relative to its own largest weight; many: they lie in one
+@pytest.mark.parametrize("batch", [1, 300])
+@pytest.mark.parametrize("rows,group,dim,n", [(1, 1, 64, 100000), (1, 8, 128, 70001), (9, 4, 64, 20000), (66, 4, 128, 10000), (3, 2, 192, 10000), (1, 4, 64, 900), (40, 1, 64, 3000)])
+@pytest.mark.parametrize("first", [True, False])
+def test_many_small_weights_in_f16(batch, rows, group, dim, n, first):
+    """One key with a weight of 1 and a value of 0, and n that are alike: weights of 2^-26 and values of 1. Their share is sum / (1 + sum), which f16's smallest step must not take away."""
+    page = 64
+    pages = -(-(n + 1 + rows) // page)
+    k_pages, v_pages = torch.zeros((pages, page, 1, dim), dtype=torch.float16, device="cuda"), torch.ones((pages, page, 1, dim), dtype=torch.float16, device="cuda")
+    score = -18.03125  # exp: 1.478e-8, 2^-26.01
+    k_pages[:, :, 0, 0] = score
+    at = 0 if first else n
+    k_pages[at // page, at % page, 0, 0], v_pages[at // page, at % page] = 0.0, 0.0
+    q = torch.zeros((batch, rows, group, dim), dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    mask = torch.zeros((batch, rows, -(-rows // 64)), dtype=torch.int64, device="cuda")  # the context alone: n + 1 keys
+    table = torch.arange(pages, dtype=torch.int32).cuda().reshape(1, pages).expand(batch, pages)  # of the same pages for all
+    got = ctx().tree_attention(q, k_pages, v_pages, table, ints(*[n + 1] * batch), mask=mask, scale=1.0)
+    ctx().sync()
+    total = n * math.exp(score)
+    want = total / (1 + total)
+    # weights come 2^7 times as large at least, so that each is off by half of f16's smallest step, 2^-25, over 2^7; the result is rounded once, below f16's normal range by 2^-25; a
+    # score has one product, and two roundings of 2^-24 of its 26 on the way to an exponential of 2^-22, in each weight alike
+    bound = n * 2.0 ** -32 + want * (2.0 ** -11 + 2 * 26.02 * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -25
+    assert float((got.double() - want).abs().max()) <= bound < want / 2

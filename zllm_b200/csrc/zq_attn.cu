@@ -232,13 +232,14 @@ template <int D, int WM, bool BF16> __global__ void __launch_bounds__(AttnShape<
                 }
                 top[h] = m;
             }
+            const float from[2] = {base[0] - kUp<BF16, 0>, base[1] - kUp<BF16, 0>};
             uint32_t pf[S::kKeys / 16][4];
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
                 float p[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    p[e] = exp2f(sc[n][e] - base[e >> 1]);
+                    p[e] = exp2f(sc[n][e] - from[e >> 1]);
                     sum[e >> 1] += p[e];
                 }
                 pf[n / 2][(n & 1) * 2] = pack2<BF16>(p[0], p[1]);

@@ -58,6 +58,10 @@ __device__ __forceinline__ uint32_t view32(const AttnArgs &a, int seq, int i, in
     return n <= 0 ? 0u : n >= 32 ? v : v & ((1u << n) - 1);
 }
 
+// The weights are rounded to the cache's type for the second product, whose operands are of one type: by half a step of each, 2^-8 of it in bf16 and 2^-11 in f16; the
+// sum of weights is one of unrounded weights, in f32. Below 2^-14 f16's steps stay as wide as they are there, and below 2^-25 nothing is left, which at 131072 keys can be 0.4 % of
+// a row. Weights in f16 are therefore taken 2^kUp times as large, in the products and in the sum, so that it falls out by itself; before that they are at most 2^MOST.
+template <bool BF16, int MOST> constexpr float kUp = BF16 ? 0.f : 15.f - MOST;
 template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     if (BF16) {
         __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);

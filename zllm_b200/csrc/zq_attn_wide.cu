@@ -25,6 +25,7 @@
 namespace zq {
 
 constexpr int kWideThreads = 320, kWideTile = 128, kBarBytes = 3 << 10;
+constexpr int kRise = 8;  // the largest score may rise by so much, as a power of two of its weight, before the sums follow
 // What the end of an item and the start of the next cost, in tiles of keys: some 10 000 cycles in which the ring stands still (the sums out of tensor memory, the first
 // weights with no product beside them).  40 rows per cache head of 128, 4 cache heads: 64 unequal sequences of up to 200 and 1000, 150 of 900 and 16 of 8000
 // positions take 34.7 / 50.5 / 93 / 48.4 us without it, 28.0 / 41.6 / 74 / 45.4 with 7, 27.9 / 42.5 / 74 / 45.6 with 11.
@@ -413,7 +414,7 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                     // Four chunks of 32 scores, the next one on its way while one is worked on.  The weights are taken relative to the maximum of earlier tiles
                     // and stay in registers until it is clear that this tile's is no more than 2^8 above it.
                     uint32_t p[64];
-                    const uint64_t off2 = twice(-top * a.scale);
+                    const uint64_t off2 = twice(kUp<BF16, kRise> - top * a.scale);
                     float m = -INFINITY;
                     tm_ld32(t_s, za);
 #pragma unroll
@@ -433,7 +434,7 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                             p[16 * c + (e >> 1)] = pack2<BF16>(lo, hi);
                         }
                     }
-                    if (!__any_sync(0xffffffffu, (m - top) * a.scale > 8.f)) {
+                    if (!__any_sync(0xffffffffu, (m - top) * a.scale > kRise)) {
                         tm_st32(t_s, *reinterpret_cast<uint32_t(*)[32]>(p));
                         tm_st32(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
                         done = true;
@@ -456,7 +457,7 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                         hide(c);
                         m = most(m, za);
                     }
-                    const bool rise = top == -INFINITY ? m > top : (m - top) * a.scale > 8.f;
+                    const bool rise = top == -INFINITY ? m > top : (m - top) * a.scale > kRise;
                     const float down = rise && top != -INFINITY ? ex2((top - m) * a.scale) : 1.f;
                     if (__any_sync(0xffffffffu, down != 1.f)) {
                         if (job) wait(kSums + 8 * s, (n_sums - 1) & 1, kStatusMmaTimeout);
@@ -472,7 +473,7 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
                         sum *= down;
                     }
                     if (rise) top = m;
-                    const uint64_t off2 = twice(top == -INFINITY ? 0.f : -top * a.scale);
+                    const uint64_t off2 = twice(top == -INFINITY ? 0.f : kUp<BF16, kRise> - top * a.scale);
                     sums[0] = sums[1] = 0;
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
