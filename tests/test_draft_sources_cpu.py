@@ -35,3 +35,11 @@ def test_sums_in_tensor_memory_are_stored_before_they_are_loaded_again():
             break
     body = loop[:end]
     assert body.index("tm_ld32(t_o") < body.index("tm_st32(t_o") < body.index("tm_st_wait();")
+
+
+def test_tensor_memory_is_given_back_behind_its_last_products():
+    """`wait` returns at once where any wait of the CTA has run out: the one in front of the deallocation must not."""
+    text = _source("zq_attn_wide.cu")
+    end = text[text.index("tc_commit(bars + kEnd)"):text.index("tcgen05.dealloc")]
+    assert "mbar_wait_bounded(&bar.end, 0)" in end and not re.search(r"\bwait\(kEnd", end)
+    assert end.index("mbar_wait_bounded(&bar.end, 0)") < end.index("__syncthreads();")

@@ -345,7 +345,9 @@ template <int D, bool BF16, bool PAIR> __global__ void __launch_bounds__(kWideTh
         }
         if (wide_elect()) tc_commit(bars + kEnd);
         __syncwarp();
-        wait(kEnd, 0, kStatusMmaTimeout);
+        // with a limit of its own, not `wait`: where another wait ran out, MMAs may still be on their way to the tensor memory that is given back below
+        if (!mbar_wait_bounded(&bar.end, 0)) atomicMax(a.status, (uint32_t)kStatusMmaTimeout);
+        __syncwarp();
     } else {
         // ---- scores to weights
         const int s = warp >> 2, row = tid & 127;
