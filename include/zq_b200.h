@@ -309,11 +309,12 @@ typedef struct zq_kv_cache {
 } zq_kv_cache;
 
 /* Angles per position of the rotary_dim / 2 pairs, on the host: base^(-2 i / rotary_dim), divided by `pair_factors[i]` where given (the
- * rope_freqs tensor of a GGUF file), scaled for contexts longer than a model was trained on: ZQ_ROPE_SCALE_LINEAR divides by `factor`,
- * ZQ_ROPE_SCALE_YARN divides pairs that turn less than `beta_slow` times over `original_context` positions by `factor`, keeps those
- * that turn more than `beta_fast` times, and blends linearly in the turns between; *out_factor is what cos and sin are multiplied by
- * (0.1 ln(factor) + 1 for YARN with factor > 1, else 1). */
-enum { ZQ_ROPE_SCALE_NONE = 0, ZQ_ROPE_SCALE_LINEAR = 1, ZQ_ROPE_SCALE_YARN = 2 };
+ * rope_freqs tensor of a GGUF file), scaled for contexts longer than a model was trained on: ZQ_ROPE_SCALE_LINEAR divides by `factor`. The two forms of
+ * YaRN divide pairs that turn less than `beta_slow` times over `original_context` positions by `factor`, keep those that turn more than `beta_fast` times, and blend
+ * between: ZQ_ROPE_SCALE_YARN linearly in the turns, as the method's paper has it; ZQ_ROPE_SCALE_YARN_PAIRS linearly in the pair's number, between the numbers
+ * (rounded outwards) at which a pair turns so often, as the programs do with which models are tuned and run: the form that the YaRN parameters of a model's
+ * files mean. *out_factor is what cos and sin are multiplied by (0.1 ln(factor) + 1 for YaRN with factor > 1, else 1). */
+enum { ZQ_ROPE_SCALE_NONE = 0, ZQ_ROPE_SCALE_LINEAR = 1, ZQ_ROPE_SCALE_YARN = 2, ZQ_ROPE_SCALE_YARN_PAIRS = 3 };
 int zq_rope_frequencies(size_t rotary_dim, double base, int scaling, double factor, double original_context, double beta_slow, double beta_fast, const float *pair_factors, float *out_inv_freq, float *out_factor, zq_error *err);
 
 /* zq_rope_qk with a position of its own for every row and angles from frequencies instead of tables: angle = dev_positions[row] *

@@ -378,7 +378,9 @@ class GgufFile:
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: int = ffi.ROPE_SCALE_NONE, factor: float = 1.0, original_context: float = 0.0, beta_slow: float = 1.0, beta_fast: float = 32.0,
                      pair_factors: Optional[Sequence[float]] = None, device=None):
     """``(inv_freq f32 [rotary_dim / 2], factor)`` for ``rope_rows`` / ``rope_append`` (``zq_rope_frequencies``): plain, linear or
-    YaRN scaling, ``pair_factors`` as a GGUF file's rope_freqs tensor holds them."""
+    YaRN scaling, ``pair_factors`` as a GGUF file's rope_freqs tensor holds them.  The YaRN parameters of a model's files go with ``ffi.ROPE_SCALE_YARN_PAIRS``,
+    whose ramp between kept and divided frequencies is linear in the pair's number; ``ffi.ROPE_SCALE_YARN`` is the ramp of the method's paper, linear in a
+    pair's turns, and gives other angles between the two."""
     half = max(rotary_dim // 2, 1)
     out, by = (C.c_float * half)(), C.c_float()
     if pair_factors is not None and len(pair_factors) != half:

@@ -214,12 +214,19 @@ using namespace zq;
 extern "C" int zq_rope_frequencies(size_t rotary_dim, double base, int scaling, double factor, double original_context, double beta_slow, double beta_fast, const float *pair_factors, float *out_inv_freq, float *out_factor, zq_error *err) {
     if (!out_inv_freq || !out_factor) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: null argument");
     if (rotary_dim == 0 || rotary_dim % 2 || rotary_dim > 4096) return set_error(err, ZQ_ERR_SHAPE, "zq_rope_frequencies: rotary=%zu (rotary must be even and positive)", rotary_dim);
-    if (scaling != ZQ_ROPE_SCALE_NONE && scaling != ZQ_ROPE_SCALE_LINEAR && scaling != ZQ_ROPE_SCALE_YARN) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: unknown scaling %d", scaling);
+    const bool yarn = scaling == ZQ_ROPE_SCALE_YARN || scaling == ZQ_ROPE_SCALE_YARN_PAIRS;
+    if (scaling != ZQ_ROPE_SCALE_NONE && scaling != ZQ_ROPE_SCALE_LINEAR && !yarn) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: unknown scaling %d", scaling);
     if (!(base > 0) || !std::isfinite(base)) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: base %g", base);
     if (scaling != ZQ_ROPE_SCALE_NONE && (!(factor > 0) || !std::isfinite(factor))) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: factor %g", factor);
-    if (scaling == ZQ_ROPE_SCALE_YARN && (!(original_context > 0) || !std::isfinite(original_context) || !(beta_fast > beta_slow) || !std::isfinite(beta_fast) || !std::isfinite(beta_slow)))
+    if (yarn && (!(original_context > 0) || !std::isfinite(original_context) || !(beta_fast > beta_slow) || !std::isfinite(beta_fast) || !std::isfinite(beta_slow)))
         return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: original context %g, turns %g to %g", original_context, beta_slow, beta_fast);
+    if (scaling == ZQ_ROPE_SCALE_YARN_PAIRS && (!(base > 1) || !(beta_slow > 0))) return set_error(err, ZQ_ERR_ARG, "zq_rope_frequencies: base %g, turns from %g: the pairs that turn so often have no number", base, beta_slow);
     const size_t half = rotary_dim / 2;
+    constexpr double kTurn = 6.28318530717958647692;
+    // base^(-i / half) original_context / (2 pi) turns: i from the turns
+    auto number = [&](double turns) { return (double)half * std::log(original_context / (turns * kTurn)) / std::log(base); };
+    auto limited = [&](double i) { return i < 0 ? 0 : i > (double)(rotary_dim - 1) ? (double)(rotary_dim - 1) : i; };
+    const double low = scaling == ZQ_ROPE_SCALE_YARN_PAIRS ? limited(std::floor(number(beta_fast))) : 0, high = scaling == ZQ_ROPE_SCALE_YARN_PAIRS ? limited(std::ceil(number(beta_slow))) : 0;
     for (size_t i = 0; i < half; ++i) {
         double f = std::pow(base, -(double)i / (double)half);
         if (pair_factors) {
@@ -227,15 +234,16 @@ extern "C" int zq_rope_frequencies(size_t rotary_dim, double base, int scaling, 
             f /= (double)pair_factors[i];
         }
         if (scaling == ZQ_ROPE_SCALE_LINEAR) f /= factor;
-        if (scaling == ZQ_ROPE_SCALE_YARN) {
-            const double turns = original_context * f / 6.28318530717958647692;
-            double keep = (turns - beta_slow) / (beta_fast - beta_slow);
+        if (yarn) {
+            double keep;
+            if (scaling == ZQ_ROPE_SCALE_YARN) keep = (original_context * f / kTurn - beta_slow) / (beta_fast - beta_slow);
+            else keep = high > low ? (high - (double)i) / (high - low) : (double)i <= low ? 1 : 0;
             keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
             f = f * keep + f / factor * (1 - keep);
         }
         out_inv_freq[i] = (float)f;
     }
-    *out_factor = scaling == ZQ_ROPE_SCALE_YARN && factor > 1 ? (float)(0.1 * std::log(factor) + 1.0) : 1.f;
+    *out_factor = yarn && factor > 1 ? (float)(0.1 * std::log(factor) + 1.0) : 1.f;
     return ZQ_OK;
 }
 

@@ -15,7 +15,7 @@ Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, IQ4_NL = 2, 8, 12, 13, 14, 20
 Q5_0, Q5_1, Q3_K, IQ4_XS = 6, 7, 11, 23
 F32, F16, BF16 = 0, 1, 2
 JOB_ROW_PARALLEL = 1
-ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_YARN = 0, 1, 2
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_YARN, ROPE_SCALE_YARN_PAIRS = 0, 1, 2, 3
 ROUTE_SOFTMAX, ROUTE_SIGMOID_BIAS, ROUTE_SQRT_SOFTPLUS_BIAS = 0, 1, 2
 MOE_NO_ROUTE = 0xFFFFFFFF  # ZQ_MOE_NO_ROUTE: an expert id that means "no route in this place"
 DIST_HANDLE_BYTES = 80
