@@ -23,10 +23,6 @@
 
 namespace zq {
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool there) {
-    const int n = there ? 16 : 0;  // 0: sixteen zero bytes, nothing is read
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 

@@ -79,6 +79,10 @@ template <bool BF16> __device__ __forceinline__ bool drop_nonfinite(uint32_t &w)
     if (hi) w &= 0x0000ffffu;
     return lo || hi;
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool there) {
+    const int n = there ? 16 : 0;  // 0: sixteen zero bytes, nothing is read
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
 struct Share {
     int64_t first, last, total;  // places of this CTA; of all
     int extra;                   // places of an item behind its units'

@@ -31,10 +31,6 @@ constexpr int kRise = 8;  // the largest score may rise by so much, as a power o
 // positions take 34.7 / 50.5 / 93 / 48.4 us without it, 28.0 / 41.6 / 74 / 45.4 with 7, 27.9 / 42.5 / 74 / 45.6 with 11.
 constexpr int kWideEnd = 7;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool there) {
-    const int n = there ? 16 : 0;  // 0: sixteen zero bytes, nothing is read
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ bool wide_elect() {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
