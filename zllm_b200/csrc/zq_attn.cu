@@ -4,7 +4,8 @@
 //
 // One pass over the keys with a running maximum and sum per row (the sums so far are multiplied down when the maximum rises).  The rows of
 // all query heads that share a head of the cache go through the matrix instructions together (m16n8k16), so that the cache is read once for them. For up to
-// 32 rows per cache head; above, zq_attn_wide.cu takes over where its layout allows. One row each of 64 sequences at 16384 positions streams the cache at 6.6 TB/s.
+// 32 rows per cache head; above, zq_attn_wide.cu takes over where its layout allows (heads of 64 to 128, pages from 8). What it leaves goes through tiles of 64 rows here, each of which
+// reads the cache again: 64 rows of 8 query heads a cache head of 256 over 32000 positions take 689 us, of 128 on the other kernel 76. One row each of 64 sequences at 16384 positions streams the cache at 6.6 TB/s.
 //
 // Work: an item is a (sequence, cache head, tile of rows); its keys are cut into units.  The units of all items, in one line, with a few
 // places behind each item for what its end costs, are dealt to the CTAs (one per SM) in equal shares, so that one long sequence or many unequal ones keep all SMs at work; an item cut by a border is

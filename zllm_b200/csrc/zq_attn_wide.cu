@@ -11,8 +11,8 @@
 // O stays in tensor memory while the largest score rises by less than 2^8: the weights are taken relative to an older maximum (exact in f32,
 // and the sum with them), so that the sums so far are hardly ever multiplied down.
 //
-// Bytes against tensor cycles: a tile of 128 keys of 128 values is 64 KB, 2850 cycles at an SM's share of the memory rate; its products take 1024
-// cycles per slot of rows and its exponentials as many, so up to 256 rows the copies bound it.
+// Bytes against tensor cycles: a tile of 128 keys of 128 values is 64 KB, 1.49 us at an SM's share of the memory rate (2850 cycles at 1.9 GHz, 2400 to 2550 at the 1.6 to
+// 1.7 GHz of long runs); its products take 1024 cycles per slot of rows and its exponentials as many, so up to 256 rows the copies bound it. (ptxas spills 40 to 104 bytes a thread.)
 //
 // Padding and the end of a sequence: boxes are whole pages, and what lies behind the sequence's end must not reach a row (0 * NaN): in tiles that hold
 // drafted rows or the end, a slot's threads clear those rows of V in shared memory, and infinities and NaN of drafted rows, which they

@@ -25,8 +25,9 @@ namespace zq {
 
 namespace cg = cooperative_groups;
 
-// 1024 threads of an SM in four CTAs: each pass waits for memory and for chains of dependent operations more than for issue slots (64 sequences of 128 003
-// tokens take 150 us; with 768 threads 214, with 512 of twice the registers 179).
+// 1024 threads of an SM in four CTAs: each pass waits for memory and for chains of dependent operations more than for issue slots (64 sequences of 13 rows of 128 003
+// tokens, drawn, took 150 us; with 768 threads 214, with 512 of twice the registers 179; with the tests next to a border in f64 152, 137 to 171 by the draw; the kernels of drawn
+// children spill 500 to 660 bytes a thread at 64 registers, in the f64 passes above all).
 constexpr int kVerifyThreads = 256, kVerifyCtas = 4, kVerifyWarps = kVerifyThreads / 32, kMaxCluster = 16, kAhead = 2, kSegment = 256;  // tokens that a warp takes at a time and whose sum is kept
 constexpr float kHeavy = -18.f;  // weights above 2^kHeavy of the largest are evaluated in f64
 constexpr int kSums = 6;         // sums of a pass over both rows: of p, of q; at two m: of what is left, its slope
