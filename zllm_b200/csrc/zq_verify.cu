@@ -112,10 +112,10 @@ __device__ __forceinline__ double warp_sum(double x) {
 }
 
 // 2^((l - top) c) to 2e-12 of itself: 2^(n + j / 32 + r), |r| <= 1 / 64, with 2^(j / 32) from a table and a Taylor sum of degree 4 for
-// 2^r; 11 f64 operations.  Below `low` (2^-900 of the largest) it is 0.
+// 2^r (Tang's table-driven method); 11 f64 operations.  Below `low` (2^-900 of the largest) it is 0.
 //
 // light(): the same in f32, the argument to twice f32's bits, off by 2^-21 of the weight.  Of weights below 2^-18 of the largest that is
-// 2^-39 each, and of either sign: 128 000 of them move a running sum by less than 1e-9 of a border's usual distance.
+// 2^-39 each, and of either sign: 128 000 of them move a running sum by less than 1e-9 of the largest weight, a ten-thousandth of the usual distance between borders.
 struct Weights {
     double c, top;
     float low, c_hi, c_lo, top32, least;
@@ -212,8 +212,8 @@ __device__ __noinline__ void exchange_sums(VerifyShared &s, int parity, int n) {
     cluster.sync();
 }
 
-// DRAWN: children were drawn from the draft's distributions. (A constant: with a condition in its place, nvcc 12.9 took the way behind the children's loop for a sequence of
-// chosen ones, whatever the condition.)
+// DRAWN: children were drawn from the draft's distributions. (A constant: with a condition of the launch in its place, nvcc 12.9 compiled what follows the children's loop as if
+// they had been chosen, whatever the condition was.)
 template <class T, bool DRAWN> __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) verify_draft_kernel(const VerifyArgs a) {
     pdl_launch_dependents();
     extern __shared__ double s_seg[];  // sums of this CTA's segments, then their slopes
